@@ -3,6 +3,8 @@
 // it after validating the operator contract.  Plain C layout only.
 #pragma once
 
+#include <stdint.h>
+
 namespace g950 {
 
 struct RowArgs {
@@ -152,6 +154,83 @@ struct AttnDecArgs {
   int splits;   // key ranges per pair
   int chunk;    // keys per range but the last, which takes the rest (multiple of 16)
   int rows;     // seqlen_q * group
+};
+
+// Appending keys and values to a paged cache (kv_append.hip).  All strides in
+// elements of their view; a row is a token's (or a cache row's) head.
+struct KvAppendArgs {
+  const void* q;            // [tokens, Hq, D]
+  const void* k;            // [tokens, Hkv, D]
+  const void* v;
+  void* q_out;              // rotated queries
+  void* k_out;              // 4 bits: the appended rows as the cache holds them, or null
+  void* v_out;
+  const void* cos;          // [positions, R / 2], fp32 or q's dtype
+  const void* sin;
+  void* k_cache;            // [pages, block_size, Hkv, D] (4 bits: bytes, D / 2)
+  void* v_cache;
+  void* k_scale;            // 4 bits: [pages, block_size, Hkv, 2] scale, offset
+  void* v_scale;
+  const int* cu;            // [B + 1] token row starts
+  const int* used;          // [B] keys of each sequence, the new ones among them
+  const int* table;         // [B, max_pages] physical page per key page
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh, vo_st, vo_sh;
+  long long cos_s, sin_s;   // row strides of the tables
+  long long kc_p, kc_r, kc_h, vc_p, vc_r, vc_h;  // page, row and head strides
+  long long ks_p, ks_r, ks_h, vs_p, vs_r, vs_h;
+  long long table_s;
+  int T, Hq, Hkv, D, R, B;
+  int positions;            // rows of the cos / sin tables
+  int pages, block_size, max_pages;
+  int interleaved;          // pairs (2i, 2i + 1) instead of (i, i + R / 2)
+  int dtype, table_dtype;   // of q / k / v, of cos / sin
+  int int4;
+  int chunks;               // vector kernel: parts a token's heads are dealt over
+};
+
+// Attention over a paged cache of 4-bit rows (attn_int4.hip).
+struct AttnInt4Args {
+  const void* q;            // [T, Hq, D]
+  void* o;
+  float* lse;               // [Hq, T]
+  const uint8_t* k;         // [pages, block_size, Hkv, D / 2]
+  const uint8_t* v;
+  const void* ks;           // [pages, block_size, Hkv, 2] scale, offset
+  const void* vs;
+  const int* cu;            // [B + 1]
+  const int* used;          // [B]
+  const int* table;         // [B, max_pages]
+  long long q_st, q_sh, o_st, o_sh, lse_h, lse_t;
+  long long k_p, k_r, k_h, v_p, v_r, v_h;          // bytes
+  long long ks_p, ks_r, ks_h, vs_p, vs_r, vs_h;    // elements
+  long long table_s;
+  int T, Hq, Hkv, D, B;
+  int pages, block_size, max_pages;
+  float scale_log2;         // scale * log2(e)
+  int left, right;          // window (bottom-right aligned); < 0: unbounded
+  int dtype;
+  int group;                // query heads per KV head
+  int seqlen_q;             // queries per sequence that the grid covers
+  int row_blocks;           // blocks of query rows per (sequence, KV head)
+  int splits, chunk;        // key ranges, keys of all but the last
+  float* part;              // [pairs * row_blocks * splits][rows][D] unnormalised O
+  float* ml;                // [pairs * row_blocks * splits][rows][2] maximum (log2 units), sum
+};
+
+// Norms around a block (block_norm.hip).
+struct BlockNormArgs {
+  const void* x;            // [rows, cols] residual stream
+  const void* h;            // [rows, cols] the block's output
+  const void* w_post;       // [cols] or null: no norm after the block
+  const void* gate;         // [rows, cols] (strides may be 0) or null
+  const void* w_pre;        // [cols] or null: y only
+  void* y;
+  void* n;
+  long long x_row, h_row, g_row, g_col, y_row, n_row;  // elements
+  int rows, cols;
+  int act;                  // of the gate: 0 none, 1 sigmoid, 2 tanh
+  int dtype;
+  float alpha, eps;
 };
 
 }  // namespace g950

@@ -6,3 +6,6 @@
 #include "attention.hip"
 #include "attn_decode.hip"
 #include "dequant.hip"
+#include "kv_append.hip"
+#include "attn_int4.hip"
+#include "block_norm.hip"

@@ -1695,6 +1695,271 @@ int op_flash_varlen(g950_module* m, const g950_view* views, uint32_t nviews, con
   return launch(m, "g950_attn_varlen_general", (unsigned)((rows + 63) / 64), 64u, va, stream);
 }
 
+// ----------------------------------------------------- paged 4-bit / 16-bit KV
+bool no_elements(const View& v) {
+  for (int i = 0; i < v.nd; ++i)
+    if (v.shape[i] == 0) return true;
+  return false;
+}
+
+// An output whose elements share addresses (stride 0 along an extent) has no
+// defined result.
+int distinct(const View& v, const char* op) {
+  for (int i = 0; i < v.nd && !no_elements(v); ++i)
+    if (v.shape[i] > 1 && v.stride[i] == 0)
+      return fail(G950_USAGE, "%s: output %s repeats its elements (stride 0)", op, v.name);
+  return G950_OK;
+}
+
+int last_contiguous(const View& v, const char* op) {
+  if (!no_elements(v) && v.shape[v.nd - 1] > 1 && v.stride[v.nd - 1] != 1)
+    return fail(G950_USAGE, "%s: the last axis of %s must be contiguous", op, v.name);
+  return G950_OK;
+}
+
+// The lists that say where tokens and keys lie: cu_seqlens_q [B + 1],
+// seqused_k [B], page_table [B, max_pages], all int32, rows contiguous.
+int paged_lists(const View& cu, const View& used, const View& table, const char* op) {
+  for (const View* v : {&cu, &used, &table}) {
+    if (v->v->dtype != G950_DTYPE_INT32) return fail(G950_USAGE, "%s: %s must be int32", op, v->name);
+    if (int rc = last_contiguous(*v, op)) return rc;
+  }
+  if (cu.shape[0] < 1 || used.shape[0] != cu.shape[0] - 1 || table.shape[0] != used.shape[0])
+    return fail(G950_USAGE, "%s: cu_seqlens_q_ptr [b + 1], seqused_k_ptr [b] and page_table_ptr [b, pages] disagree on b", op);
+  if (cu.shape[0] > 0x7FFFFFF || table.shape[1] > 0x7FFFFFFF) return fail(G950_USAGE, "%s: extent too large", op);
+  return G950_OK;
+}
+
+// A K or V cache [pages, block_size, heads, `last`] like another one; its last
+// axis contiguous.
+int paged_cache(const View& c, const View& like, long long heads, long long last, uint32_t dt, const char* op) {
+  if (c.v->dtype != dt) return fail(G950_USAGE, "%s: %s must be %s", op, c.name, dtname(dt));
+  if (c.shape[0] != like.shape[0] || c.shape[1] != like.shape[1] || c.shape[2] != heads || c.shape[3] != last)
+    return fail(G950_USAGE, "%s: %s must be [pages, block_size, %lld, %lld] like the other caches", op, c.name, heads, last);
+  if (c.shape[0] > 0x7FFFFFFF || c.shape[1] > 0x7FFFFFFF) return fail(G950_USAGE, "%s: extent too large", op);
+  if (c.shape[1] < 1) return fail(G950_USAGE, "%s: pages of no keys", op);
+  return last_contiguous(c, op);
+}
+
+int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
+                    bool int4, void* stream) {
+  const char* op = int4 ? "paged_append_int4" : "paged_append";
+  if (nviews != (int4 ? 15u : 11u) || nsc != 1)
+    return fail(G950_USAGE, "%s: needs %d views (cos_ptr .. %s) and the scalar interleaved", op, int4 ? 15 : 11,
+                int4 ? "v_scale_ptr" : "v_ptr");
+  View cos, cu, kc, ko, k, ks, table, qo, q, used, sin, vc, vo, v, vs;
+  uint32_t i = 0;
+  auto next = [&](const char* name, int nd, View& w, bool out) { return check_view(views, i++, name, nd, w, out); };
+  if (int rc = next("cos_ptr", 2, cos, false)) return rc;
+  if (int rc = next("cu_seqlens_q_ptr", 1, cu, false)) return rc;
+  if (int rc = next("k_cache_ptr", 4, kc, true)) return rc;
+  if (int4) if (int rc = next("k_out_ptr", 3, ko, true)) return rc;
+  if (int rc = next("k_ptr", 3, k, false)) return rc;
+  if (int4) if (int rc = next("k_scale_ptr", 4, ks, true)) return rc;
+  if (int rc = next("page_table_ptr", 2, table, false)) return rc;
+  if (int rc = next("q_out_ptr", 3, qo, true)) return rc;
+  if (int rc = next("q_ptr", 3, q, false)) return rc;
+  if (int rc = next("seqused_k_ptr", 1, used, false)) return rc;
+  if (int rc = next("sin_ptr", 2, sin, false)) return rc;
+  if (int rc = next("v_cache_ptr", 4, vc, true)) return rc;
+  if (int4) if (int rc = next("v_out_ptr", 3, vo, true)) return rc;
+  if (int rc = next("v_ptr", 3, v, false)) return rc;
+  if (int4) if (int rc = next("v_scale_ptr", 4, vs, true)) return rc;
+  long long interleaved;
+  if (int rc = scalar_int(&sc[0], "interleaved", interleaved)) return rc;
+  const uint32_t dt = k.v->dtype;
+  if (!is_float(dt) || (int4 && !is_float16ish(dt)) || q.v->dtype != dt || v.v->dtype != dt || qo.v->dtype != dt)
+    return fail(G950_USAGE, "%s: q, k, v and q_out must share one dtype (%sbfloat16, float16)", op, int4 ? "" : "float32, ");
+  const long long T = k.shape[0], HK = k.shape[1], D = k.shape[2], H = q.shape[1];
+  if (q.shape[0] != T || q.shape[2] != D || v.shape[0] != T || v.shape[1] != HK || v.shape[2] != D)
+    return fail(G950_USAGE, "%s: q [tokens, h, d], k and v [tokens, hk, d] disagree", op);
+  if (HK < 1 || D < 1 || T > 0x7FFFFFFF || H > 65536 || HK > 65536 || D > 65536)
+    return fail(G950_USAGE, "%s: extent empty or too large", op);
+  if (int4 && (D % 2 || D > 256)) return fail(G950_USAGE, "%s: d must be even and at most 256", op);
+  for (int d = 0; d < 3; ++d)
+    if (qo.shape[d] != q.shape[d]) return fail(G950_USAGE, "%s: q_out_ptr must have q's shape", op);
+  for (const View* w : {&q, &k, &v, &qo, &cos, &sin})
+    if (int rc = last_contiguous(*w, op)) return rc;
+  const long long R = 2 * cos.shape[1];
+  if (sin.shape[0] != cos.shape[0] || sin.shape[1] != cos.shape[1] || sin.v->dtype != cos.v->dtype)
+    return fail(G950_USAGE, "%s: cos_ptr and sin_ptr differ in shape or dtype", op);
+  if (cos.v->dtype != G950_DTYPE_FLOAT32 && cos.v->dtype != dt)
+    return fail(G950_USAGE, "%s: cos_ptr and sin_ptr must be float32 or q's dtype", op);
+  if (R > D) return fail(G950_USAGE, "%s: the tables turn %lld dims, rows have %lld", op, R, D);
+  if (cos.shape[0] > 0x7FFFFFFF) return fail(G950_USAGE, "%s: extent too large", op);
+  if (int rc = paged_lists(cu, used, table, op)) return rc;
+  const uint32_t cdt = int4 ? (uint32_t)G950_DTYPE_UINT8 : dt;
+  if (int rc = paged_cache(kc, kc, HK, int4 ? D / 2 : D, cdt, op)) return rc;
+  if (int rc = paged_cache(vc, kc, HK, int4 ? D / 2 : D, cdt, op)) return rc;
+  for (const View* w : {&qo, &kc, &vc})
+    if (int rc = distinct(*w, op)) return rc;
+  KvAppendArgs a{};
+  if (int4) {
+    for (View* w : {&ks, &vs}) {
+      if (int rc = paged_cache(*w, kc, HK, 2, dt, op)) return rc;
+      if (int rc = distinct(*w, op)) return rc;
+    }
+    for (View* w : {&ko, &vo}) {
+      if (no_elements(*w)) continue;  // not wanted
+      if (w->v->dtype != dt || w->shape[0] != T || w->shape[1] != HK || w->shape[2] != D)
+        return fail(G950_USAGE, "%s: %s must be empty or have k's shape and dtype", op, w->name);
+      if (w->addr() == (w == &ko ? k : v).addr())
+        return fail(G950_USAGE, "%s: %s may not be the input it comes from", op, w->name);
+      if (int rc = last_contiguous(*w, op)) return rc;
+      if (int rc = distinct(*w, op)) return rc;
+    }
+    a.k_out = no_elements(ko) ? nullptr : ko.v->data;
+    a.v_out = no_elements(vo) ? nullptr : vo.v->data;
+    a.ko_st = ko.stride[0]; a.ko_sh = ko.stride[1]; a.vo_st = vo.stride[0]; a.vo_sh = vo.stride[1];
+    a.k_scale = ks.v->data; a.v_scale = vs.v->data;
+    a.ks_p = ks.stride[0]; a.ks_r = ks.stride[1]; a.ks_h = ks.stride[2];
+    a.vs_p = vs.stride[0]; a.vs_r = vs.stride[1]; a.vs_h = vs.stride[2];
+  }
+  a.q = q.v->data; a.k = k.v->data; a.v = v.v->data; a.q_out = qo.v->data;
+  a.cos = cos.v->data; a.sin = sin.v->data; a.k_cache = kc.v->data; a.v_cache = vc.v->data;
+  a.cu = (const int*)cu.v->data; a.used = (const int*)used.v->data; a.table = (const int*)table.v->data;
+  a.q_st = q.stride[0]; a.q_sh = q.stride[1]; a.k_st = k.stride[0]; a.k_sh = k.stride[1];
+  a.v_st = v.stride[0]; a.v_sh = v.stride[1]; a.qo_st = qo.stride[0]; a.qo_sh = qo.stride[1];
+  a.cos_s = cos.stride[0]; a.sin_s = sin.stride[0];
+  a.kc_p = kc.stride[0]; a.kc_r = kc.stride[1]; a.kc_h = kc.stride[2];
+  a.vc_p = vc.stride[0]; a.vc_r = vc.stride[1]; a.vc_h = vc.stride[2];
+  a.table_s = table.stride[0];
+  a.T = (int)T; a.Hq = (int)H; a.Hkv = (int)HK; a.D = (int)D; a.R = (int)R; a.B = (int)used.shape[0];
+  a.positions = (int)cos.shape[0];
+  a.pages = (int)kc.shape[0]; a.block_size = (int)kc.shape[1];
+  a.max_pages = (int)table.shape[1];
+  a.interleaved = interleaved ? 1 : 0;
+  a.dtype = (int)dt; a.table_dtype = (int)cos.v->dtype; a.int4 = int4 ? 1 : 0;
+  const long long rows = a.B ? T * (H + 2 * HK) : 0;
+  return launch(m, "g950_kv_append_general", (unsigned)std::min((rows + 3) / 4, 1ll << 20), 256u, a, stream);
+}
+
+int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
+                            void* stream) {
+  const char* op = "paged_attention_int4";
+  if (nviews != 11 || nsc != 6)
+    return fail(G950_USAGE, "%s: needs 11 views (cu_seqlens_q_ptr .. workspace_ptr) and 6 scalars", op);
+  View cu, k, ks, o, table, q, used, lse, v, vs, ws;
+  const struct { View* w; const char* name; int nd; bool out; } vw[11] = {
+      {&cu, "cu_seqlens_q_ptr", 1, false}, {&k, "k_cache_ptr", 4, false}, {&ks, "k_scale_ptr", 4, false},
+      {&o, "o_ptr", 3, true}, {&table, "page_table_ptr", 2, false}, {&q, "q_ptr", 3, false},
+      {&used, "seqused_k_ptr", 1, false}, {&lse, "softmax_lse_ptr", 2, true}, {&v, "v_cache_ptr", 4, false},
+      {&vs, "v_scale_ptr", 4, false}, {&ws, "workspace_ptr", 1, true}};
+  for (uint32_t i = 0; i < 11; ++i)
+    if (int rc = check_view(views, i, vw[i].name, vw[i].nd, *vw[i].w, vw[i].out)) return rc;
+  long long causal, SK, SQ, left, right;
+  double scale;
+  if (int rc = scalar_int(&sc[0], "is_causal", causal)) return rc;
+  if (int rc = scalar_float(&sc[1], "scale_softmax", scale)) return rc;
+  if (int rc = scalar_int(&sc[2], "seqlen_k", SK)) return rc;
+  if (int rc = scalar_int(&sc[3], "seqlen_q", SQ)) return rc;
+  if (int rc = scalar_int(&sc[4], "window_size_left", left)) return rc;
+  if (int rc = scalar_int(&sc[5], "window_size_right", right)) return rc;
+  const uint32_t dt = q.v->dtype;
+  if (!is_float16ish(dt) || o.v->dtype != dt) return fail(G950_USAGE, "%s: q and o must share one dtype (bfloat16, float16)", op);
+  const long long T = q.shape[0], H = q.shape[1], D = q.shape[2], HK = k.shape[2];
+  if (HK < 1 || H < 1 || H % HK) return fail(G950_USAGE, "%s: %lld query heads on %lld KV heads", op, H, HK);
+  if (D < 2 || D % 2 || D > 256) return fail(G950_USAGE, "%s: d must be even and at most 256", op);
+  if (T > 0x7FFFFFFF || H > 65536) return fail(G950_USAGE, "%s: extent too large", op);
+  if (SQ < 0 || SK < 0 || SQ > 0x7FFFFFF || SK > 0x7FFFFFFF) return fail(G950_USAGE, "%s: seqlen_q / seqlen_k out of range", op);
+  if (!std::isfinite(scale)) return fail(G950_USAGE, "%s: scale_softmax must be finite", op);
+  for (int d = 0; d < 3; ++d)
+    if (o.shape[d] != q.shape[d]) return fail(G950_USAGE, "%s: o_ptr must have q's shape", op);
+  if (lse.v->dtype != G950_DTYPE_FLOAT32 || lse.shape[0] != H || lse.shape[1] != T)
+    return fail(G950_USAGE, "%s: softmax_lse_ptr must be float32 [h, tokens]", op);
+  if (int rc = last_contiguous(q, op)) return rc;
+  if (int rc = last_contiguous(o, op)) return rc;
+  if (int rc = paged_lists(cu, used, table, op)) return rc;
+  if (int rc = paged_cache(k, k, HK, D / 2, G950_DTYPE_UINT8, op)) return rc;
+  if (int rc = paged_cache(v, k, HK, D / 2, G950_DTYPE_UINT8, op)) return rc;
+  if (int rc = paged_cache(ks, k, HK, 2, dt, op)) return rc;
+  if (int rc = paged_cache(vs, k, HK, 2, dt, op)) return rc;
+  if (int rc = distinct(o, op)) return rc;
+  if (int rc = distinct(lse, op)) return rc;
+  if (ws.v->dtype != G950_DTYPE_FLOAT32) return fail(G950_USAGE, "%s: workspace_ptr must be float32", op);
+  if (int rc = last_contiguous(ws, op)) return rc;
+  AttnInt4Args a{};
+  a.q = q.v->data; a.o = o.v->data; a.lse = (float*)lse.v->data;
+  a.k = (const uint8_t*)k.v->data; a.v = (const uint8_t*)v.v->data; a.ks = ks.v->data; a.vs = vs.v->data;
+  a.cu = (const int*)cu.v->data; a.used = (const int*)used.v->data; a.table = (const int*)table.v->data;
+  a.q_st = q.stride[0]; a.q_sh = q.stride[1]; a.o_st = o.stride[0]; a.o_sh = o.stride[1];
+  a.lse_h = lse.stride[0]; a.lse_t = lse.stride[1];
+  a.k_p = k.stride[0]; a.k_r = k.stride[1]; a.k_h = k.stride[2];
+  a.v_p = v.stride[0]; a.v_r = v.stride[1]; a.v_h = v.stride[2];
+  a.ks_p = ks.stride[0]; a.ks_r = ks.stride[1]; a.ks_h = ks.stride[2];
+  a.vs_p = vs.stride[0]; a.vs_r = vs.stride[1]; a.vs_h = vs.stride[2];
+  a.table_s = table.stride[0];
+  a.T = (int)T; a.Hq = (int)H; a.Hkv = (int)HK; a.D = (int)D; a.B = (int)used.shape[0];
+  a.pages = (int)k.shape[0]; a.block_size = (int)k.shape[1]; a.max_pages = (int)table.shape[1];
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  auto limit = [](long long w) { return w < 0 ? -1 : (int)std::min(w, 0x7FFFFFFFll); };
+  a.left = limit(left);
+  a.right = causal ? 0 : limit(right);
+  a.dtype = (int)dt; a.group = (int)(H / HK); a.seqlen_q = (int)SQ;
+  const long long rows = a.B && SQ ? T * H : 0;
+  if (rows > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+  return launch(m, "g950_attn_int4_general", (unsigned)rows, 64u, a, stream);
+}
+
+// --------------------------------------------------- norms around a block
+int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
+                  void* stream) {
+  if (nviews != 7 || nsc != 3)
+    return fail(G950_USAGE, "block_norm: needs views (G, H, N, W_post, W_pre, X, Y), scalars (eps, gate_act, residual_scale)");
+  View g, h, n, wo, wi, x, y;
+  if (int rc = check_view(views, 0, "G", 2, g, false)) return rc;
+  if (int rc = check_view(views, 1, "H", 2, h, false)) return rc;
+  if (int rc = check_view(views, 2, "N", 2, n, true)) return rc;
+  if (int rc = check_view(views, 3, "W_post", 1, wo, false)) return rc;
+  if (int rc = check_view(views, 4, "W_pre", 1, wi, false)) return rc;
+  if (int rc = check_view(views, 5, "X", 2, x, false)) return rc;
+  if (int rc = check_view(views, 6, "Y", 2, y, true)) return rc;
+  auto rows_as_x = [&](const View& w) {
+    if (!is_float(x.v->dtype) || w.v->dtype != x.v->dtype)
+      return fail(G950_USAGE, "block_norm: X/%s dtypes %s/%s unsupported (float32, bfloat16, float16, same)", w.name,
+                  dtname(x.v->dtype), dtname(w.v->dtype));
+    if (w.shape[0] != x.shape[0] || w.shape[1] != x.shape[1]) return fail(G950_USAGE, "block_norm: X and %s shapes differ", w.name);
+    return last_contiguous(w, "block_norm");
+  };
+  for (const View* w : {&x, &h, &y})
+    if (int rc = rows_as_x(*w)) return rc;
+  if (x.shape[0] > 0x7FFFFFFF || x.shape[1] > 0x7FFFFFFF) return fail(G950_USAGE, "block_norm: extent too large");
+  double eps, alpha;
+  long long act;
+  if (int rc = scalar_float(&sc[0], "eps", eps)) return rc;
+  if (int rc = scalar_int(&sc[1], "gate_act", act)) return rc;
+  if (int rc = scalar_float(&sc[2], "residual_scale", alpha)) return rc;
+  if (act < 0 || act > 2) return fail(G950_USAGE, "block_norm: gate_act %lld (0 none, 1 sigmoid, 2 tanh)", act);
+  const long long cols = x.shape[1];
+  if (cols == 0) return fail(G950_USAGE, "block_norm: empty row");
+  // absent parts are empty views
+  const bool post = wo.shape[0] != 0, pre = wi.shape[0] != 0, gate = !no_elements(g);
+  if (post) if (int rc = param_view(wo, x, "block_norm: W_post")) return rc;
+  if (pre) {
+    if (int rc = param_view(wi, x, "block_norm: W_pre")) return rc;
+    if (int rc = rows_as_x(n)) return rc;
+    if (int rc = distinct(n, "block_norm")) return rc;
+  } else if (!no_elements(n)) {
+    return fail(G950_USAGE, "block_norm: N without W_pre");
+  }
+  if (gate && (g.v->dtype != x.v->dtype || g.shape[0] != x.shape[0] || g.shape[1] != cols))
+    return fail(G950_USAGE, "block_norm: G must have X's shape (strides may be 0) and dtype");
+  if (!gate && act) return fail(G950_USAGE, "block_norm: gate_act without G");
+  if (int rc = distinct(y, "block_norm")) return rc;
+  BlockNormArgs a{};
+  a.x = x.v->data; a.h = h.v->data; a.y = y.v->data;
+  a.w_post = post ? wo.v->data : nullptr;
+  a.w_pre = pre ? wi.v->data : nullptr;
+  a.n = pre ? n.v->data : nullptr;
+  a.gate = gate ? g.v->data : nullptr;
+  a.x_row = x.stride[0]; a.h_row = h.stride[0]; a.y_row = y.stride[0]; a.n_row = n.stride[0];
+  a.g_row = g.stride[0]; a.g_col = g.stride[1];
+  a.rows = (int)x.shape[0]; a.cols = (int)cols;
+  a.act = (int)act; a.dtype = (int)x.v->dtype;
+  a.alpha = (float)alpha; a.eps = (float)eps;
+  return launch(m, "g950_block_norm_general", (unsigned)a.rows, 256u, a, stream);
+}
+
 // ------------------------------------------------------------------- copy
 int op_copy(g950_module* m, const g950_view* views, uint32_t nviews, uint32_t nsc, void* stream) {
   if (nviews != 2 || nsc != 0) return fail(G950_USAGE, "copy: needs views (x, y) and no scalars");
@@ -1777,6 +2042,11 @@ int dispatch(g950_module* m, uint32_t op, const g950_view* views, uint32_t nview
       case G950_OP_SOFTMAX_INNER: return op_softmax_inner(m, views, nviews, scalars, nscalars, stream);
       case G950_OP_LAYERNORM_ROW: return op_layernorm_row(m, views, nviews, scalars, nscalars, stream);
       case G950_OP_GQA: return op_gqa(m, views, nviews, scalars, nscalars, stream);
+      case G950_OP_PAGED_APPEND: return op_paged_append(m, views, nviews, scalars, nscalars, false, stream);
+      case G950_OP_PAGED_APPEND_INT4: return op_paged_append(m, views, nviews, scalars, nscalars, true, stream);
+      case G950_OP_PAGED_ATTENTION_INT4:
+        return op_paged_attention_int4(m, views, nviews, scalars, nscalars, stream);
+      case G950_OP_BLOCK_NORM: return op_block_norm(m, views, nviews, scalars, nscalars, stream);
       default: return fail(G950_USAGE, "g950_launch: unknown operator contract %u", op);
     }
   } catch (...) {

@@ -236,6 +236,66 @@ def attn_fwd_causal_kernel(q_ptr, k_ptr, v_ptr, out_ptr, Z, H, N_CTX, scale,
     return _launch(op, tensors, outputs, scalars, stream, sync, prepare)
 
 
+def paged_append_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k_cache_ptr, v_cache_ptr, page_table_ptr,
+                        cu_seqlens_q_ptr, seqused_k_ptr, interleaved, *, stream=None, sync=False, prepare=False):
+    """Position rotation of q and k, k and v appended to a paged cache
+    (G950_OP_PAGED_APPEND; no reference counterpart).  q/q_out [tokens, h, d],
+    k/v [tokens, hk, d], cos/sin [positions, r / 2] (the first r dims turn), caches
+    [pages, block_size, hk, d], page_table [b, pages], cu_seqlens_q [b + 1],
+    seqused_k [b] (keys of each sequence, the new ones among them)."""
+    return _launch(rt.OP_PAGED_APPEND,
+                   {"q_ptr": q_ptr, "k_ptr": k_ptr, "v_ptr": v_ptr, "cos_ptr": cos_ptr, "sin_ptr": sin_ptr,
+                    "q_out_ptr": q_out_ptr, "k_cache_ptr": k_cache_ptr, "v_cache_ptr": v_cache_ptr,
+                    "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
+                    "seqused_k_ptr": seqused_k_ptr}, {"q_out_ptr", "k_cache_ptr", "v_cache_ptr"},
+                   {"interleaved": interleaved}, stream, sync, prepare)
+
+
+def paged_append_int4_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k_out_ptr, v_out_ptr, k_cache_ptr,
+                             k_scale_ptr, v_cache_ptr, v_scale_ptr, page_table_ptr, cu_seqlens_q_ptr, seqused_k_ptr,
+                             interleaved, *, stream=None, sync=False, prepare=False):
+    """paged_append_kernel into a cache of 4 bits (G950_OP_PAGED_APPEND_INT4):
+    codes uint8 [pages, block_size, hk, d / 2], scale and offset [pages,
+    block_size, hk, 2] in the model's type.  k_out/v_out [tokens, hk, d]: the
+    appended rows as the cache holds them (empty: not wanted)."""
+    return _launch(rt.OP_PAGED_APPEND_INT4,
+                   {"q_ptr": q_ptr, "k_ptr": k_ptr, "v_ptr": v_ptr, "cos_ptr": cos_ptr, "sin_ptr": sin_ptr,
+                    "q_out_ptr": q_out_ptr, "k_out_ptr": k_out_ptr, "v_out_ptr": v_out_ptr, "k_cache_ptr": k_cache_ptr,
+                    "k_scale_ptr": k_scale_ptr, "v_cache_ptr": v_cache_ptr, "v_scale_ptr": v_scale_ptr,
+                    "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
+                    "seqused_k_ptr": seqused_k_ptr},
+                   {"q_out_ptr", "k_out_ptr", "v_out_ptr", "k_cache_ptr", "k_scale_ptr", "v_cache_ptr", "v_scale_ptr"},
+                   {"interleaved": interleaved}, stream, sync, prepare)
+
+
+def paged_attention_int4_kernel(q_ptr, k_cache_ptr, k_scale_ptr, v_cache_ptr, v_scale_ptr, page_table_ptr,
+                                cu_seqlens_q_ptr, seqused_k_ptr, o_ptr, softmax_lse_ptr, workspace_ptr, seqlen_q, seqlen_k,
+                                scale_softmax, is_causal, window_size_left, window_size_right, *, stream=None,
+                                sync=False, prepare=False):
+    """Attention over a paged cache of 4 bits (G950_OP_PAGED_ATTENTION_INT4; no
+    reference counterpart): q/o [tokens, h, d], lse float32 [h, tokens], the
+    cache and its lists as paged_append_int4_kernel fills them; windows as in
+    flash_varlen_fwd_kernel, sizes below 0 without limit."""
+    return _launch(rt.OP_PAGED_ATTENTION_INT4,
+                   {"q_ptr": q_ptr, "k_cache_ptr": k_cache_ptr, "k_scale_ptr": k_scale_ptr, "v_cache_ptr": v_cache_ptr,
+                    "v_scale_ptr": v_scale_ptr, "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
+                    "seqused_k_ptr": seqused_k_ptr, "o_ptr": o_ptr, "softmax_lse_ptr": softmax_lse_ptr,
+                    "workspace_ptr": workspace_ptr}, {"o_ptr", "softmax_lse_ptr", "workspace_ptr"},
+                   {"seqlen_q": seqlen_q, "seqlen_k": seqlen_k, "scale_softmax": scale_softmax, "is_causal": is_causal,
+                    "window_size_left": window_size_left, "window_size_right": window_size_right}, stream, sync, prepare)
+
+
+def block_norm_kernel(X, H, W_post, G, W_pre, Y, N, eps, gate_act, residual_scale, *, stream=None, sync=False,
+                      prepare=False):
+    """The norms around a block with its gate and residual (G950_OP_BLOCK_NORM;
+    no reference counterpart): u = H rsqrt(mean(H^2) + eps) W_post, Y =
+    residual_scale X + act(G) u, N = Y rsqrt(mean(Y^2) + eps) W_pre, by rows.
+    Empty W_post, G or W_pre (with N): that part is left out.  gate_act: 0
+    none, 1 sigmoid, 2 tanh."""
+    return _launch(rt.OP_BLOCK_NORM, {"X": X, "H": H, "W_post": W_post, "G": G, "W_pre": W_pre, "Y": Y, "N": N}, {"Y", "N"},
+                   {"eps": eps, "gate_act": gate_act, "residual_scale": residual_scale}, stream, sync, prepare)
+
+
 def stream_copy(x, y, *, stream=None, sync=False, prepare=False):
     """y = x through the streaming-copy kernel (nontemporal 16-byte loads and
     stores, the row kernels' memory path); used to calibrate HBM counters."""
@@ -314,3 +374,84 @@ def attention(q, k, v, scale=None, causal=True, out=None, lse=None, **kw):
     attn_fwd_causal_kernel(q, k, v, o, z, h, s, scale, *q.stride(), *k.stride(), *v.stride(),
                            *o.stride(), CAUSAL=causal, lse_ptr=lse, **kw)
     return o, lse
+
+
+def paged_append(q, k, v, cos, sin, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, interleaved=False,
+                 out=None, **kw):
+    """Appends k and v to the cache and returns the rotated q (``out=q``: in
+    place; q may be None).  See paged_append_kernel."""
+    import torch
+    q = k.new_empty((k.shape[0], 0, k.shape[2])) if q is None else q
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    paged_append_kernel(q, k, v, cos, sin, out, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k,
+                        bool(interleaved), **kw)
+    return out
+
+
+def int4_cache(pages, block_size, heads, dim, dtype, device="cuda"):
+    """An empty 4-bit K or V cache: codes uint8 [pages, block_size, heads, dim / 2]
+    and scales dtype [pages, block_size, heads, 2], a page holding each head's
+    rows together (the layout the attention kernels stream best)."""
+    import torch
+    codes = torch.zeros((pages, heads, block_size, dim // 2), dtype=torch.uint8, device=device)
+    scale = torch.zeros((pages, heads, block_size, 2), dtype=dtype, device=device)
+    return codes.transpose(1, 2), scale.transpose(1, 2)
+
+
+def paged_append_int4(q, k, v, cos, sin, k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k,
+                      interleaved=False, out=None, values=False, k_out=None, v_out=None, **kw):
+    """paged_append into a cache of 4 bits (int4_cache).  Returns the rotated q
+    and, with ``values`` (or k_out / v_out given), the appended keys and values
+    as the cache holds them; else None for both."""
+    import torch
+    q = k.new_empty((k.shape[0], 0, k.shape[2])) if q is None else q
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    if values:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
+        v_out = torch.empty_like(v, memory_format=torch.contiguous_format) if v_out is None else v_out
+    none = k.new_empty((0, 0, 0)) if k_out is None or v_out is None else None
+    paged_append_int4_kernel(q, k, v, cos, sin, out, none if k_out is None else k_out, none if v_out is None else v_out,
+                             k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, bool(interleaved),
+                             **kw)
+    return out, k_out, v_out
+
+
+def paged_attention_int4(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, seqlen_q, seqlen_k,
+                         scale=None, causal=True, window=(-1, -1), out=None, lse=None, workspace=None, **kw):
+    """Attention of q over a paged cache of 4 bits; seqlen_q is the most
+    queries, seqlen_k the most keys of a sequence.  Returns o and lse [h, tokens]."""
+    import torch
+    t, h, d = q.shape
+    o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    lse = torch.empty((h, t), dtype=torch.float32, device=q.device) if lse is None else lse
+    if workspace is None:
+        workspace = torch.empty(0, dtype=torch.float32, device=q.device)
+    paged_attention_int4_kernel(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, o, lse,
+                                workspace, seqlen_q, seqlen_k, 1.0 / math.sqrt(d) if scale is None else float(scale),
+                                bool(causal), int(window[0]), int(window[1]), **kw)
+    return o, lse
+
+
+_GATE_ACTS = {None: 0, "none": 0, "sigmoid": 1, "tanh": 2}
+
+
+def block_norm(x, h, w_pre, eps, w_post=None, gate=None, gate_act=None, residual_scale=1.0, out=None, norm_out=None,
+               **kw):
+    """y = residual_scale x + act(gate) norm(h, w_post) and n = norm(y, w_pre)
+    (block_norm_kernel); gate broadcasts to x; w_pre None: y only (n is None).
+    ``out=x`` and ``norm_out=h`` work in place."""
+    import torch
+    if gate_act not in _GATE_ACTS:
+        raise rt.G950Error(rt.USAGE, f"block_norm: unknown gate_act {gate_act!r}")
+    y = torch.empty_like(x) if out is None else out
+    n = None
+    if w_pre is not None:
+        n = torch.empty_like(x) if norm_out is None else norm_out
+    none1 = x.new_empty(0) if w_post is None or w_pre is None else None
+    none2 = x.new_empty((0, 0)) if gate is None or n is None else None
+    if gate is not None:
+        gate = gate.expand(x.shape)
+    block_norm_kernel(x, h, none1 if w_post is None else w_post, none2 if gate is None else gate,
+                      none1 if w_pre is None else w_pre, y, none2 if n is None else n, float(eps), _GATE_ACTS[gate_act],
+                      float(residual_scale), **kw)
+    return y, n

@@ -175,6 +175,62 @@ typedef struct g950_scalar {
  *   scalars GROUP, HEAD_DIM, H_KV, H_Q, N_CTX, scale, stride_kh, stride_kk,
  *           stride_kn, stride_oh, stride_om, stride_on, stride_qh, stride_qk,
  *           stride_qm, stride_vh, stride_vk, stride_vn (BLOCK_N only shapes the tile)
+ *
+ * The remaining contracts have no counterpart in the reference: what a serving
+ * program does around paged attention.  Tokens of sequence b are rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 of q; seqused_k[b] counts the keys
+ * the sequence has once these tokens' are appended, so its token i stands at
+ * position seqused_k[b] - (its tokens) + i.  Rows past cu_seqlens_q[B] and
+ * sequences whose rows do not lie in q are left alone, outputs included.
+ *
+ * G950_OP_PAGED_APPEND  the position rotation of q and k by rows of the cos /
+ *                      sin tables (R / 2 columns: the first R dims turn, pairs
+ *                      (i, i + R / 2) or, interleaved, (2i, 2i + 1)), k and v
+ *                      appended to the paged cache; fp32 arithmetic, one rounding.
+ *                      q_out_ptr may be q_ptr itself (same strides), else they may
+ *                      not overlap.  A token at a position below 0 or past the
+ *                      tables is left out; a key page that the table or the pool
+ *                      does not hold drops only its cache row.  Cache rows that two
+ *                      tokens of a call name end as either.
+ *   views   cos_ptr[P,R/2], cu_seqlens_q_ptr i32[B+1], k_cache_ptr[pages,
+ *           block_size,HK,D], k_ptr[T,HK,D], page_table_ptr i32[B,max_pages],
+ *           q_out_ptr[T,H,D], q_ptr[T,H,D] (H may be 0), seqused_k_ptr i32[B],
+ *           sin_ptr[P,R/2], v_cache_ptr, v_ptr: f32 | bf16 | f16 (same; the tables
+ *           also f32), any strides but a contiguous last axis
+ *   scalars interleaved
+ * G950_OP_PAGED_APPEND_INT4  the same into a cache of 4 bits (D even, <= 256; bf16 |
+ *                      f16): a (token, head) row x, rotated and not yet rounded, is
+ *                      held as codes c and a pair (s, o) of the model's type T,
+ *                      s = T((max - min) / 15), o = T(min + 8 s), c = clamp(rint((x - o)
+ *                      (1 / s)) + 8, 0, 15), standing for (c - 8) s + o.  Byte i holds dims
+ *                      2i (low half) and 2i + 1.  A row holding NaN or infinities has
+ *                      s = o = NaN.
+ *   views   cos_ptr, cu_seqlens_q_ptr, k_cache_ptr u8[pages,block_size,HK,D/2],
+ *           k_out_ptr[T,HK,D] or empty (the appended rows as the cache now holds
+ *           them, rounded to T), k_ptr, k_scale_ptr[pages,block_size,HK,2],
+ *           page_table_ptr, q_out_ptr, q_ptr, seqused_k_ptr, sin_ptr, v_cache_ptr,
+ *           v_out_ptr, v_ptr, v_scale_ptr
+ *   scalars interleaved
+ * G950_OP_PAGED_ATTENTION_INT4  attention over that cache: GQA, query i of a
+ *                      sequence with n of them sees keys j with i + seqused_k - n - left <= j
+ *                      <= i + seqused_k - n + right (window sizes below 0: no limit; causal:
+ *                      right = 0) whose page the pool holds; queries from seqlen_q on are
+ *                      left alone; O = 0 and LSE = +inf for a row without keys (and, as
+ *                      in G950_OP_FLASH_VARLEN, LSE = +inf where the sum is NaN)
+ *   views   cu_seqlens_q_ptr, k_cache_ptr, k_scale_ptr, o_ptr[T,H,D],
+ *           page_table_ptr, q_ptr[T,H,D], seqused_k_ptr, softmax_lse_ptr f32[H,T],
+ *           v_cache_ptr, v_scale_ptr, workspace_ptr f32 (1-D, any length, also 0)
+ *   scalars is_causal, scale_softmax, seqlen_k (about the longest sequence's
+ *           keys: shapes the key ranges only), seqlen_q, window_size_left,
+ *           window_size_right
+ * G950_OP_BLOCK_NORM   the norms around a block with its gate and residual:
+ *                      u = H rsqrt(mean(H^2) + eps) W_post (H itself without W_post),
+ *                      Y = residual_scale X + act(G) u, N = Y rsqrt(mean(Y^2) + eps) W_pre
+ *                      of Y before its rounding.  Y may be X and N may be H.
+ *   views   G[R,C] (strides may be 0) or empty, H[R,C], N[R,C] (empty without
+ *           W_pre), W_post[C] or empty, W_pre[C] or empty, X[R,C], Y[R,C]: one
+ *           float dtype
+ *   scalars eps, gate_act (0 none, 1 sigmoid, 2 tanh), residual_scale
  */
 enum g950_op {
   G950_OP_SOFTMAX = 1,
@@ -192,7 +248,11 @@ enum g950_op {
   G950_OP_DEQUANT_MATMUL = 13,
   G950_OP_SOFTMAX_INNER = 14,
   G950_OP_LAYERNORM_ROW = 15,
-  G950_OP_GQA = 16
+  G950_OP_GQA = 16,
+  G950_OP_PAGED_APPEND = 17,
+  G950_OP_PAGED_APPEND_INT4 = 18,
+  G950_OP_PAGED_ATTENTION_INT4 = 19,
+  G950_OP_BLOCK_NORM = 20
 };
 
 typedef struct g950_module g950_module;
