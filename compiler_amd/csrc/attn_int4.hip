@@ -113,8 +113,508 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
         empty ? __builtin_huge_valf() : (m + __log2f(l)) * 0.69314718055994530942f;
 }
 
+// ---------------------------------------------------------------- fast form
+// d 64, 128 or 256, pages of whole 16-key runs, 16-byte rows.  A workgroup owns
+// one (sequence, KV head, block of 16 RT query rows, key range); a query row is
+// (query, head of the group), so K and V are read once for the whole group.  Its
+// 4 waves take 32-key tiles in turn and share nothing until the end: each fills
+// its own LDS ring by direct global->LDS DMA and waits for its own loads only.
+//
+// What bounds it is the vector ALU beside the bytes: a tile of 32 keys is
+// 64 d values in 64 lanes and leaves HBM in about a thousand cycles of a SIMD.  No value
+// is therefore ever dequantised: the matrix cores multiply the codes, and scale and
+// offset enter where a tile has few numbers.
+//   * A word holds 8 codes; (w >> 4 i) & 0x000F000F | bias makes two of them
+//     numbers at once, 128 + c in bfloat16 or 1024 + c in float16 (the code lands in
+//     the low mantissa bits): 7 operations for 8 codes.
+//   * S = s (sum q c) + o sum q, c in -8 .. 7: the bias leaves through the MFMA's
+//     addend, -(bias + 8) sum q.  Exact products, fp32 sums.
+//   * O = sum (p s) c + sum p o: the probability carries V's scale, rounded to
+//     bfloat16 once (its range, as s may be any size); the bias leaves through one
+//     more MFMA with a constant -136 in place of V, over the same rounded values, so
+//     that nothing of it is left.  p o and the softmax sum stay in fp32.
+//   * V^T needs keys along the contraction: a lane reads the same word of its four
+//     keys of each half, and byte permutes put two keys beside each other before
+//     the masks; no transpose.  Lane (g, l)'s keys are g + 4 e of each half, so the
+//     four rows of a read lie in different LDS banks.
+//   * K's dims are taken in the order in which the words hold them; q's fragments
+//     are laid out to match, once.
+constexpr int I4_WAVES = 4;
+constexpr int I4_TK = 32;  // keys per tile of one wave
+
+__device__ __forceinline__ void dma_lane16(const char* src, uint32_t lds_dst) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_dst);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void dma_lane4(const char* src, uint32_t lds_dst) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_dst);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+}
+
+template <bool F16>
+__device__ __forceinline__ f32x4 int4_mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+
+// scale (low half) and offset (high half) of a pair
+template <bool F16>
+__device__ __forceinline__ void int4_pair(uint32_t w, float& s, float& o) {
+  if constexpr (F16) {
+    s = f16_to_f32((uint16_t)w);
+    o = f16_to_f32((uint16_t)(w >> 16));
+  } else {
+    s = __uint_as_float(w << 16);
+    o = __uint_as_float(w & 0xFFFF0000u);
+  }
+}
+
+// value of `v` combined over the four lanes holding one query row
+template <class Op>
+__device__ __forceinline__ float int4_row(float v) {
+  v = Op::apply(v, __shfl_xor(v, 16));
+  return Op::apply(v, __shfl_xor(v, 32));
+}
+
+template <int D, bool F16, int RT>
+__device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
+  constexpr int RB = D / 2;                       // bytes of a row
+  constexpr int KT = I4_TK * RB;                  // bytes of a tile's K (or V)
+  constexpr int TILE = 2 * KT + 256;              // K, V, 64 pairs
+  constexpr int ST = D == 64 ? 7 : D == 128 ? 4 : 2;  // tiles in flight per wave
+  constexpr int RING = ST * TILE;
+  constexpr int DC = KT / 1024;                   // DMA instructions of a tile's K
+  constexpr int DPT = 2 * DC + 1;
+  constexpr int LPK = RB / 16;                    // lanes (16 bytes) per key of a DMA instruction
+  constexpr int KPI = 64 / LPK;                   // keys per instruction
+  constexpr int KS = D / 32;                      // words of a lane per K row: k-steps of S^T
+  constexpr int VW = D == 256 ? 2 : 1;            // words (d 64: half words) of a lane per V row
+  constexpr int VN = D == 64 ? 4 : 8;             // codes of each
+  constexpr int NB = VW * VN;                     // 16-d blocks of O^T
+  constexpr int ROWS = 16 * RT;
+  constexpr uint32_t KBIAS = F16 ? 0x64006400u : 0x43004300u;
+  constexpr float KOFF = F16 ? 1032.0f : 136.0f;
+  static_assert(ROWS * D * 4 <= RING, "a wave's partial O fits its ring");
+  __shared__ __attribute__((aligned(1024))) char lds[I4_WAVES * RING];
+  __shared__ float ml[I4_WAVES][ROWS][2];
+  if (blockDim.x != I4_WAVES * 64) return;  // launch shape must match the kernel
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g4 = lane >> 4, l16 = lane & 15;
+  const int pairs = p.B * p.Hkv;
+  const int pair = blockIdx.x % pairs;
+  const int block = (blockIdx.x / pairs) % p.row_blocks, split = blockIdx.x / pairs / p.row_blocks;
+  const int z = pair / p.Hkv, hk = pair % p.Hkv;
+  const int G = p.group;
+  const Int4Seq sq = int4_seq(p, z);
+  const int rows = min(sq.nq, p.seqlen_q) * G;  // of this sequence and KV head
+  const int row0 = block * ROWS;
+  if (row0 >= rows) return;
+  const int nrows = min(ROWS, rows - row0);
+  // visible keys of query i: [base + i - left, base + i + right] within the sequence
+  const long long base = (long long)p.used[z] - sq.nq;
+  const int nk = p.pages > 0 ? sq.nk : 0;
+  auto first_key = [&](int i) {
+    const long long k = base + i - p.left;
+    return p.left < 0 || k < 0 ? 0 : k > nk ? nk : (int)k;
+  };
+  auto last_key = [&](int i) {
+    const long long k = base + i + p.right;
+    return p.right < 0 || k >= nk ? nk - 1 : k < -1 ? -1 : (int)k;
+  };
+  const int i_lo = row0 / G, i_hi = (row0 + nrows - 1) / G;
+  const int kend = last_key(i_hi) + 1, kbeg = first_key(i_lo) / I4_TK * I4_TK;
+  const int all_from = first_key(i_hi), all_to = last_key(i_lo);  // keys every row sees
+
+  // query fragments: row l16 of tile rt; lane group g4 holds dims g4 D / 4 ..,
+  // word ks their 8 from 8 ks on, as pairs (r, r + 4)
+  u32x4 qf[RT][KS];
+  float qsum[RT];
+  int kmin[RT], kmax[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + min(rt * 16 + l16, nrows - 1);
+    const int i = r / G, h = hk * G + r % G;
+    kmin[rt] = first_key(i);
+    kmax[rt] = last_key(i);
+    const char* src = (const char*)p.q + 2 * ((long long)(sq.q0 + i) * p.q_st + (long long)h * p.q_sh + g4 * (D / 4));
+    float s = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const u32x4 w = *(const u32x4*)(src + ks * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float a, b;
+        int4_pair<F16>(w[e], a, b);
+        s += a + b;
+      }
+      qf[rt][ks] = (u32x4){__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
+                           __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
+    }
+    qsum[rt] = int4_row<OpSum>(s);
+  }
+
+  char* ring = lds + wave * RING;
+  const uint32_t ring32 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring;
+  const char* kbase = (const char*)p.k + (long long)hk * p.k_h;
+  const char* vbase = (const char*)p.v + (long long)hk * p.v_h;
+  // this lane's share of a DMA instruction: key dkey (of KPI), 16-byte piece dpos
+  const int dkey = lane / LPK, dpos = lane % LPK;
+  // and of the pairs: word lane = ((kind * 2 + half) * 4 + g) * 4 + e holds key g + 4 e of the half
+  const int skey = ((lane >> 2) & 3) + 4 * (lane & 3), shalf = (lane >> 4) & 1;
+  const char* sbase = lane < 32 ? (const char*)p.ks + 2 * ((long long)hk * p.ks_h + (long long)skey * p.ks_r)
+                                : (const char*)p.vs + 2 * ((long long)hk * p.vs_h + (long long)skey * p.vs_r);
+  const uint32_t s_p = 2 * (uint32_t)(lane < 32 ? p.ks_p : p.vs_p), s_r = 2 * (uint32_t)(lane < 32 ? p.ks_r : p.vs_r);
+  const int* table = p.table + (long long)z * p.table_s;
+
+  int lo = kbeg, hi = kend;
+  if (p.splits > 1) {
+    lo = max(lo, split * p.chunk);
+    hi = split + 1 < p.splits ? min(hi, (split + 1) * p.chunk) : hi;
+  }
+  const int ntiles = hi > lo ? (hi - lo + I4_TK - 1) / I4_TK : 0;
+  const int nloc = ntiles > wave ? (ntiles - wave + I4_WAVES - 1) / I4_WAVES : 0;
+
+  // pages and rows of this wave's next 32 tiles, one 16-key half per lane; a half
+  // without a page (or past the end) reads page 0 and is masked
+  int pages = 0, prow = 0;
+  uint64_t live[2] = {0, 0};  // by the parity of the batch of 32 tiles
+  auto issue = [&](int j) {
+    if ((j & 31) == 0) {
+      const int key = lo + I4_TK * (wave + I4_WAVES * (j + (lane >> 1))) + 16 * (lane & 1);
+      const int e = key / p.block_size;
+      int ph = key < hi && e < p.max_pages ? table[e] : -1;
+      ph = ph < p.pages ? ph : -1;
+      const uint64_t m = __ballot(ph >= 0);
+      if (j & 32) live[1] = m;
+      else live[0] = m;
+      prow = ph < 0 ? 0 : key - e * p.block_size;
+      pages = max(ph, 0);
+    }
+    const int at = 2 * (j & 31);
+    const int pg[2] = {__builtin_amdgcn_readlane(pages, at), __builtin_amdgcn_readlane(pages, at + 1)};
+    const int pr[2] = {__builtin_amdgcn_readlane(prow, at), __builtin_amdgcn_readlane(prow, at + 1)};
+    const uint32_t dst = ring32 + (j % ST) * TILE;
+    const char *ksrc[2], *vsrc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      ksrc[t] = kbase + (long long)pg[t] * p.k_p + (long long)pr[t] * p.k_r;
+      vsrc[t] = vbase + (long long)pg[t] * p.v_p + (long long)pr[t] * p.v_r;
+    }
+#pragma unroll
+    for (int u = 0; u < DC; ++u) {
+      const int k = u * KPI + dkey;  // key of the tile
+      const bool second = KPI <= 16 ? u * KPI >= 16 : k >= 16;
+      dma_lane16((second ? ksrc[1] : ksrc[0]) + (k & 15) * (int)p.k_r + dpos * 16, dst + u * 1024);
+    }
+#pragma unroll
+    for (int u = 0; u < DC; ++u) {
+      const int k = u * KPI + dkey;
+      const bool second = KPI <= 16 ? u * KPI >= 16 : k >= 16;
+      dma_lane16((second ? vsrc[1] : vsrc[0]) + (k & 15) * (int)p.v_r + dpos * 16, dst + KT + u * 1024);
+    }
+    const uint32_t pl = shalf ? pg[1] : pg[0], rl = shalf ? pr[1] : pr[0];
+    dma_lane4(sbase + (uint64_t)pl * s_p + (uint64_t)rl * s_r, dst + 2 * KT);
+  };
+
+  f32x4 o[RT][NB], ob[RT];
+  float ms[RT], l[RT], zo[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    ms[rt] = -__builtin_huge_valf();
+    l[rt] = zo[rt] = 0.0f;
+    ob[rt] = (f32x4){};
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[rt][b] = (f32x4){};
+  }
+  const float c2 = p.scale_log2;
+  const int kperm = (l16 >> 2) + 4 * (l16 & 3);  // K row of S^T's row l16
+  const uint32_t m136 = 0xC308C308u;             // -136 in bfloat16, twice
+  const u32x4 unbias = {m136, m136, m136, m136};
+  for (int j = 0; j < ST && j < nloc; ++j) issue(j);
+  for (int i = 0; i < nloc; ++i) {
+    // tile i has landed once at most the later tiles' loads are in flight
+    if (i + ST <= nloc) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * DPT) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const char* st = ring + (i % ST) * TILE;
+    const int kv0 = lo + I4_TK * (wave + I4_WAVES * i);
+    f32x4 s[2][RT];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t kw[KS];
+      const char* kr = st + (t * 16 + kperm) * RB + g4 * (RB / 4);
+      if constexpr (KS == 2) {
+        const u32x2 w = *(const u32x2*)kr;
+        kw[0] = w[0];
+        kw[1] = w[1];
+      } else {
+#pragma unroll
+        for (int c = 0; c < KS / 4; ++c) {
+          const u32x4 w = *(const u32x4*)(kr + 16 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kw[4 * c + e] = w[e];
+        }
+      }
+      f32x4 acc[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float q = -KOFF * qsum[rt];
+        acc[rt] = (f32x4){q, q, q, q};
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        u32x4 kf;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kf[r] = ((kw[ks] >> (4 * r)) & 0x000F000Fu) | KBIAS;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt] = int4_mfma<F16>(kf, qf[rt][ks], acc[rt]);
+      }
+      const u32x4 kp = *(const u32x4*)(st + 2 * KT + t * 64 + g4 * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float sc, of;
+        int4_pair<F16>(kp[e], sc, of);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[t][rt][e] = fmaf(sc, acc[rt][e], of * qsum[rt]);
+      }
+    }
+    const uint32_t alive = (uint32_t)(live[(i >> 5) & 1] >> (2 * (i & 31))) & 3;
+    const bool mask = alive != 3 || kv0 < all_from || kv0 + I4_TK - 1 > all_to || kv0 + I4_TK > hi;
+    if (mask) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = kv0 + 16 * t + g4 + 4 * e;
+            if (!((alive >> t) & 1) || key < kmin[rt] || key > kmax[rt] || key >= hi) s[t][rt][e] = -__builtin_huge_valf();
+          }
+    }
+    u32x4 pf[RT];
+    float vs[2][4], vo[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const u32x4 vp = *(const u32x4*)(st + 2 * KT + 128 + t * 64 + g4 * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) int4_pair<F16>(vp[e], vs[t][e], vo[t][e]);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float mh = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
+                             fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3]))) * c2;
+      if (__any(mh > ms[rt] + 8.0f)) {
+        const float mt = int4_row<OpMax>(mh);
+        const bool move = mt > ms[rt] + 8.0f;
+        const float alpha = move ? __builtin_amdgcn_exp2f(ms[rt] - mt) : 1.0f;
+        l[rt] *= alpha;
+        zo[rt] *= alpha;
+        ob[rt] *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[rt][b] *= alpha;
+        ms[rt] = move ? mt : ms[rt];
+      }
+      // rows without a visible key so far: exponent base 0, exp2(-inf) = 0
+      const float mb = (ms[rt] == -__builtin_huge_valf()) ? 0.0f : ms[rt];
+      float ps[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float pe[4], zp[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pe[e] = __builtin_amdgcn_exp2f(fmaf(s[t][rt][e], c2, -mb));
+          ps[t][e] = pe[e] * vs[t][e];
+          zp[e] = vo[t][e];
+        }
+        if (mask) {  // what a row does not see may hold anything
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool none = s[t][rt][e] == -__builtin_huge_valf();
+            ps[t][e] = none ? 0.0f : ps[t][e];
+            zp[e] = none ? 0.0f : zp[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) zo[rt] = fmaf(pe[e], zp[e], zo[rt]);
+        l[rt] += (pe[0] + pe[1]) + (pe[2] + pe[3]);
+      }
+      auto two = [](float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+      };
+      pf[rt] = (u32x4){two(ps[0][0], ps[0][1]), two(ps[0][2], ps[0][3]), two(ps[1][0], ps[1][1]), two(ps[1][2], ps[1][3])};
+      ob[rt] = int4_mfma<false>(unbias, pf[rt], ob[rt]);
+    }
+    // V: words of keys g4 + 4 e of both halves, two keys side by side
+    const char* vr = st + KT + g4 * RB + l16 * (D == 64 ? 2 : 4);
+#pragma unroll
+    for (int c = 0; c < VW; ++c) {
+      u32x4 half[D == 64 ? 1 : 2];  // codes 0 .. 3 (and 4 .. 7) of the pairs of keys
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const char* a = vr + (16 * t + 4 * e) * RB + c * 64;
+          if constexpr (D == 64) {
+            half[0][2 * t + e / 2] = (uint32_t)*(const uint16_t*)a | (uint32_t)*(const uint16_t*)(a + 4 * RB) << 16;
+          } else {
+            const uint32_t w0 = *(const uint32_t*)a, w1 = *(const uint32_t*)(a + 4 * RB);
+            half[0][2 * t + e / 2] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+            half[1][2 * t + e / 2] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+          }
+        }
+#pragma unroll
+      for (int n = 0; n < VN; ++n) {
+        u32x4 vf;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vf[r] = ((half[n / 4][r] >> (4 * (n & 3))) & 0x000F000Fu) | 0x43004300u;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][c * VN + n] = int4_mfma<false>(vf, pf[rt], o[rt][c * VN + n]);
+      }
+    }
+    // this tile's LDS reads have returned before its slot is refilled
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (i + ST < nloc) issue(i + ST);
+  }
+
+  // ---- the four waves' partial rows: O through each wave's own ring (16-byte
+  // chunks XOR-swizzled by the row), maxima and sums beside it.  Block b = c VN + n,
+  // element e: dim 128 c + VN (4 g4 + e) + n.
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rt * 16 + l16;
+    const float ls = int4_row<OpSum>(l[rt]), add = int4_row<OpSum>(zo[rt]) + ob[rt][0];
+#pragma unroll
+    for (int c = 0; c < VW; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int n = 0; n < VN; n += 4) {
+          const int chunk = (128 * c + VN * (4 * g4 + e) + n) / 4;
+          *(f32x4*)(ring + r * D * 4 + ((chunk ^ l16) << 4)) =
+              (f32x4){o[rt][c * VN + n][e] + add, o[rt][c * VN + n + 1][e] + add, o[rt][c * VN + n + 2][e] + add,
+                      o[rt][c * VN + n + 3][e] + add};
+        }
+    if (g4 == 0) {
+      ml[wave][r][0] = ms[rt];
+      ml[wave][r][1] = ls;
+    }
+  }
+  __syncthreads();
+  constexpr int CPR = D / 4;  // 16-byte chunks (4 d) per row
+  for (int it = tid; it < nrows * CPR; it += I4_WAVES * 64) {
+    const int r = it / CPR, c = it % CPR;
+    float m = ml[0][r][0];
+#pragma unroll
+    for (int w = 1; w < I4_WAVES; ++w) m = fmaxf(m, ml[w][r][0]);
+    f32x4 sum = {};
+    float lt = 0.0f;
+#pragma unroll
+    for (int w = 0; w < I4_WAVES; ++w) {
+      const float mw = ml[w][r][0], lw = ml[w][r][1];
+      // no finite score: no key of this row (l = 0), or only NaN ones
+      const float f = mw == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      lt = fmaf(f, lw, lt);
+      const f32x4 ow = *(const f32x4*)(lds + w * RING + r * D * 4 + ((c ^ (r & 15)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, ow[e], sum[e]);
+    }
+    if (p.splits > 1) {
+      const long long rec = (((long long)pair * p.row_blocks + block) * p.splits + split) * ROWS + r;
+      *(f32x4*)(p.part + rec * D + c * 4) = sum;
+      if (c == 0) {
+        p.ml[2 * rec] = m;
+        p.ml[2 * rec + 1] = lt;
+      }
+      continue;
+    }
+    const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
+    const bool empty = !(lt > 0.0f);  // zero or NaN
+    const float inv = empty ? 1.0f : 1.0f / lt;
+    char* dst = (char*)p.o + 2 * ((long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + c * 4);
+    if constexpr (F16)
+      *(u32x2*)dst = (u32x2){__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[0] * inv, sum[1] * inv}, f16x2)),
+                             __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[2] * inv, sum[3] * inv}, f16x2))};
+    else
+      *(u32x2*)dst = (u32x2){__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[0] * inv, sum[1] * inv}, bf16x2)),
+                             __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[2] * inv, sum[3] * inv}, bf16x2))};
+    if (c == 0)
+      p.lse[(long long)h * p.lse_h + (long long)(sq.q0 + i) * p.lse_t] =
+          empty ? __builtin_huge_valf() : (m + __log2f(lt)) * 0.69314718055994530942f;
+  }
+}
+
+// Joins the key ranges: one wave per query row, lane s holds range s's maximum
+// and sum (at most 64 ranges), D / 64 outputs per lane.
+template <int D, bool F16, int ROWS>
+__device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
+  const int lane = threadIdx.x & 63;
+  const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per = p.row_blocks * ROWS;
+  const int pair = (int)(item / per), row = (int)(item % per);
+  if (pair >= p.B * p.Hkv) return;
+  const int z = pair / p.Hkv, hk = pair % p.Hkv;
+  const Int4Seq sq = int4_seq(p, z);
+  if (row >= min(sq.nq, p.seqlen_q) * p.group) return;
+  const long long rec = ((long long)pair * p.row_blocks + row / ROWS) * p.splits * ROWS + row % ROWS;
+  float m = -__builtin_huge_valf(), l = 0.0f;
+  if (lane < p.splits) {
+    m = p.ml[2 * (rec + (long long)lane * ROWS)];
+    l = p.ml[2 * (rec + (long long)lane * ROWS) + 1];
+  }
+  const float mt = wave_reduce<OpMax>(m);
+  // no finite score in a range: nothing seen (O = l = 0), or only NaN, which stays
+  const float f = m == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(m - mt);
+  const float lt = wave_reduce<OpSum>(f * l);
+  constexpr int E = D / 64, U = 8;
+  float acc[E] = {};
+  for (int s0 = 0; s0 < p.splits; s0 += U) {
+    float v[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[u][e] = p.part[(rec + (long long)min(s0 + u, p.splits - 1) * ROWS) * D + lane * E + e];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s0 + u, 63)));
+      if (s0 + u < p.splits)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[u][e], acc[e]);
+    }
+  }
+  const int i = row / p.group, h = hk * p.group + row % p.group;
+  const bool empty = !(lt > 0.0f);
+  const float inv = empty ? 1.0f : 1.0f / lt;
+  uint16_t* dst = (uint16_t*)p.o + (long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = F16 ? f32_to_f16(acc[e] * inv) : f32_to_bf16(acc[e] * inv);
+  if (lane == 0)
+    p.lse[(long long)h * p.lse_h + (long long)(sq.q0 + i) * p.lse_t] =
+        empty ? __builtin_huge_valf() : (mt + __log2f(lt)) * 0.69314718055994530942f;
+}
+
 }  // namespace g950
 
 extern "C" __global__ __launch_bounds__(64) void g950_attn_int4_general(const g950::AttnInt4Args p) {
   g950::attn_int4_general_body(p);
 }
+// Two workgroups per CU (256 registers).
+#define G950_INT4(NAME, D, F16, RT)                                                                    \
+  extern "C" __global__ __launch_bounds__(256, 2) void NAME##_r##RT(const g950::AttnInt4Args p) {      \
+    g950::attn_int4_body<D, F16, RT>(p);                                                               \
+  }                                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void NAME##_r##RT##_merge(const g950::AttnInt4Args p) { \
+    g950::attn_int4_merge_body<D, F16, 16 * RT>(p);                                                    \
+  }
+G950_INT4(g950_attn_int4_bf16_d64, 64, false, 1)
+G950_INT4(g950_attn_int4_bf16_d64, 64, false, 2)
+G950_INT4(g950_attn_int4_bf16_d128, 128, false, 1)
+G950_INT4(g950_attn_int4_bf16_d128, 128, false, 2)
+G950_INT4(g950_attn_int4_bf16_d256, 256, false, 1)
+G950_INT4(g950_attn_int4_f16_d64, 64, true, 1)
+G950_INT4(g950_attn_int4_f16_d64, 64, true, 2)
+G950_INT4(g950_attn_int4_f16_d128, 128, true, 1)
+G950_INT4(g950_attn_int4_f16_d128, 128, true, 2)
+G950_INT4(g950_attn_int4_f16_d256, 256, true, 1)

@@ -1831,7 +1831,53 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   a.interleaved = interleaved ? 1 : 0;
   a.dtype = (int)dt; a.table_dtype = (int)cos.v->dtype; a.int4 = int4 ? 1 : 0;
   const long long rows = a.B ? T * (H + 2 * HK) : 0;
+  // whole vectors: rows of 32 to 256 dims (a power of two) that turn as a whole or
+  // not at all, 16-byte rows everywhere (4-byte code words and pairs)
+  auto rows_at = [&](const View& w, int bytes) {
+    bool ok = w.addr() % bytes == 0;
+    for (int d = 0; d + 1 < w.nd; ++d) ok = ok && w.stride[d] * w.isz % bytes == 0;
+    return ok || no_elements(w);
+  };
+  bool vec = (D == 32 || D == 64 || D == 128 || D == 256) && (R == 0 || R == D) && rows_at(q, 16) && rows_at(k, 16) &&
+             rows_at(v, 16) && rows_at(qo, 16) && (R == 0 || (rows_at(cos, 16) && rows_at(sin, 16)));
+  vec = vec && (int4 ? rows_at(kc, 4) && rows_at(vc, 4) && rows_at(ks, 4) && rows_at(vs, 4) && rows_at(ko, 16) && rows_at(vo, 16)
+                     : rows_at(kc, 16) && rows_at(vc, 16));
+  if (vec && rows) {
+    // a wave takes all heads of a token, or fewer while there are CUs without waves
+    const long long groups = (H + 2 * HK + 1024 / D - 1) / (1024 / D);
+    const long long cus = m ? m->cus : 256;
+    a.chunks = (int)std::max(1ll, std::min(groups, 16 * cus / std::max(T, 1ll)));
+    const long long blocks = (T * a.chunks + 3) / 4;
+    if (blocks > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+    char name[64];
+    snprintf(name, sizeof name, "g950_kv_append%s_%s_d%lld", int4 ? "_int4" : "", rr_dtype(dt), D);
+    return launch(m, name, (unsigned)blocks, 256u, a, stream);
+  }
   return launch(m, "g950_kv_append_general", (unsigned)std::min((rows + 3) / 4, 1ll << 20), 256u, a, stream);
+}
+
+// How attention over the 4-bit cache cuts a call: blocks of 16 or 32 query rows
+// per (sequence, KV head), and key ranges.
+struct Int4Shape {
+  long long rows;        // query rows of a workgroup
+  long long row_blocks;  // per (sequence, KV head)
+  long long blocks;      // of the call
+  long long splits;      // key ranges wanted
+};
+constexpr long long kInt4Target = 4, kInt4MinKeys = 256, kInt4OneRange = 512;
+
+Int4Shape int4_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
+                     long long seqlen_k) {
+  const long long cus = m ? m->cus : 256, rows = seqlen_q * (h / hk);
+  Int4Shape f;
+  f.rows = d == 256 || rows <= 16 ? 16 : 32;
+  f.row_blocks = (rows + f.rows - 1) / f.rows;
+  f.blocks = b * hk * f.row_blocks;
+  f.splits = f.blocks ? std::min({(kInt4Target * cus + f.blocks - 1) / f.blocks, (seqlen_k + kInt4MinKeys - 1) / kInt4MinKeys,
+                                  64ll})  // the merge holds a row's ranges in one wave's lanes
+                      : 1;
+  f.splits = seqlen_k <= kInt4OneRange ? 1 : std::max(f.splits, 1ll);
+  return f;
 }
 
 int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
@@ -1898,6 +1944,41 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
   a.dtype = (int)dt; a.group = (int)(H / HK); a.seqlen_q = (int)SQ;
   const long long rows = a.B && SQ ? T * H : 0;
   if (rows > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+  // the fast kernels: 16-byte rows (codes, q), 8-byte pieces of o, pairs of 4 bytes, 16-key
+  // runs within a page, row offsets of a run within 32 bits
+  auto m16 = [](const View& w) {
+    return aligned16(w.addr()) && w.stride[0] % 16 == 0 && w.stride[1] % 16 == 0 && w.stride[2] % 16 == 0 && w.stride[1] >= 0 &&
+           w.stride[1] < (1ll << 27);
+  };
+  auto m4 = [](const View& w) {
+    return w.addr() % 4 == 0 && w.stride[0] % 2 == 0 && w.stride[1] % 2 == 0 && w.stride[2] % 2 == 0 && w.stride[0] >= 0 &&
+           w.stride[0] < (1ll << 30) && w.stride[1] >= 0 && w.stride[1] < (1ll << 30);
+  };
+  const long long most = 0x7FFF0000;  // keys: positions a little past the last one stay within 32 bits
+  SK = std::min(SK, most);
+  const bool fast = (D == 64 || D == 128 || D == 256) && (long long)a.max_pages * a.block_size <= most && a.scale_log2 > 0.0f && std::isfinite(a.scale_log2) &&
+                    a.block_size % 16 == 0 && m16(k) && m16(v) && m4(ks) && m4(vs) && aligned16(q.addr()) &&
+                    a.q_st % 8 == 0 && a.q_sh % 8 == 0 && o.addr() % 8 == 0 && a.o_st % 4 == 0 && a.o_sh % 4 == 0;
+  if (fast && rows) {
+    const Int4Shape f = int4_shape(m, a.B, H, HK, D, std::min(SQ, T), SK);
+    if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
+    // as many key ranges as the workspace holds records for
+    const long long rec = f.blocks * f.rows * (D + 2);
+    const long long splits = std::min(f.splits, ws.shape[0] / rec);
+    a.row_blocks = (int)f.row_blocks;
+    a.splits = (int)std::max(splits, 1ll);
+    a.chunk = (int)std::min(((SK + a.splits - 1) / a.splits + 127) / 128 * 128, most);
+    a.part = (float*)ws.v->data;
+    a.ml = a.part + f.blocks * f.rows * a.splits * D;
+    if (f.blocks * a.splits > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+    char name[64];
+    const int n = snprintf(name, sizeof name, "g950_attn_int4_%s_d%lld_r%lld", dt == G950_DTYPE_BFLOAT16 ? "bf16" : "f16", D,
+                           f.rows / 16);
+    if (int rc = launch(m, name, (unsigned)(f.blocks * a.splits), 256u, a, stream)) return rc;
+    if (a.splits == 1) return G950_OK;
+    snprintf(name + n, sizeof name - n, "_merge");
+    return launch(m, name, (unsigned)((f.blocks * f.rows + 3) / 4), 256u, a, stream);
+  }
   return launch(m, "g950_attn_int4_general", (unsigned)rows, 64u, a, stream);
 }
 
@@ -1957,6 +2038,17 @@ int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const
   a.rows = (int)x.shape[0]; a.cols = (int)cols;
   a.act = (int)act; a.dtype = (int)x.v->dtype;
   a.alpha = (float)alpha; a.eps = (float)eps;
+  // the smallest form that holds a row; a gate that is neither contiguous along
+  // the row nor one per row, and longer rows, take the general kernel
+  static const struct { int items, block; } kForms[] = {{1, 64}, {2, 64}, {1, 256}, {2, 256}, {4, 256}, {8, 256}, {4, 1024}};
+  const long long nv = (cols * x.isz + 15) / 16;
+  const int gk = !gate ? 0 : a.g_col == 1 || cols == 1 ? 1 : a.g_col == 0 ? 2 : -1;
+  for (const auto& f : kForms) {
+    if (gk < 0 || nv > (long long)f.items * f.block) continue;
+    char name[64];
+    snprintf(name, sizeof name, "g950_block_norm_%s_i%d_b%d_g%d", rr_dtype(x.v->dtype), f.items, f.block, gk);
+    return launch(m, name, (unsigned)a.rows, (unsigned)f.block, a, stream);
+  }
   return launch(m, "g950_block_norm_general", (unsigned)a.rows, 256u, a, stream);
 }
 
@@ -2091,6 +2183,18 @@ size_t g950_workspace_bytes(g950_module* m, void* stream) {
   for (const auto* ws : {&m->ws, &m->ws_opt})
     if (const auto it = ws->find(stream); it != ws->end()) n += it->second.second;
   return n;
+}
+
+size_t g950_paged_attention_int4_workspace(g950_module* m, int64_t b, int64_t h, int64_t hk, int64_t d, int64_t seqlen_q,
+                                           int64_t seqlen_k) {
+  const int64_t most = 1ll << 31;
+  if (b <= 0 || hk <= 0 || h < hk || h % hk || d <= 0 || seqlen_q <= 0 || seqlen_k <= 0 || b > most || h > 65536 || d > 256 ||
+      seqlen_q > most || seqlen_k > most)
+    return 0;
+  const Int4Shape f = int4_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
+  // a call of more blocks than there are places for takes one range
+  if (f.splits <= 1 || (d != 64 && d != 128 && d != 256)) return 0;
+  return (size_t)f.blocks * (size_t)f.rows * (size_t)f.splits * (size_t)(d + 2) * 4;
 }
 
 int g950_sync(void* stream) {

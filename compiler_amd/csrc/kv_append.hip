@@ -20,6 +20,8 @@
 // Nothing is written for tokens past cu[B] or of a sequence whose rows are not
 // rows of q; nor, at a position below 0 or past the tables; a page that the
 // table or the pool does not hold drops only the cache row.
+#include <type_traits>
+
 namespace g950 {
 
 // Where a token goes (the same for all lanes of a wave).
@@ -74,19 +76,18 @@ __device__ __forceinline__ KvPlace kv_place(const KvAppendArgs& a, int t) {
   return w;
 }
 
-// (a, b) turned; each operation rounds on its own
-__device__ __forceinline__ void kv_turn(float a, float b, float c, float s, float& y, float& z) {
-#pragma clang fp contract(off)
-  const float ac = a * c, bs = b * s, bc = b * c, as = a * s;
-  y = ac - bs;
-  z = bc + as;
-}
-
-// an fp32 value as it stands: a following conversion to float16 does not draw
-// the operation before it into one rounding (v_fma_mixlo_f16)
+// an fp32 value as it stands: neither a sum draws the product before it into a
+// fused multiply-add (-ffp-contract=fast does so whatever a pragma says) nor a
+// conversion to float16 the operation before it into one rounding
 __device__ __forceinline__ float kv_keep(float v) {
   asm("" : "+v"(v));
   return v;
+}
+
+// (a, b) turned; each operation rounds on its own
+__device__ __forceinline__ void kv_turn(float a, float b, float c, float s, float& y, float& z) {
+  y = kv_keep(a * c) - kv_keep(b * s);
+  z = kv_keep(b * c) + kv_keep(a * s);
 }
 
 // value rounded to the model's type (dtype code) and back
@@ -115,7 +116,6 @@ __device__ __forceinline__ KvScale kv_scale(float lo, float hi, bool nan, int dt
   return r;
 }
 __device__ __forceinline__ int kv_code(float x, const KvScale& k) {
-#pragma clang fp contract(off)
   const float c = rintf((x - k.o) * k.inv) + 8.0f;  // (NaN: 0)
   return (int)fminf(fmaxf(c, 0.0f), 15.0f);
 }
@@ -201,8 +201,216 @@ __device__ __forceinline__ void kv_append_general_body(const KvAppendArgs& a) {
   }
 }
 
+// ---- whole vectors: D = 16 L dims, L a power of two; all of them turn or none
+// A wave takes a token's heads, 64 / L at a time (queries, then keys, then
+// values); lane u of a head holds dims 8 u .. and D / 2 + 8 u .., so that both
+// members of a pair (i, i + D / 2), or of two pairs (2i, 2i + 1), are its own, and
+// a row's cos and sin are loaded once for all heads.  The first heads' loads
+// are issued before the token's place is looked up (three dependent loads).
+template <typename T>
+__device__ __forceinline__ void kv_load8(const char* p, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[4 + e] = b[e];
+    }
+  } else {
+    const u32x4 w = *(const u32x4*)p;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t b = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+      v[e] = std::is_same_v<T, bf16_t> ? bf16_to_f32(b) : f16_to_f32(b);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void kv_store8(char* p, const float* v) {
+  if constexpr (sizeof(T) == 4) {
+    *(f32x4*)p = (f32x4){v[0], v[1], v[2], v[3]};
+    *(f32x4*)(p + 16) = (f32x4){v[4], v[5], v[6], v[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (std::is_same_v<T, bf16_t>)
+        w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){v[2 * e], v[2 * e + 1]}, bf16x2));
+      else
+        w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){v[2 * e], v[2 * e + 1]}, f16x2));
+    }
+    *(u32x4*)p = w;
+  }
+}
+
+// combined over the L lanes of a head
+template <class Op, int L>
+__device__ __forceinline__ float kv_row(float v) {
+  const float id = Op::identity;
+  if constexpr (L >= 2) v = Op::apply(v, dpp_f32<0xB1, 0xF>(id, v));
+  if constexpr (L >= 4) v = Op::apply(v, dpp_f32<0x4E, 0xF>(id, v));
+  if constexpr (L >= 8) v = Op::apply(v, dpp_f32<0x141, 0xF>(id, v));
+  if constexpr (L >= 16) v = Op::apply(v, dpp_f32<0x140, 0xF>(id, v));
+  return v;
+}
+
+template <typename T, int L, bool INT4>
+__device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
+  constexpr int D = 16 * L, RPW = 64 / L, SZ = (int)sizeof(T);
+  constexpr int DT = SZ == 4 ? DT_F32 : std::is_same_v<T, bf16_t> ? DT_BF16 : DT_F16;
+  const int lane = threadIdx.x & 63, u = lane % L, sub = lane / L;
+  const long long w = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = (int)(w / a.chunks), chunk = (int)(w % a.chunks);
+  if (t >= a.T) return;
+  const int slots = a.Hq + 2 * a.Hkv, groups = (slots + RPW - 1) / RPW;
+  const char* qrow = (const char*)a.q + t * a.q_st * SZ;
+  const char* krow = (const char*)a.k + t * a.k_st * SZ;
+  const char* vrow = (const char*)a.v + t * a.v_st * SZ;
+  // a lane past the last head repeats it and stores nothing
+  auto load = [&](int g, float (&x)[2][8]) {
+    const int s = min(g * RPW + sub, slots - 1);
+    const char* p = s < a.Hq ? qrow + s * a.q_sh * SZ
+                             : s < a.Hq + a.Hkv ? krow + (s - a.Hq) * a.k_sh * SZ : vrow + (s - a.Hq - a.Hkv) * a.v_sh * SZ;
+    kv_load8<T>(p + u * 8 * SZ, x[0]);
+    kv_load8<T>(p + (D / 2 + u * 8) * SZ, x[1]);
+  };
+  float x[2][8];
+  load(chunk, x);
+  const KvPlace at = kv_place(a, t);
+  if (at.seq < 0) return;
+  float c[8], s[8];
+  if (a.R) {
+    // half-split: pairs 8 u .. + 7; interleaved: 4 u .. + 3 and D / 4 + 4 u .. + 3
+    const int i0 = a.interleaved ? 4 * u : 8 * u, i1 = a.interleaved ? D / 4 + 4 * u : 8 * u + 4;
+    const long long co = at.pos * a.cos_s, so = at.pos * a.sin_s;
+    if (a.table_dtype == DT_F32) {
+      const f32x4 c0 = *(const f32x4*)((const float*)a.cos + co + i0), c1 = *(const f32x4*)((const float*)a.cos + co + i1);
+      const f32x4 s0 = *(const f32x4*)((const float*)a.sin + so + i0), s1 = *(const f32x4*)((const float*)a.sin + so + i1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[e] = c0[e]; c[4 + e] = c1[e];
+        s[e] = s0[e]; s[4 + e] = s1[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[e] = load_as_f32(a.cos, co + i0 + e, DT); c[4 + e] = load_as_f32(a.cos, co + i1 + e, DT);
+        s[e] = load_as_f32(a.sin, so + i0 + e, DT); s[4 + e] = load_as_f32(a.sin, so + i1 + e, DT);
+      }
+    }
+  }
+  for (int g = chunk; g < groups; g += a.chunks) {
+    float next[2][8];
+    if (g + a.chunks < groups) load(g + a.chunks, next);
+    const int slot = g * RPW + sub;
+    const bool is_q = slot < a.Hq, is_v = slot >= a.Hq + a.Hkv;
+    const int h = is_q ? slot : is_v ? slot - a.Hq - a.Hkv : slot - a.Hq;
+    if (a.R) {
+      float y[2][8];
+      if (a.interleaved) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            kv_turn(x[v][2 * e], x[v][2 * e + 1], c[4 * v + e], s[4 * v + e], y[v][2 * e], y[v][2 * e + 1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) kv_turn(x[0][e], x[1][e], c[e], s[e], y[0][e], y[1][e]);
+      }
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[v][e] = is_v ? x[v][e] : y[v][e];
+    }
+    if (slot < slots && (is_q || (!INT4 && at.page >= 0))) {
+      char* p = is_q ? (char*)a.q_out + (t * a.qo_st + h * a.qo_sh) * SZ
+                     : is_v ? (char*)a.v_cache + (at.page * a.vc_p + at.row * a.vc_r + h * a.vc_h) * SZ
+                            : (char*)a.k_cache + (at.page * a.kc_p + at.row * a.kc_r + h * a.kc_h) * SZ;
+      kv_store8<T>(p + u * 8 * SZ, x[0]);
+      kv_store8<T>(p + (D / 2 + u * 8) * SZ, x[1]);
+    }
+    if constexpr (INT4) {
+      if (g * RPW + RPW > a.Hq) {  // (uniform) some lane holds a key or value
+        float lo = x[0][0], hi = x[0][0];
+        bool nan = false;
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            nan |= x[v][e] != x[v][e];
+            lo = fminf(lo, x[v][e]);
+            hi = fmaxf(hi, x[v][e]);
+          }
+        lo = -kv_row<OpMax, L>(-lo);
+        hi = kv_row<OpMax, L>(hi);
+        const KvScale k = kv_scale(lo, hi, kv_row<OpMax, L>(nan ? 1.0f : 0.0f) != 0.0f, DT);
+        int code[2][8];
+        uint32_t word[2] = {0, 0};
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            code[v][e] = kv_code(x[v][e], k);
+            word[v] |= (uint32_t)code[v][e] << (4 * e);
+          }
+        if (slot < slots && !is_q) {
+          char* out = is_v ? (char*)a.v_out : (char*)a.k_out;
+          if (out) {
+            out += (is_v ? t * a.vo_st + h * a.vo_sh : t * a.ko_st + h * a.ko_sh) * SZ;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[v][e] = kv_value(code[v][e], k);
+              kv_store8<T>(out + (v * D / 2 + u * 8) * SZ, x[v]);
+            }
+          }
+          if (at.page >= 0) {
+            char* dst = is_v ? (char*)a.v_cache + (at.page * a.vc_p + at.row * a.vc_r + h * a.vc_h)
+                             : (char*)a.k_cache + (at.page * a.kc_p + at.row * a.kc_r + h * a.kc_h);
+            *(uint32_t*)(dst + 4 * u) = word[0];
+            *(uint32_t*)(dst + D / 4 + 4 * u) = word[1];
+            if (u == 0) {
+              char* sc = is_v ? (char*)a.v_scale + 2 * (at.page * a.vs_p + at.row * a.vs_r + h * a.vs_h)
+                              : (char*)a.k_scale + 2 * (at.page * a.ks_p + at.row * a.ks_r + h * a.ks_h);
+              uint32_t pair;
+              if constexpr (DT == DT_BF16)
+                pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){k.s, k.o}, bf16x2));
+              else
+                pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){k.s, k.o}, f16x2));
+              *(uint32_t*)sc = pair;
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[v][e] = next[v][e];
+  }
+}
+
 }  // namespace g950
 
 extern "C" __global__ __launch_bounds__(256) void g950_kv_append_general(const g950::KvAppendArgs a) {
   g950::kv_append_general_body(a);
 }
+
+#define G950_KV(TNAME, T, D)                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void g950_kv_append_##TNAME##_d##D(const g950::KvAppendArgs a) { \
+    g950::kv_append_body<T, D / 16, false>(a);                                                           \
+  }
+#define G950_KV4(TNAME, T, D)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256) void g950_kv_append_int4_##TNAME##_d##D(const g950::KvAppendArgs a) { \
+    g950::kv_append_body<T, D / 16, true>(a);                                                                 \
+  }
+#define G950_KV_SET(M, TNAME, T) \
+  M(TNAME, T, 32)                \
+  M(TNAME, T, 64)                \
+  M(TNAME, T, 128)               \
+  M(TNAME, T, 256)
+G950_KV_SET(G950_KV, f32, float)
+G950_KV_SET(G950_KV, bf16, g950::bf16_t)
+G950_KV_SET(G950_KV, f16, g950::f16_t)
+G950_KV_SET(G950_KV4, bf16, g950::bf16_t)
+G950_KV_SET(G950_KV4, f16, g950::f16_t)

@@ -25,7 +25,7 @@ _ORDER: dict = {}
 
 
 def _launch(op, named_tensors: dict, outputs: set, named_scalars: dict, stream=None, sync=False,
-            prepare=False):
+            prepare=False, one_device=False):
     form = (op, len(named_tensors), len(named_scalars))
     order = _ORDER.get(form)
     if order is None:
@@ -34,6 +34,11 @@ def _launch(op, named_tensors: dict, outputs: set, named_scalars: dict, stream=N
     names, outs, scalar_names = order
     tensors = [named_tensors[n] for n in names]
     scalars = [named_scalars[n] for n in scalar_names]
+    if one_device:
+        here = rt.module().device
+        for t in tensors:
+            if t.get_device() != here:
+                raise rt.G950Error(rt.USAGE, f"tensors on device {t.get_device()}, the current device is {here}")
     if prepare:
         return rt.module().prepare(op, tensors, outs, scalars, stream=stream)
     return rt.module().launch(op, tensors, outs, scalars, stream=stream, sync=sync)
@@ -248,7 +253,8 @@ def paged_append_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k_cach
                     "q_out_ptr": q_out_ptr, "k_cache_ptr": k_cache_ptr, "v_cache_ptr": v_cache_ptr,
                     "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
                     "seqused_k_ptr": seqused_k_ptr}, {"q_out_ptr", "k_cache_ptr", "v_cache_ptr"},
-                   {"interleaved": interleaved}, stream, sync, prepare)
+                   {"interleaved": interleaved}, stream, sync, prepare,
+                   one_device=True)
 
 
 def paged_append_int4_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k_out_ptr, v_out_ptr, k_cache_ptr,
@@ -265,7 +271,8 @@ def paged_append_int4_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k
                     "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
                     "seqused_k_ptr": seqused_k_ptr},
                    {"q_out_ptr", "k_out_ptr", "v_out_ptr", "k_cache_ptr", "k_scale_ptr", "v_cache_ptr", "v_scale_ptr"},
-                   {"interleaved": interleaved}, stream, sync, prepare)
+                   {"interleaved": interleaved}, stream, sync, prepare,
+                   one_device=True)
 
 
 def paged_attention_int4_kernel(q_ptr, k_cache_ptr, k_scale_ptr, v_cache_ptr, v_scale_ptr, page_table_ptr,
@@ -282,7 +289,8 @@ def paged_attention_int4_kernel(q_ptr, k_cache_ptr, k_scale_ptr, v_cache_ptr, v_
                     "seqused_k_ptr": seqused_k_ptr, "o_ptr": o_ptr, "softmax_lse_ptr": softmax_lse_ptr,
                     "workspace_ptr": workspace_ptr}, {"o_ptr", "softmax_lse_ptr", "workspace_ptr"},
                    {"seqlen_q": seqlen_q, "seqlen_k": seqlen_k, "scale_softmax": scale_softmax, "is_causal": is_causal,
-                    "window_size_left": window_size_left, "window_size_right": window_size_right}, stream, sync, prepare)
+                    "window_size_left": window_size_left, "window_size_right": window_size_right}, stream, sync, prepare,
+                   one_device=True)
 
 
 def block_norm_kernel(X, H, W_post, G, W_pre, Y, N, eps, gate_act, residual_scale, *, stream=None, sync=False,
@@ -293,7 +301,8 @@ def block_norm_kernel(X, H, W_post, G, W_pre, Y, N, eps, gate_act, residual_scal
     Empty W_post, G or W_pre (with N): that part is left out.  gate_act: 0
     none, 1 sigmoid, 2 tanh."""
     return _launch(rt.OP_BLOCK_NORM, {"X": X, "H": H, "W_post": W_post, "G": G, "W_pre": W_pre, "Y": Y, "N": N}, {"Y", "N"},
-                   {"eps": eps, "gate_act": gate_act, "residual_scale": residual_scale}, stream, sync, prepare)
+                   {"eps": eps, "gate_act": gate_act, "residual_scale": residual_scale}, stream, sync, prepare,
+                   one_device=True)
 
 
 def stream_copy(x, y, *, stream=None, sync=False, prepare=False):
@@ -416,16 +425,33 @@ def paged_append_int4(q, k, v, cos, sin, k_cache, k_scale, v_cache, v_scale, pag
     return out, k_out, v_out
 
 
+def _workspace(floats, like, stream):
+    """Memory for one call on ``stream`` (None: the current one), which torch
+    may hand on when the call returns: to later work of that stream.  None for
+    hipStreamPerThread (handle 2), which names a stream of every thread."""
+    import torch
+    handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
+    if stream is None or not floats or handle == 2:
+        return torch.empty(0 if handle == 2 else floats, dtype=torch.float32, device=like.device)
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(handle) if handle else torch.cuda.default_stream()
+    with torch.cuda.stream(stream):
+        return torch.empty(floats, dtype=torch.float32, device=like.device)
+
+
 def paged_attention_int4(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, seqlen_q, seqlen_k,
                          scale=None, causal=True, window=(-1, -1), out=None, lse=None, workspace=None, **kw):
     """Attention of q over a paged cache of 4 bits; seqlen_q is the most
-    queries, seqlen_k the most keys of a sequence.  Returns o and lse [h, tokens]."""
+    queries, seqlen_k the most keys of a sequence.  Returns o and lse [h, tokens].
+    The workspace (float32) comes from torch's allocator, on the call's stream,
+    unless given."""
     import torch
     t, h, d = q.shape
     o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
     lse = torch.empty((h, t), dtype=torch.float32, device=q.device) if lse is None else lse
     if workspace is None:
-        workspace = torch.empty(0, dtype=torch.float32, device=q.device)
+        workspace = _workspace(rt.module().attention_int4_workspace(
+            cu_seqlens_q.shape[0] - 1, h, k_cache.shape[2], d, min(seqlen_q, t), seqlen_k), q, kw.get("stream"))
     paged_attention_int4_kernel(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, o, lse,
                                 workspace, seqlen_q, seqlen_k, 1.0 / math.sqrt(d) if scale is None else float(scale),
                                 bool(causal), int(window[0]), int(window[1]), **kw)

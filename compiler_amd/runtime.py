@@ -8,6 +8,7 @@ object is missing, or no GPU is present, loading raises ``G950Error``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -47,7 +48,7 @@ DT_BOOL, DT_INT8, DT_UINT8, DT_INT16, DT_UINT16, DT_INT32 = 1, 2, 3, 4, 5, 6
 DT_UINT32, DT_INT64, DT_UINT64, DT_F16, DT_BF16, DT_F32, DT_F64 = 7, 8, 9, 10, 11, 12, 13
 
 EXPORTS = ("g950_open", "g950_launch", "g950_launch_noalloc", "g950_workspace_bytes", "g950_validate",
-           "g950_last_kernel", "g950_last_form", "g950_sync", "g950_strerror",
+           "g950_paged_attention_int4_workspace", "g950_last_kernel", "g950_last_form", "g950_sync", "g950_strerror",
            "g950_last_error", "g950_close", "g950_bundle_open", "g950_bundle_check", "g950_bundle_reason",
            "g950_bundle_count", "g950_bundle_view", "g950_bundle_scalar", "g950_bundle_exec",
            "g950_bundle_close")
@@ -119,6 +120,8 @@ def load_library():
         lib.g950_launch_noalloc.restype = ctypes.c_int
         lib.g950_workspace_bytes.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         lib.g950_workspace_bytes.restype = ctypes.c_size_t
+        lib.g950_paged_attention_int4_workspace.argtypes = [ctypes.c_void_p] + [ctypes.c_int64] * 6
+        lib.g950_paged_attention_int4_workspace.restype = ctypes.c_size_t
         lib.g950_validate.argtypes = [ctypes.c_uint32, ctypes.POINTER(View), ctypes.c_uint32,
                                       ctypes.POINTER(Scalar), ctypes.c_uint32]
         lib.g950_validate.restype = ctypes.c_int
@@ -307,6 +310,12 @@ class Module:
             stream = torch.cuda.current_stream(self.device)
         handle = ctypes.c_void_p(stream.cuda_stream if hasattr(stream, "cuda_stream") else stream)
         return int(self._lib.g950_workspace_bytes(self._handle, handle))
+
+    @functools.lru_cache(maxsize=1024)
+    def attention_int4_workspace(self, b, h, hk, d, seqlen_q, seqlen_k) -> int:
+        """Floats of workspace with which paged_attention_int4 cuts the keys as
+        far as it pays (g950_paged_attention_int4_workspace; sizes alone)."""
+        return int(self._lib.g950_paged_attention_int4_workspace(self._handle, b, h, hk, d, seqlen_q, seqlen_k)) // 4
 
     def prepare(self, op: int, tensors, outputs, scalars, stream=None):
         """Pack the call once; the returned object re-launches it with one C

@@ -219,7 +219,10 @@ typedef struct g950_scalar {
  *                      in G950_OP_FLASH_VARLEN, LSE = +inf where the sum is NaN)
  *   views   cu_seqlens_q_ptr, k_cache_ptr, k_scale_ptr, o_ptr[T,H,D],
  *           page_table_ptr, q_ptr[T,H,D], seqused_k_ptr, softmax_lse_ptr f32[H,T],
- *           v_cache_ptr, v_scale_ptr, workspace_ptr f32 (1-D, any length, also 0)
+ *           v_cache_ptr, v_scale_ptr, workspace_ptr f32 (1-D, 16-byte aligned: the
+ *           key ranges that work side by side leave their records here; any length,
+ *           also 0: as many ranges as fit; g950_paged_attention_int4_workspace gives
+ *           the length that serves all.  The number of ranges shows in the last bits)
  *   scalars is_causal, scale_softmax, seqlen_k (about the longest sequence's
  *           keys: shapes the key ranges only), seqlen_q, window_size_left,
  *           window_size_right
@@ -301,6 +304,14 @@ int g950_launch_noalloc(g950_module *module, uint32_t op, const g950_view *views
  * (operator_workspace_private/_shared, a100c/runtime/a100rt.h:180-181); it
  * lets a caller see that g950_launch_noalloc left it untouched. */
 size_t g950_workspace_bytes(g950_module *module, void *stream);
+
+/* Bytes of workspace_ptr with which G950_OP_PAGED_ATTENTION_INT4 cuts the keys
+ * as far as it pays: b sequences of at most seqlen_q queries and seqlen_k keys.
+ * 0: one range, no workspace wanted.  The caller owns the workspace, as it owns the
+ * outputs: calls that may overlap (streams, graphs) need one each.  `module`
+ * (for the device's size) may be NULL. */
+size_t g950_paged_attention_int4_workspace(g950_module *module, int64_t b, int64_t h, int64_t hk, int64_t d,
+                                           int64_t seqlen_q, int64_t seqlen_k);
 
 /* Run every contract check and the kernel choice of g950_launch without
  * touching a device (no module, no HIP call).  On success
