@@ -172,6 +172,35 @@ __device__ __forceinline__ void int4_pair(uint32_t w, float& s, float& o) {
   }
 }
 
+// Two codes of a word as numbers, (w & 0x000F000F) | bias, in one operation: with
+// both constants as literals the compiler takes two, so they are kept in
+// registers that it cannot see through.  (Not the instruction itself in inline asm:
+// the wait states that an MFMA needs behind the writer of its operand are not
+// inserted behind asm.)
+struct Int4Codes {
+  uint32_t mask = 0x000F000Fu, kbias, vbias = 0x43004300u;
+  __device__ __forceinline__ explicit Int4Codes(uint32_t kb) : kbias(kb) {
+    asm("" : "+s"(mask), "+v"(kbias), "+v"(vbias));
+  }
+  __device__ __forceinline__ uint32_t k(uint32_t w) const { return (w & mask) | kbias; }
+  __device__ __forceinline__ uint32_t v(uint32_t w) const { return (w & mask) | vbias; }
+};
+
+// 8 dims of a query row as pairs (r, r + 4), the order in which a word's codes are
+// taken; their sum is added to s
+template <bool F16>
+__device__ __forceinline__ u32x4 int4_query(const char* src, float& s) {
+  const u32x4 w = *(const u32x4*)src;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float a, b;
+    int4_pair<F16>(w[e], a, b);
+    s += a + b;
+  }
+  return (u32x4){__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
+                 __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
+}
+
 // value of `v` combined over the four lanes holding one query row
 template <class Op>
 __device__ __forceinline__ float int4_row(float v) {
@@ -179,12 +208,116 @@ __device__ __forceinline__ float int4_row(float v) {
   return Op::apply(v, __shfl_xor(v, 32));
 }
 
+// Keys of a sequence that its queries (those the grid covers) see, in tiles of 64:
+// from kbeg on, n of them; n = 0 where there is no query, else at least 1.
+struct Int4Span {
+  Int4Seq sq;
+  int nq, nk;       // queries covered, keys that can be read
+  long long base;   // visible keys of query i: [base + i - left, base + i + right]
+  int kbeg, n;
+  __device__ __forceinline__ int first_key(const AttnInt4Args& p, int i) const {
+    const long long k = base + i - p.left;
+    return p.left < 0 || k < 0 ? 0 : k > nk ? nk : (int)k;
+  }
+  __device__ __forceinline__ int last_key(const AttnInt4Args& p, int i) const {
+    const long long k = base + i + p.right;
+    return p.right < 0 || k >= nk ? nk - 1 : k < -1 ? -1 : (int)k;
+  }
+};
+__device__ __forceinline__ Int4Span int4_span(const AttnInt4Args& p, int z) {
+  Int4Span s;
+  s.sq = int4_seq(p, z);
+  s.nq = min(s.sq.nq, p.seqlen_q);
+  s.nk = p.pages > 0 ? s.sq.nk : 0;
+  s.base = (long long)p.used[z] - s.sq.nq;
+  s.kbeg = s.first_key(p, 0) / 64 * 64;
+  s.n = s.nq > 0 ? max(1, (s.last_key(p, s.nq - 1) + 1 - s.kbeg + 63) / 64) : 0;
+  return s;
+}
+
+// What a workgroup does: tiles t0 .. t1 - 1 of a block of query rows of a
+// (sequence, KV head); rec: where its partial rows go, -1 if it has all the tiles.
+// A sequence's tiles are cut into at most `splits` parts of at least 4 by its own
+// length, which lives on the device: short sequences leave no part far longer than
+// others'.  Workgroups that share a CU are about a multiple of 256 apart: the
+// sequence moves on with the part, so that they differ in length where the batch does.
+struct Int4Part {
+  int z, hk, block, t0, t1, rec;
+};
+// tiles of a part, of n
+__device__ __forceinline__ int int4_part(const AttnInt4Args& p, int n) { return max((n + p.splits - 1) / p.splits, 4); }
+__device__ __forceinline__ Int4Part int4_deal(const AttnInt4Args& p, Int4Span& sp) {
+  const int pairs = p.B * p.Hkv, units = pairs * p.row_blocks;
+  const int split = blockIdx.x / units, unit = blockIdx.x % units;
+  Int4Part w;
+  w.z = (unit % pairs / p.Hkv + split * p.turn) % p.B;
+  w.hk = unit % p.Hkv;
+  w.block = p.row_blocks - 1 - unit / pairs;  // those that see most keys first
+  sp = int4_span(p, w.z);
+  const int c = int4_part(p, sp.n);
+  w.t0 = split * c;
+  w.t1 = min(sp.n, w.t0 + c);
+  w.rec = sp.n <= c ? -1 : ((w.z * p.Hkv + w.hk) * p.row_blocks + w.block) * p.splits + split;
+  return w;
+}
+
+// The four waves' partial rows of a workgroup joined: row r's O unnormalised in wave w's
+// LDS (16-byte chunks XOR-swizzled by the row), its maximum (log2 units) and sum in
+// ml[w][r].  Writes o and lse, or record rec0.
+template <int D, bool F16, int ROWS, int WLDS>
+__device__ __forceinline__ void int4_finish(const AttnInt4Args& p, const char* lds, const float* ml, const Int4Seq& sq,
+                                            int hk, int rec0, int row0, int nrows) {
+  const int G = p.group;
+  constexpr int CPR = D / 4;  // 16-byte chunks (4 d) per row
+  for (int it = threadIdx.x; it < nrows * CPR; it += I4_WAVES * 64) {
+    const int r = it / CPR, c = it % CPR;
+    float m = ml[2 * r];
+#pragma unroll
+    for (int w = 1; w < I4_WAVES; ++w) m = fmaxf(m, ml[2 * (w * ROWS + r)]);
+    f32x4 sum = {};
+    float lt = 0.0f;
+#pragma unroll
+    for (int w = 0; w < I4_WAVES; ++w) {
+      const float mw = ml[2 * (w * ROWS + r)], lw = ml[2 * (w * ROWS + r) + 1];
+      // no finite score: no key of this row (l = 0), or only NaN ones
+      const float f = mw == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      lt = fmaf(f, lw, lt);
+      const f32x4 ow = *(const f32x4*)(lds + w * WLDS + r * D * 4 + ((c ^ (r & 15)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, ow[e], sum[e]);
+    }
+    if (rec0 >= 0) {
+      const long long rec = (long long)rec0 * ROWS + r;
+      *(f32x4*)(p.part + rec * D + c * 4) = sum;
+      if (c == 0) {
+        p.ml[2 * rec] = m;
+        p.ml[2 * rec + 1] = lt;
+      }
+      continue;
+    }
+    const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
+    const bool empty = !(lt > 0.0f);  // zero or NaN
+    const float inv = empty ? 1.0f : 1.0f / lt;
+    char* dst = (char*)p.o + 2 * ((long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + c * 4);
+    if constexpr (F16)
+      *(u32x2*)dst = (u32x2){__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[0] * inv, sum[1] * inv}, f16x2)),
+                             __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[2] * inv, sum[3] * inv}, f16x2))};
+    else
+      *(u32x2*)dst = (u32x2){__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[0] * inv, sum[1] * inv}, bf16x2)),
+                             __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[2] * inv, sum[3] * inv}, bf16x2))};
+    if (c == 0)
+      p.lse[(long long)h * p.lse_h + (long long)(sq.q0 + i) * p.lse_t] =
+          empty ? __builtin_huge_valf() : (m + __log2f(lt)) * 0.69314718055994530942f;
+  }
+}
+
 template <int D, bool F16, int RT>
 __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr int RB = D / 2;                       // bytes of a row
   constexpr int KT = I4_TK * RB;                  // bytes of a tile's K (or V)
   constexpr int TILE = 2 * KT + 256;              // K, V, 64 pairs
-  constexpr int ST = D == 64 ? 7 : D == 128 ? 4 : 2;  // tiles in flight per wave
+  // tiles in flight per wave: 35 KiB of LDS per workgroup with one row tile, 70 with two
+  constexpr int ST = RT == 1 ? (D == 64 ? 4 : 2) : (D == 64 ? 7 : 4);
   constexpr int RING = ST * TILE;
   constexpr int DC = KT / 1024;                   // DMA instructions of a tile's K
   constexpr int DPT = 2 * DC + 1;
@@ -197,37 +330,28 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr int ROWS = 16 * RT;
   constexpr uint32_t KBIAS = F16 ? 0x64006400u : 0x43004300u;
   constexpr float KOFF = F16 ? 1032.0f : 136.0f;
-  static_assert(ROWS * D * 4 <= RING, "a wave's partial O fits its ring");
-  __shared__ __attribute__((aligned(1024))) char lds[I4_WAVES * RING];
+  constexpr int WLDS = RING > ROWS * D * 4 ? RING : ROWS * D * 4;  // a wave's LDS: its ring, then its partial O
+  __shared__ __attribute__((aligned(1024))) char lds[I4_WAVES * WLDS];
   __shared__ float ml[I4_WAVES][ROWS][2];
   if (blockDim.x != I4_WAVES * 64) return;  // launch shape must match the kernel
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, l16 = lane & 15;
-  const int pairs = p.B * p.Hkv;
-  const int pair = blockIdx.x % pairs;
-  const int block = (blockIdx.x / pairs) % p.row_blocks, split = blockIdx.x / pairs / p.row_blocks;
-  const int z = pair / p.Hkv, hk = pair % p.Hkv;
   const int G = p.group;
-  const Int4Seq sq = int4_seq(p, z);
-  const int rows = min(sq.nq, p.seqlen_q) * G;  // of this sequence and KV head
-  const int row0 = block * ROWS;
-  if (row0 >= rows) return;
+  Int4Span sp;
+  const Int4Part w = int4_deal(p, sp);
+  const int hk = w.hk;
+  const Int4Seq& sq = sp.sq;
+  const int rows = sp.nq * G;  // of this sequence and KV head
+  const int row0 = w.block * ROWS;
+  if (row0 >= rows || w.t0 >= sp.n) return;
   const int nrows = min(ROWS, rows - row0);
-  // visible keys of query i: [base + i - left, base + i + right] within the sequence
-  const long long base = (long long)p.used[z] - sq.nq;
-  const int nk = p.pages > 0 ? sq.nk : 0;
-  auto first_key = [&](int i) {
-    const long long k = base + i - p.left;
-    return p.left < 0 || k < 0 ? 0 : k > nk ? nk : (int)k;
-  };
-  auto last_key = [&](int i) {
-    const long long k = base + i + p.right;
-    return p.right < 0 || k >= nk ? nk - 1 : k < -1 ? -1 : (int)k;
-  };
+  auto first_key = [&](int i) { return sp.first_key(p, i); };
+  auto last_key = [&](int i) { return sp.last_key(p, i); };
   const int i_lo = row0 / G, i_hi = (row0 + nrows - 1) / G;
-  const int kend = last_key(i_hi) + 1, kbeg = first_key(i_lo) / I4_TK * I4_TK;
   const int all_from = first_key(i_hi), all_to = last_key(i_lo);  // keys every row sees
+  const int lo = max(sp.kbeg + 64 * w.t0, first_key(i_lo) / I4_TK * I4_TK);
+  const int hi = min(last_key(i_hi) + 1, w.t1 < sp.n ? sp.kbeg + 64 * w.t1 : 0x7FFFFFFF);
 
   // query fragments: row l16 of tile rt; lane group g4 holds dims g4 D / 4 ..,
   // word ks their 8 from 8 ks on, as pairs (r, r + 4)
@@ -244,20 +368,12 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     float s = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const u32x4 w = *(const u32x4*)(src + ks * 16);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float a, b;
-        int4_pair<F16>(w[e], a, b);
-        s += a + b;
-      }
-      qf[rt][ks] = (u32x4){__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
-                           __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
+      qf[rt][ks] = int4_query<F16>(src + ks * 16, s);
     }
     qsum[rt] = int4_row<OpSum>(s);
   }
 
-  char* ring = lds + wave * RING;
+  char* ring = lds + wave * WLDS;
   const uint32_t ring32 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring;
   const char* kbase = (const char*)p.k + (long long)hk * p.k_h;
   const char* vbase = (const char*)p.v + (long long)hk * p.v_h;
@@ -268,13 +384,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   const char* sbase = lane < 32 ? (const char*)p.ks + 2 * ((long long)hk * p.ks_h + (long long)skey * p.ks_r)
                                 : (const char*)p.vs + 2 * ((long long)hk * p.vs_h + (long long)skey * p.vs_r);
   const uint32_t s_p = 2 * (uint32_t)(lane < 32 ? p.ks_p : p.vs_p), s_r = 2 * (uint32_t)(lane < 32 ? p.ks_r : p.vs_r);
-  const int* table = p.table + (long long)z * p.table_s;
-
-  int lo = kbeg, hi = kend;
-  if (p.splits > 1) {
-    lo = max(lo, split * p.chunk);
-    hi = split + 1 < p.splits ? min(hi, (split + 1) * p.chunk) : hi;
-  }
+  const int* table = p.table + (long long)w.z * p.table_s;
   const int ntiles = hi > lo ? (hi - lo + I4_TK - 1) / I4_TK : 0;
   const int nloc = ntiles > wave ? (ntiles - wave + I4_WAVES - 1) / I4_WAVES : 0;
 
@@ -331,6 +441,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     for (int b = 0; b < NB; ++b) o[rt][b] = (f32x4){};
   }
   const float c2 = p.scale_log2;
+  const Int4Codes two(KBIAS);
   const int kperm = (l16 >> 2) + 4 * (l16 & 3);  // K row of S^T's row l16
   const uint32_t m136 = 0xC308C308u;             // -136 in bfloat16, twice
   const u32x4 unbias = {m136, m136, m136, m136};
@@ -368,7 +479,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
       for (int ks = 0; ks < KS; ++ks) {
         u32x4 kf;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) kf[r] = ((kw[ks] >> (4 * r)) & 0x000F000Fu) | KBIAS;
+        for (int r = 0; r < 4; ++r) kf[r] = two.k(kw[ks] >> (4 * r));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt] = int4_mfma<F16>(kf, qf[rt][ks], acc[rt]);
       }
@@ -441,10 +552,10 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
         for (int e = 0; e < 4; ++e) zo[rt] = fmaf(pe[e], zp[e], zo[rt]);
         l[rt] += (pe[0] + pe[1]) + (pe[2] + pe[3]);
       }
-      auto two = [](float a, float b) {
+      auto pack = [](float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
       };
-      pf[rt] = (u32x4){two(ps[0][0], ps[0][1]), two(ps[0][2], ps[0][3]), two(ps[1][0], ps[1][1]), two(ps[1][2], ps[1][3])};
+      pf[rt] = (u32x4){pack(ps[0][0], ps[0][1]), pack(ps[0][2], ps[0][3]), pack(ps[1][0], ps[1][1]), pack(ps[1][2], ps[1][3])};
       ob[rt] = int4_mfma<false>(unbias, pf[rt], ob[rt]);
     }
     // V: words of keys g4 + 4 e of both halves, two keys side by side
@@ -469,7 +580,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
       for (int n = 0; n < VN; ++n) {
         u32x4 vf;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) vf[r] = ((half[n / 4][r] >> (4 * (n & 3))) & 0x000F000Fu) | 0x43004300u;
+        for (int r = 0; r < 4; ++r) vf[r] = two.v(half[n / 4][r] >> (4 * (n & 3)));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) o[rt][c * VN + n] = int4_mfma<false>(vf, pf[rt], o[rt][c * VN + n]);
       }
@@ -503,95 +614,58 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     }
   }
   __syncthreads();
-  constexpr int CPR = D / 4;  // 16-byte chunks (4 d) per row
-  for (int it = tid; it < nrows * CPR; it += I4_WAVES * 64) {
-    const int r = it / CPR, c = it % CPR;
-    float m = ml[0][r][0];
-#pragma unroll
-    for (int w = 1; w < I4_WAVES; ++w) m = fmaxf(m, ml[w][r][0]);
-    f32x4 sum = {};
-    float lt = 0.0f;
-#pragma unroll
-    for (int w = 0; w < I4_WAVES; ++w) {
-      const float mw = ml[w][r][0], lw = ml[w][r][1];
-      // no finite score: no key of this row (l = 0), or only NaN ones
-      const float f = mw == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      lt = fmaf(f, lw, lt);
-      const f32x4 ow = *(const f32x4*)(lds + w * RING + r * D * 4 + ((c ^ (r & 15)) << 4));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, ow[e], sum[e]);
-    }
-    if (p.splits > 1) {
-      const long long rec = (((long long)pair * p.row_blocks + block) * p.splits + split) * ROWS + r;
-      *(f32x4*)(p.part + rec * D + c * 4) = sum;
-      if (c == 0) {
-        p.ml[2 * rec] = m;
-        p.ml[2 * rec + 1] = lt;
-      }
-      continue;
-    }
-    const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
-    const bool empty = !(lt > 0.0f);  // zero or NaN
-    const float inv = empty ? 1.0f : 1.0f / lt;
-    char* dst = (char*)p.o + 2 * ((long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + c * 4);
-    if constexpr (F16)
-      *(u32x2*)dst = (u32x2){__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[0] * inv, sum[1] * inv}, f16x2)),
-                             __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[2] * inv, sum[3] * inv}, f16x2))};
-    else
-      *(u32x2*)dst = (u32x2){__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[0] * inv, sum[1] * inv}, bf16x2)),
-                             __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){sum[2] * inv, sum[3] * inv}, bf16x2))};
-    if (c == 0)
-      p.lse[(long long)h * p.lse_h + (long long)(sq.q0 + i) * p.lse_t] =
-          empty ? __builtin_huge_valf() : (m + __log2f(lt)) * 0.69314718055994530942f;
-  }
+  int4_finish<D, F16, ROWS, WLDS>(p, lds, &ml[0][0][0], sq, hk, w.rec, row0, nrows);
 }
 
-// Joins the key ranges: one wave per query row, lane s holds range s's maximum
-// and sum (at most 64 ranges), D / 64 outputs per lane.
+// Joins the parts of a block of query rows: one wave per row, lane s holds part s's
+// maximum and sum (at most 64 parts), D / 64 outputs per lane.
 template <int D, bool F16, int ROWS>
 __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
   const int lane = threadIdx.x & 63;
   const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = p.row_blocks * ROWS;
-  const int pair = (int)(item / per), row = (int)(item % per);
-  if (pair >= p.B * p.Hkv) return;
+  const int id = (int)(item / p.merge_rows), r = (int)(item % p.merge_rows);
+  if (id >= p.B * p.Hkv * p.row_blocks) return;
+  const int block = id % p.row_blocks, pair = id / p.row_blocks;
   const int z = pair / p.Hkv, hk = pair % p.Hkv;
-  const Int4Seq sq = int4_seq(p, z);
-  if (row >= min(sq.nq, p.seqlen_q) * p.group) return;
-  const long long rec = ((long long)pair * p.row_blocks + row / ROWS) * p.splits * ROWS + row % ROWS;
+  const int row = block * ROWS + r;
+  const Int4Span sp = int4_span(p, z);
+  if (row >= sp.nq * p.group) return;
+  const int c = int4_part(p, sp.n), count = (sp.n + c - 1) / c;
+  if (count <= 1) return;  // its workgroup had all of it
+  const long long rec = (long long)id * p.splits * ROWS + r;
   float m = -__builtin_huge_valf(), l = 0.0f;
-  if (lane < p.splits) {
+  if (lane < count) {
     m = p.ml[2 * (rec + (long long)lane * ROWS)];
     l = p.ml[2 * (rec + (long long)lane * ROWS) + 1];
   }
   const float mt = wave_reduce<OpMax>(m);
-  // no finite score in a range: nothing seen (O = l = 0), or only NaN, which stays
+  // no finite score in a part: nothing seen (O = l = 0), or only NaN, which stays
   const float f = m == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(m - mt);
   const float lt = wave_reduce<OpSum>(f * l);
   constexpr int E = D / 64, U = 8;
   float acc[E] = {};
-  for (int s0 = 0; s0 < p.splits; s0 += U) {
+  for (int s0 = 0; s0 < count; s0 += U) {
     float v[U][E];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[u][e] = p.part[(rec + (long long)min(s0 + u, p.splits - 1) * ROWS) * D + lane * E + e];
+      for (int e = 0; e < E; ++e) v[u][e] = p.part[(rec + (long long)min(s0 + u, count - 1) * ROWS) * D + lane * E + e];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s0 + u, 63)));
-      if (s0 + u < p.splits)
+      if (s0 + u < count)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[u][e], acc[e]);
     }
   }
   const int i = row / p.group, h = hk * p.group + row % p.group;
-  const bool empty = !(lt > 0.0f);
+  const bool empty = !(lt > 0.0f);  // zero or NaN
   const float inv = empty ? 1.0f : 1.0f / lt;
-  uint16_t* dst = (uint16_t*)p.o + (long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + lane * E;
+  uint16_t* dst = (uint16_t*)p.o + (long long)(sp.sq.q0 + i) * p.o_st + (long long)h * p.o_sh + lane * E;
 #pragma unroll
   for (int e = 0; e < E; ++e) dst[e] = F16 ? f32_to_f16(acc[e] * inv) : f32_to_bf16(acc[e] * inv);
   if (lane == 0)
-    p.lse[(long long)h * p.lse_h + (long long)(sq.q0 + i) * p.lse_t] =
+    p.lse[(long long)h * p.lse_h + (long long)(sp.sq.q0 + i) * p.lse_t] =
         empty ? __builtin_huge_valf() : (mt + __log2f(lt)) * 0.69314718055994530942f;
 }
 
@@ -600,9 +674,9 @@ __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
 extern "C" __global__ __launch_bounds__(64) void g950_attn_int4_general(const g950::AttnInt4Args p) {
   g950::attn_int4_general_body(p);
 }
-// Two workgroups per CU (256 registers).
+// Four workgroups per CU with one row tile (128 registers), else two.
 #define G950_INT4(NAME, D, F16, RT)                                                                    \
-  extern "C" __global__ __launch_bounds__(256, 2) void NAME##_r##RT(const g950::AttnInt4Args p) {      \
+  extern "C" __global__ __launch_bounds__(256, RT == 1 && D < 256 ? 4 : 2) void NAME##_r##RT(const g950::AttnInt4Args p) {      \
     g950::attn_int4_body<D, F16, RT>(p);                                                               \
   }                                                                                                    \
   extern "C" __global__ __launch_bounds__(256) void NAME##_r##RT##_merge(const g950::AttnInt4Args p) { \

@@ -212,9 +212,11 @@ struct AttnInt4Args {
   int group;                // query heads per KV head
   int seqlen_q;             // queries per sequence that the grid covers
   int row_blocks;           // blocks of query rows per (sequence, KV head)
-  int splits, chunk;        // key ranges, keys of all but the last
-  float* part;              // [pairs * row_blocks * splits][rows][D] unnormalised O
-  float* ml;                // [pairs * row_blocks * splits][rows][2] maximum (log2 units), sum
+  int splits;               // parts that a block's keys are cut into at most
+  int turn;                 // sequences to move on by from one part to the next
+  int merge_rows;           // rows of a block that any sequence can have
+  float* part;              // [blocks * splits][rows][D] unnormalised O
+  float* ml;                // [blocks * splits][rows][2] maximum (log2 units), sum
 };
 
 // Norms around a block (block_norm.hip).

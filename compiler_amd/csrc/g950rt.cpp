@@ -1856,27 +1856,27 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   return launch(m, "g950_kv_append_general", (unsigned)std::min((rows + 3) / 4, 1ll << 20), 256u, a, stream);
 }
 
-// How attention over the 4-bit cache cuts a call: blocks of 16 or 32 query rows
-// per (sequence, KV head), and key ranges.
+// How attention over the 4-bit cache cuts a call: blocks of 16 or 32 query rows per
+// (sequence, KV head), and parts of their keys, whose records need a workspace.
 struct Int4Shape {
-  long long rows;        // query rows of a workgroup
+  long long rows;        // query rows of a block
   long long row_blocks;  // per (sequence, KV head)
   long long blocks;      // of the call
-  long long splits;      // key ranges wanted
+  long long splits;      // parts wanted
 };
-constexpr long long kInt4Target = 4, kInt4MinKeys = 256, kInt4OneRange = 512;
+constexpr long long kInt4Target = 4, kInt4MinKeys = 256, kInt4OneRange = 1024;
 
 Int4Shape int4_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
                      long long seqlen_k) {
   const long long cus = m ? m->cus : 256, rows = seqlen_q * (h / hk);
-  Int4Shape f;
+  Int4Shape f{};
   f.rows = d == 256 || rows <= 16 ? 16 : 32;
   f.row_blocks = (rows + f.rows - 1) / f.rows;
   f.blocks = b * hk * f.row_blocks;
-  f.splits = f.blocks ? std::min({(kInt4Target * cus + f.blocks - 1) / f.blocks, (seqlen_k + kInt4MinKeys - 1) / kInt4MinKeys,
-                                  64ll})  // the merge holds a row's ranges in one wave's lanes
-                      : 1;
-  f.splits = seqlen_k <= kInt4OneRange ? 1 : std::max(f.splits, 1ll);
+  f.splits = 1;
+  if (f.blocks && seqlen_k > kInt4OneRange)
+    f.splits = std::max(1ll, std::min({kInt4Target * cus / f.blocks, (seqlen_k + kInt4MinKeys - 1) / kInt4MinKeys,
+                                       64ll}));  // the merge holds a row's parts in one wave's lanes
   return f;
 }
 
@@ -1952,7 +1952,7 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
   };
   auto m4 = [](const View& w) {
     return w.addr() % 4 == 0 && w.stride[0] % 2 == 0 && w.stride[1] % 2 == 0 && w.stride[2] % 2 == 0 && w.stride[0] >= 0 &&
-           w.stride[0] < (1ll << 30) && w.stride[1] >= 0 && w.stride[1] < (1ll << 30);
+           w.stride[0] < (1ll << 30) && w.stride[1] >= 0 && w.stride[1] < (1ll << 26);
   };
   const long long most = 0x7FFF0000;  // keys: positions a little past the last one stay within 32 bits
   SK = std::min(SK, most);
@@ -1962,22 +1962,22 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
   if (fast && rows) {
     const Int4Shape f = int4_shape(m, a.B, H, HK, D, std::min(SQ, T), SK);
     if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
-    // as many key ranges as the workspace holds records for
-    const long long rec = f.blocks * f.rows * (D + 2);
-    const long long splits = std::min(f.splits, ws.shape[0] / rec);
+    // as many parts as the workspace holds records for
     a.row_blocks = (int)f.row_blocks;
-    a.splits = (int)std::max(splits, 1ll);
-    a.chunk = (int)std::min(((SK + a.splits - 1) / a.splits + 127) / 128 * 128, most);
+    a.splits = (int)std::max(std::min(f.splits, ws.shape[0] / (f.blocks * f.rows * (D + 2))), 1ll);
+    a.turn = std::max(a.B / a.splits, 1);
+    a.merge_rows = (int)std::min(f.rows, std::min(SQ, T) * (H / HK));
     a.part = (float*)ws.v->data;
     a.ml = a.part + f.blocks * f.rows * a.splits * D;
-    if (f.blocks * a.splits > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+    const long long grid = f.blocks * a.splits;
+    if (grid > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
     char name[64];
     const int n = snprintf(name, sizeof name, "g950_attn_int4_%s_d%lld_r%lld", dt == G950_DTYPE_BFLOAT16 ? "bf16" : "f16", D,
                            f.rows / 16);
-    if (int rc = launch(m, name, (unsigned)(f.blocks * a.splits), 256u, a, stream)) return rc;
+    if (int rc = launch(m, name, (unsigned)grid, 256u, a, stream)) return rc;
     if (a.splits == 1) return G950_OK;
     snprintf(name + n, sizeof name - n, "_merge");
-    return launch(m, name, (unsigned)((f.blocks * f.rows + 3) / 4), 256u, a, stream);
+    return launch(m, name, (unsigned)((f.blocks * a.merge_rows + 3) / 4), 256u, a, stream);
   }
   return launch(m, "g950_attn_int4_general", (unsigned)rows, 64u, a, stream);
 }
@@ -2189,12 +2189,10 @@ size_t g950_paged_attention_int4_workspace(g950_module* m, int64_t b, int64_t h,
                                            int64_t seqlen_k) {
   const int64_t most = 1ll << 31;
   if (b <= 0 || hk <= 0 || h < hk || h % hk || d <= 0 || seqlen_q <= 0 || seqlen_k <= 0 || b > most || h > 65536 || d > 256 ||
-      seqlen_q > most || seqlen_k > most)
+      seqlen_q > most || seqlen_k > most || (d != 64 && d != 128 && d != 256))
     return 0;
   const Int4Shape f = int4_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
-  // a call of more blocks than there are places for takes one range
-  if (f.splits <= 1 || (d != 64 && d != 128 && d != 256)) return 0;
-  return (size_t)f.blocks * (size_t)f.rows * (size_t)f.splits * (size_t)(d + 2) * 4;
+  return f.splits > 1 ? (size_t)(f.blocks * f.rows * f.splits * (d + 2)) * 4 : 0;
 }
 
 int g950_sync(void* stream) {

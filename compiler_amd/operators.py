@@ -13,6 +13,7 @@ semantics, attention's ``CAUSAL``, is a keyword argument.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -25,7 +26,7 @@ _ORDER: dict = {}
 
 
 def _launch(op, named_tensors: dict, outputs: set, named_scalars: dict, stream=None, sync=False,
-            prepare=False, one_device=False):
+            prepare=False):
     form = (op, len(named_tensors), len(named_scalars))
     order = _ORDER.get(form)
     if order is None:
@@ -34,14 +35,22 @@ def _launch(op, named_tensors: dict, outputs: set, named_scalars: dict, stream=N
     names, outs, scalar_names = order
     tensors = [named_tensors[n] for n in names]
     scalars = [named_scalars[n] for n in scalar_names]
-    if one_device:
-        here = rt.module().device
-        for t in tensors:
-            if t.get_device() != here:
-                raise rt.G950Error(rt.USAGE, f"tensors on device {t.get_device()}, the current device is {here}")
     if prepare:
         return rt.module().prepare(op, tensors, outs, scalars, stream=stream)
     return rt.module().launch(op, tensors, outs, scalars, stream=stream, sync=sync)
+
+
+def _launch_sorted(op, tensors, outs, scalars, stream, sync, prepare):
+    """The call with its tensors, output flags and scalars in sorted-name order
+    (no dictionaries on the way); all tensors live on the current device."""
+    mod = rt.module()
+    here = mod.device
+    for t in tensors:
+        if t.get_device() != here:
+            raise rt.G950Error(rt.USAGE, f"tensors on device {t.get_device()}, the current device is {here}")
+    if prepare:
+        return mod.prepare(op, tensors, outs, scalars, stream=stream)
+    return mod.launch(op, tensors, outs, scalars, stream=stream, sync=sync)
 
 
 def softmax_kernel(x_ptr, y_ptr, n_cols, *, stream=None, sync=False, prepare=False):
@@ -248,13 +257,11 @@ def paged_append_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k_cach
     k/v [tokens, hk, d], cos/sin [positions, r / 2] (the first r dims turn), caches
     [pages, block_size, hk, d], page_table [b, pages], cu_seqlens_q [b + 1],
     seqused_k [b] (keys of each sequence, the new ones among them)."""
-    return _launch(rt.OP_PAGED_APPEND,
-                   {"q_ptr": q_ptr, "k_ptr": k_ptr, "v_ptr": v_ptr, "cos_ptr": cos_ptr, "sin_ptr": sin_ptr,
-                    "q_out_ptr": q_out_ptr, "k_cache_ptr": k_cache_ptr, "v_cache_ptr": v_cache_ptr,
-                    "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
-                    "seqused_k_ptr": seqused_k_ptr}, {"q_out_ptr", "k_cache_ptr", "v_cache_ptr"},
-                   {"interleaved": interleaved}, stream, sync, prepare,
-                   one_device=True)
+    return _launch_sorted(rt.OP_PAGED_APPEND,
+                          (cos_ptr, cu_seqlens_q_ptr, k_cache_ptr, k_ptr, page_table_ptr, q_out_ptr, q_ptr,
+                           seqused_k_ptr, sin_ptr, v_cache_ptr, v_ptr),
+                          (False, False, True, False, False, True, False, False, False, True, False), (interleaved,),
+                          stream, sync, prepare)
 
 
 def paged_append_int4_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k_out_ptr, v_out_ptr, k_cache_ptr,
@@ -264,15 +271,11 @@ def paged_append_int4_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k
     codes uint8 [pages, block_size, hk, d / 2], scale and offset [pages,
     block_size, hk, 2] in the model's type.  k_out/v_out [tokens, hk, d]: the
     appended rows as the cache holds them (empty: not wanted)."""
-    return _launch(rt.OP_PAGED_APPEND_INT4,
-                   {"q_ptr": q_ptr, "k_ptr": k_ptr, "v_ptr": v_ptr, "cos_ptr": cos_ptr, "sin_ptr": sin_ptr,
-                    "q_out_ptr": q_out_ptr, "k_out_ptr": k_out_ptr, "v_out_ptr": v_out_ptr, "k_cache_ptr": k_cache_ptr,
-                    "k_scale_ptr": k_scale_ptr, "v_cache_ptr": v_cache_ptr, "v_scale_ptr": v_scale_ptr,
-                    "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
-                    "seqused_k_ptr": seqused_k_ptr},
-                   {"q_out_ptr", "k_out_ptr", "v_out_ptr", "k_cache_ptr", "k_scale_ptr", "v_cache_ptr", "v_scale_ptr"},
-                   {"interleaved": interleaved}, stream, sync, prepare,
-                   one_device=True)
+    return _launch_sorted(rt.OP_PAGED_APPEND_INT4,
+                          (cos_ptr, cu_seqlens_q_ptr, k_cache_ptr, k_out_ptr, k_ptr, k_scale_ptr, page_table_ptr,
+                           q_out_ptr, q_ptr, seqused_k_ptr, sin_ptr, v_cache_ptr, v_out_ptr, v_ptr, v_scale_ptr),
+                          (False, False, True, True, False, True, False, True, False, False, False, True, True, False,
+                           True), (interleaved,), stream, sync, prepare)
 
 
 def paged_attention_int4_kernel(q_ptr, k_cache_ptr, k_scale_ptr, v_cache_ptr, v_scale_ptr, page_table_ptr,
@@ -283,14 +286,12 @@ def paged_attention_int4_kernel(q_ptr, k_cache_ptr, k_scale_ptr, v_cache_ptr, v_
     reference counterpart): q/o [tokens, h, d], lse float32 [h, tokens], the
     cache and its lists as paged_append_int4_kernel fills them; windows as in
     flash_varlen_fwd_kernel, sizes below 0 without limit."""
-    return _launch(rt.OP_PAGED_ATTENTION_INT4,
-                   {"q_ptr": q_ptr, "k_cache_ptr": k_cache_ptr, "k_scale_ptr": k_scale_ptr, "v_cache_ptr": v_cache_ptr,
-                    "v_scale_ptr": v_scale_ptr, "page_table_ptr": page_table_ptr, "cu_seqlens_q_ptr": cu_seqlens_q_ptr,
-                    "seqused_k_ptr": seqused_k_ptr, "o_ptr": o_ptr, "softmax_lse_ptr": softmax_lse_ptr,
-                    "workspace_ptr": workspace_ptr}, {"o_ptr", "softmax_lse_ptr", "workspace_ptr"},
-                   {"seqlen_q": seqlen_q, "seqlen_k": seqlen_k, "scale_softmax": scale_softmax, "is_causal": is_causal,
-                    "window_size_left": window_size_left, "window_size_right": window_size_right}, stream, sync, prepare,
-                   one_device=True)
+    return _launch_sorted(rt.OP_PAGED_ATTENTION_INT4,
+                          (cu_seqlens_q_ptr, k_cache_ptr, k_scale_ptr, o_ptr, page_table_ptr, q_ptr, seqused_k_ptr,
+                           softmax_lse_ptr, v_cache_ptr, v_scale_ptr, workspace_ptr),
+                          (False, False, False, True, False, False, False, True, False, False, True),
+                          (is_causal, scale_softmax, seqlen_k, seqlen_q, window_size_left, window_size_right), stream,
+                          sync, prepare)
 
 
 def block_norm_kernel(X, H, W_post, G, W_pre, Y, N, eps, gate_act, residual_scale, *, stream=None, sync=False,
@@ -300,9 +301,9 @@ def block_norm_kernel(X, H, W_post, G, W_pre, Y, N, eps, gate_act, residual_scal
     residual_scale X + act(G) u, N = Y rsqrt(mean(Y^2) + eps) W_pre, by rows.
     Empty W_post, G or W_pre (with N): that part is left out.  gate_act: 0
     none, 1 sigmoid, 2 tanh."""
-    return _launch(rt.OP_BLOCK_NORM, {"X": X, "H": H, "W_post": W_post, "G": G, "W_pre": W_pre, "Y": Y, "N": N}, {"Y", "N"},
-                   {"eps": eps, "gate_act": gate_act, "residual_scale": residual_scale}, stream, sync, prepare,
-                   one_device=True)
+    return _launch_sorted(rt.OP_BLOCK_NORM, (G, H, N, W_post, W_pre, X, Y),
+                          (False, False, True, False, False, False, True), (eps, gate_act, residual_scale), stream, sync,
+                          prepare)
 
 
 def stream_copy(x, y, *, stream=None, sync=False, prepare=False):
@@ -385,6 +386,13 @@ def attention(q, k, v, scale=None, causal=True, out=None, lse=None, **kw):
     return o, lse
 
 
+@functools.lru_cache(maxsize=None)
+def _none(dtype, device, rank):
+    """A view without elements: an argument left out."""
+    import torch
+    return torch.empty((0,) * rank, dtype=dtype, device=device)
+
+
 def paged_append(q, k, v, cos, sin, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, interleaved=False,
                  out=None, **kw):
     """Appends k and v to the cache and returns the rotated q (``out=q``: in
@@ -418,7 +426,7 @@ def paged_append_int4(q, k, v, cos, sin, k_cache, k_scale, v_cache, v_scale, pag
     if values:
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
         v_out = torch.empty_like(v, memory_format=torch.contiguous_format) if v_out is None else v_out
-    none = k.new_empty((0, 0, 0)) if k_out is None or v_out is None else None
+    none = _none(k.dtype, k.device, 3)
     paged_append_int4_kernel(q, k, v, cos, sin, out, none if k_out is None else k_out, none if v_out is None else v_out,
                              k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, bool(interleaved),
                              **kw)
@@ -473,11 +481,10 @@ def block_norm(x, h, w_pre, eps, w_post=None, gate=None, gate_act=None, residual
     n = None
     if w_pre is not None:
         n = torch.empty_like(x) if norm_out is None else norm_out
-    none1 = x.new_empty(0) if w_post is None or w_pre is None else None
-    none2 = x.new_empty((0, 0)) if gate is None or n is None else None
-    if gate is not None:
+    none = _none(x.dtype, x.device, 1)
+    if gate is not None and gate.shape != x.shape:
         gate = gate.expand(x.shape)
-    block_norm_kernel(x, h, none1 if w_post is None else w_post, none2 if gate is None else gate,
-                      none1 if w_pre is None else w_pre, y, none2 if n is None else n, float(eps), _GATE_ACTS[gate_act],
-                      float(residual_scale), **kw)
+    block_norm_kernel(x, h, none if w_post is None else w_post, _none(x.dtype, x.device, 2) if gate is None else gate,
+                      none if w_pre is None else w_pre, y, _none(x.dtype, x.device, 2) if n is None else n, float(eps),
+                      _GATE_ACTS[gate_act], float(residual_scale), **kw)
     return y, n
