@@ -146,6 +146,11 @@ __device__ __forceinline__ void dma_lane16(const char* src, uint32_t lds_dst) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_dst);
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
 }
+// the same from a wave-uniform base and a 32-bit lane offset
+__device__ __forceinline__ void dma_base16(const char* base, uint32_t off, uint32_t lds_dst) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_dst);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(m0) : "memory");
+}
 __device__ __forceinline__ void dma_lane4(const char* src, uint32_t lds_dst) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_dst);
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0) : "memory");
@@ -316,9 +321,10 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr int RB = D / 2;                       // bytes of a row
   constexpr int KT = I4_TK * RB;                  // bytes of a tile's K (or V)
   constexpr int TILE = 2 * KT + 256;              // K, V, 64 pairs
+  constexpr int PAIRS = 512;                      // the pairs of one tile in fp32
   // tiles in flight per wave: 35 KiB of LDS per workgroup with one row tile, 70 with two
   constexpr int ST = RT == 1 ? (D == 64 ? 4 : 2) : (D == 64 ? 7 : 4);
-  constexpr int RING = ST * TILE;
+  constexpr int RING = ST * TILE + PAIRS;
   constexpr int DC = KT / 1024;                   // DMA instructions of a tile's K
   constexpr int DPT = 2 * DC + 1;
   constexpr int LPK = RB / 16;                    // lanes (16 bytes) per key of a DMA instruction
@@ -379,6 +385,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   const char* vbase = (const char*)p.v + (long long)hk * p.v_h;
   // this lane's share of a DMA instruction: key dkey (of KPI), 16-byte piece dpos
   const int dkey = lane / LPK, dpos = lane % LPK;
+  const uint32_t koff = (dkey & 15) * (uint32_t)p.k_r + dpos * 16, voff = (dkey & 15) * (uint32_t)p.v_r + dpos * 16;
   // and of the pairs: word lane = ((kind * 2 + half) * 4 + g) * 4 + e holds key g + 4 e of the half
   const int skey = ((lane >> 2) & 3) + 4 * (lane & 3), shalf = (lane >> 4) & 1;
   const char* sbase = lane < 32 ? (const char*)p.ks + 2 * ((long long)hk * p.ks_h + (long long)skey * p.ks_r)
@@ -415,17 +422,16 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
       vsrc[t] = vbase + (long long)pg[t] * p.v_p + (long long)pr[t] * p.v_r;
     }
 #pragma unroll
-    for (int u = 0; u < DC; ++u) {
-      const int k = u * KPI + dkey;  // key of the tile
-      const bool second = KPI <= 16 ? u * KPI >= 16 : k >= 16;
-      dma_lane16((second ? ksrc[1] : ksrc[0]) + (k & 15) * (int)p.k_r + dpos * 16, dst + u * 1024);
-    }
+    for (int kind = 0; kind < 2; ++kind)
 #pragma unroll
-    for (int u = 0; u < DC; ++u) {
-      const int k = u * KPI + dkey;
-      const bool second = KPI <= 16 ? u * KPI >= 16 : k >= 16;
-      dma_lane16((second ? vsrc[1] : vsrc[0]) + (k & 15) * (int)p.v_r + dpos * 16, dst + KT + u * 1024);
-    }
+      for (int u = 0; u < DC; ++u) {
+        const char* const* src = kind ? vsrc : ksrc;
+        const uint32_t to = dst + (kind ? KT : 0) + u * 1024, off = kind ? voff : koff;
+        if constexpr (KPI <= 16)
+          dma_base16(src[u * KPI / 16], off + u * KPI % 16 * (uint32_t)(kind ? p.v_r : p.k_r), to);
+        else
+          dma_lane16((dkey < 16 ? src[0] : src[1]) + off, to);
+      }
     const uint32_t pl = shalf ? pg[1] : pg[0], rl = shalf ? pr[1] : pr[0];
     dma_lane4(sbase + (uint64_t)pl * s_p + (uint64_t)rl * s_r, dst + 2 * KT);
   };
@@ -440,7 +446,8 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[rt][b] = (f32x4){};
   }
-  const float c2 = p.scale_log2;
+  const float unit = lane < 32 ? p.scale_log2 : 1.0f;
+  const char* const pairs = ring + ST * TILE + 32 * g4;
   const Int4Codes two(KBIAS);
   const int kperm = (l16 >> 2) + 4 * (l16 & 3);  // K row of S^T's row l16
   const uint32_t m136 = 0xC308C308u;             // -136 in bfloat16, twice
@@ -452,6 +459,13 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const char* st = ring + (i % ST) * TILE;
     const int kv0 = lo + I4_TK * (wave + I4_WAVES * i);
+    // every lane decodes one of the 64 pairs (K's in log2 units) for all of them: read
+    // back once K is unpacked
+    {
+      float sc, of;
+      int4_pair<F16>(*(const uint32_t*)(st + 2 * KT + 4 * lane), sc, of);
+      *(f32x2*)(ring + ST * TILE + 8 * lane) = (f32x2){sc * unit, of * unit};
+    }
     f32x4 s[2][RT];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -483,14 +497,12 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt] = int4_mfma<F16>(kf, qf[rt][ks], acc[rt]);
       }
-      const u32x4 kp = *(const u32x4*)(st + 2 * KT + t * 64 + g4 * 16);
+      const f32x4 kp[2] = {*(const f32x4*)(pairs + t * 128), *(const f32x4*)(pairs + t * 128 + 16)};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float sc, of;
-        int4_pair<F16>(kp[e], sc, of);
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[t][rt][e] = fmaf(sc, acc[rt][e], of * qsum[rt]);
-      }
+        for (int rt = 0; rt < RT; ++rt)
+          s[t][rt][e] = fmaf(kp[e / 2][2 * (e & 1)], acc[rt][e], kp[e / 2][2 * (e & 1) + 1] * qsum[rt]);
     }
     const uint32_t alive = (uint32_t)(live[(i >> 5) & 1] >> (2 * (i & 31))) & 3;
     const bool mask = alive != 3 || kv0 < all_from || kv0 + I4_TK - 1 > all_to || kv0 + I4_TK > hi;
@@ -509,14 +521,17 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     float vs[2][4], vo[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const u32x4 vp = *(const u32x4*)(st + 2 * KT + 128 + t * 64 + g4 * 16);
+      const f32x4 vp[2] = {*(const f32x4*)(pairs + 256 + t * 128), *(const f32x4*)(pairs + 256 + t * 128 + 16)};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) int4_pair<F16>(vp[e], vs[t][e], vo[t][e]);
+      for (int e = 0; e < 4; ++e) {
+        vs[t][e] = vp[e / 2][2 * (e & 1)];
+        vo[t][e] = vp[e / 2][2 * (e & 1) + 1];
+      }
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float mh = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
-                             fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3]))) * c2;
+                             fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
       if (__any(mh > ms[rt] + 8.0f)) {
         const float mt = int4_row<OpMax>(mh);
         const bool move = mt > ms[rt] + 8.0f;
@@ -536,7 +551,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
         float pe[4], zp[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pe[e] = __builtin_amdgcn_exp2f(fmaf(s[t][rt][e], c2, -mb));
+          pe[e] = __builtin_amdgcn_exp2f(s[t][rt][e] - mb);
           ps[t][e] = pe[e] * vs[t][e];
           zp[e] = vo[t][e];
         }
