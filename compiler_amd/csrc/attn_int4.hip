@@ -117,7 +117,7 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
 // d 64, 128 or 256, pages of whole 16-key runs, 16-byte rows.  A workgroup owns
 // one (sequence, KV head, block of 16 RT query rows, key range); a query row is
 // (query, head of the group), so K and V are read once for the whole group.  Its
-// 4 waves take 32-key tiles in turn and share nothing until the end: each fills
+// 4 (or 16) waves take 32-key tiles in turn and share nothing until the end: each fills
 // its own LDS ring by direct global->LDS DMA and waits for its own loads only.
 //
 // What bounds it is the vector ALU beside the bytes: a tile of 32 keys is
@@ -139,7 +139,6 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
 //     four rows of a read lie in different LDS banks.
 //   * K's dims are taken in the order in which the words hold them; q's fragments
 //     are laid out to match, once.
-constexpr int I4_WAVES = 4;
 constexpr int I4_TK = 32;  // keys per tile of one wave
 
 __device__ __forceinline__ void dma_lane16(const char* src, uint32_t lds_dst) {
@@ -269,20 +268,20 @@ __device__ __forceinline__ Int4Part int4_deal(const AttnInt4Args& p, Int4Span& s
 // The four waves' partial rows of a workgroup joined: row r's O unnormalised in wave w's
 // LDS (16-byte chunks XOR-swizzled by the row), its maximum (log2 units) and sum in
 // ml[w][r].  Writes o and lse, or record rec0.
-template <int D, bool F16, int ROWS, int WLDS>
+template <int D, bool F16, int ROWS, int WLDS, int NW>
 __device__ __forceinline__ void int4_finish(const AttnInt4Args& p, const char* lds, const float* ml, const Int4Seq& sq,
                                             int hk, int rec0, int row0, int nrows) {
   const int G = p.group;
   constexpr int CPR = D / 4;  // 16-byte chunks (4 d) per row
-  for (int it = threadIdx.x; it < nrows * CPR; it += I4_WAVES * 64) {
+  for (int it = threadIdx.x; it < nrows * CPR; it += NW * 64) {
     const int r = it / CPR, c = it % CPR;
     float m = ml[2 * r];
 #pragma unroll
-    for (int w = 1; w < I4_WAVES; ++w) m = fmaxf(m, ml[2 * (w * ROWS + r)]);
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, ml[2 * (w * ROWS + r)]);
     f32x4 sum = {};
     float lt = 0.0f;
 #pragma unroll
-    for (int w = 0; w < I4_WAVES; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float mw = ml[2 * (w * ROWS + r)], lw = ml[2 * (w * ROWS + r) + 1];
       // no finite score: no key of this row (l = 0), or only NaN ones
       const float f = mw == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
@@ -316,7 +315,7 @@ __device__ __forceinline__ void int4_finish(const AttnInt4Args& p, const char* l
   }
 }
 
-template <int D, bool F16, int RT>
+template <int D, bool F16, int RT, int NW>
 __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr int RB = D / 2;                       // bytes of a row
   constexpr int KT = I4_TK * RB;                  // bytes of a tile's K (or V)
@@ -337,9 +336,9 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr uint32_t KBIAS = F16 ? 0x64006400u : 0x43004300u;
   constexpr float KOFF = F16 ? 1032.0f : 136.0f;
   constexpr int WLDS = RING > ROWS * D * 4 ? RING : ROWS * D * 4;  // a wave's LDS: its ring, then its partial O
-  __shared__ __attribute__((aligned(1024))) char lds[I4_WAVES * WLDS];
-  __shared__ float ml[I4_WAVES][ROWS][2];
-  if (blockDim.x != I4_WAVES * 64) return;  // launch shape must match the kernel
+  __shared__ __attribute__((aligned(1024))) char lds[NW * WLDS];
+  __shared__ float ml[NW][ROWS][2];
+  if (blockDim.x != NW * 64) return;  // launch shape must match the kernel
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, l16 = lane & 15;
@@ -393,7 +392,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   const uint32_t s_p = 2 * (uint32_t)(lane < 32 ? p.ks_p : p.vs_p), s_r = 2 * (uint32_t)(lane < 32 ? p.ks_r : p.vs_r);
   const int* table = p.table + (long long)w.z * p.table_s;
   const int ntiles = hi > lo ? (hi - lo + I4_TK - 1) / I4_TK : 0;
-  const int nloc = ntiles > wave ? (ntiles - wave + I4_WAVES - 1) / I4_WAVES : 0;
+  const int nloc = ntiles > wave ? (ntiles - wave + NW - 1) / NW : 0;
 
   // pages and rows of this wave's next 32 tiles, one 16-key half per lane; a half
   // without a page (or past the end) reads page 0 and is masked
@@ -401,7 +400,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   uint64_t live[2] = {0, 0};  // by the parity of the batch of 32 tiles
   auto issue = [&](int j) {
     if ((j & 31) == 0) {
-      const int key = lo + I4_TK * (wave + I4_WAVES * (j + (lane >> 1))) + 16 * (lane & 1);
+      const int key = lo + I4_TK * (wave + NW * (j + (lane >> 1))) + 16 * (lane & 1);
       const int e = key / p.block_size;
       int ph = key < hi && e < p.max_pages ? table[e] : -1;
       ph = ph < p.pages ? ph : -1;
@@ -458,7 +457,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     if (i + ST <= nloc) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * DPT) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const char* st = ring + (i % ST) * TILE;
-    const int kv0 = lo + I4_TK * (wave + I4_WAVES * i);
+    const int kv0 = lo + I4_TK * (wave + NW * i);
     // every lane decodes one of the 64 pairs (K's in log2 units) for all of them: read
     // back once K is unpacked
     {
@@ -629,7 +628,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     }
   }
   __syncthreads();
-  int4_finish<D, F16, ROWS, WLDS>(p, lds, &ml[0][0][0], sq, hk, w.rec, row0, nrows);
+  int4_finish<D, F16, ROWS, WLDS, NW>(p, lds, &ml[0][0][0], sq, hk, w.rec, row0, nrows);
 }
 
 // Joins the parts of a block of query rows: one wave per row, lane s holds part s's
@@ -692,7 +691,7 @@ extern "C" __global__ __launch_bounds__(64) void g950_attn_int4_general(const g9
 // Four workgroups per CU with one row tile (128 registers), else two.
 #define G950_INT4(NAME, D, F16, RT)                                                                    \
   extern "C" __global__ __launch_bounds__(256, RT == 1 && D < 256 ? 4 : 2) void NAME##_r##RT(const g950::AttnInt4Args p) {      \
-    g950::attn_int4_body<D, F16, RT>(p);                                                               \
+    g950::attn_int4_body<D, F16, RT, 4>(p);                                                               \
   }                                                                                                    \
   extern "C" __global__ __launch_bounds__(256) void NAME##_r##RT##_merge(const g950::AttnInt4Args p) { \
     g950::attn_int4_merge_body<D, F16, 16 * RT>(p);                                                    \
@@ -707,3 +706,13 @@ G950_INT4(g950_attn_int4_f16_d64, 64, true, 2)
 G950_INT4(g950_attn_int4_f16_d128, 128, true, 1)
 G950_INT4(g950_attn_int4_f16_d128, 128, true, 2)
 G950_INT4(g950_attn_int4_f16_d256, 256, true, 1)
+// 16 waves to a block (one workgroup per CU): where there are one to two blocks of many
+// keys per CU, and parts would only be joined again.
+#define G950_INT4W(NAME, D, F16)                                                                   \
+  extern "C" __global__ __launch_bounds__(1024) void NAME##_r1w(const g950::AttnInt4Args p) {     \
+    g950::attn_int4_body<D, F16, 1, 16>(p);                                                        \
+  }
+G950_INT4W(g950_attn_int4_bf16_d64, 64, false)
+G950_INT4W(g950_attn_int4_bf16_d128, 128, false)
+G950_INT4W(g950_attn_int4_f16_d64, 64, true)
+G950_INT4W(g950_attn_int4_f16_d128, 128, true)

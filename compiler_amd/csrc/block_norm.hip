@@ -120,6 +120,9 @@ __device__ __forceinline__ void block_norm_body(const BlockNormArgs& a) {
   __shared__ float scratch[BLOCK / 64 > 0 ? BLOCK / 64 : 1];
   const int tid = threadIdx.x, cols = a.cols;
   const int nv = (cols + V - 1) / V;
+  // the weights and gates come in while the row does; long rows have no
+  // registers for them until the row is summed
+  constexpr bool EARLY = ITEMS <= 2;
   const long long r = blockIdx.x;
   const char* xr = (const char*)a.x + r * a.x_row * (long long)sizeof(T);
   const char* hr = (const char*)a.h + r * a.h_row * (long long)sizeof(T);
@@ -134,12 +137,9 @@ __device__ __forceinline__ void block_norm_body(const BlockNormArgs& a) {
     if (j < nv) {
       h[i] = M::load(hr, j, cols, true);
       x[i] = M::load(xr, j, cols, true);
-      if constexpr (GATE == 1) g[i] = M::load(gr, j, cols, false);
+      if constexpr (GATE == 1 && EARLY) g[i] = M::load(gr, j, cols, false);
     }
   }
-  // the weights come from L2 while the row comes from memory; long rows
-  // have no registers for them until the row is summed
-  constexpr bool EARLY = ITEMS <= 2;
   auto weights = [&](const void* w, u32x4(&to)[ITEMS]) {
     if (w) {
 #pragma unroll
@@ -165,7 +165,14 @@ __device__ __forceinline__ void block_norm_body(const BlockNormArgs& a) {
       }
     rh = 1.0f / sqrtf(block_reduce<OpSum, BLOCK>(s, scratch) / (float)cols + a.eps);
   }
-  if constexpr (!EARLY) weights(a.w_post, wo);
+  if constexpr (!EARLY) {
+    weights(a.w_post, wo);
+    if constexpr (GATE == 1) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        if (tid + i * BLOCK < nv) g[i] = M::load(gr, tid + i * BLOCK, cols, false);
+    }
+  }
   float y[ITEMS][V];
   float s = 0.0f;
 #pragma unroll
@@ -213,8 +220,8 @@ extern "C" __global__ __launch_bounds__(256) void g950_block_norm_general(const 
   G950_BN(TNAME, T, 2, 64)     \
   G950_BN(TNAME, T, 1, 256)    \
   G950_BN(TNAME, T, 2, 256)    \
-  G950_BN(TNAME, T, 4, 256)    \
-  G950_BN(TNAME, T, 8, 256)    \
+  G950_BN(TNAME, T, 2, 512)    \
+  G950_BN(TNAME, T, 2, 1024)   \
   G950_BN(TNAME, T, 4, 1024)
 G950_BN_SET(f32, float)
 G950_BN_SET(bf16, g950::bf16_t)

@@ -1863,6 +1863,7 @@ struct Int4Shape {
   long long row_blocks;  // per (sequence, KV head)
   long long blocks;      // of the call
   long long splits;      // parts wanted
+  bool wide;             // 16 waves to a workgroup
 };
 constexpr long long kInt4Target = 4, kInt4MinKeys = 256, kInt4OneRange = 1024;
 
@@ -1874,7 +1875,8 @@ Int4Shape int4_shape(const g950_module* m, long long b, long long h, long long h
   f.row_blocks = (rows + f.rows - 1) / f.rows;
   f.blocks = b * hk * f.row_blocks;
   f.splits = 1;
-  if (f.blocks && seqlen_k > kInt4OneRange)
+  f.wide = f.rows == 16 && d <= 128 && seqlen_k > kInt4OneRange && f.blocks >= cus && f.blocks <= 2 * cus;
+  if (f.blocks && seqlen_k > kInt4OneRange && !f.wide)
     f.splits = std::max(1ll, std::min({kInt4Target * cus / f.blocks, (seqlen_k + kInt4MinKeys - 1) / kInt4MinKeys,
                                        64ll}));  // the merge holds a row's parts in one wave's lanes
   return f;
@@ -1974,6 +1976,7 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
     char name[64];
     const int n = snprintf(name, sizeof name, "g950_attn_int4_%s_d%lld_r%lld", dt == G950_DTYPE_BFLOAT16 ? "bf16" : "f16", D,
                            f.rows / 16);
+    if (f.wide) return launch(m, std::string(name) + "w", (unsigned)grid, 1024u, a, stream);
     if (int rc = launch(m, name, (unsigned)grid, 256u, a, stream)) return rc;
     if (a.splits == 1) return G950_OK;
     snprintf(name + n, sizeof name - n, "_merge");
@@ -2040,7 +2043,7 @@ int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const
   a.alpha = (float)alpha; a.eps = (float)eps;
   // the smallest form that holds a row; a gate that is neither contiguous along
   // the row nor one per row, and longer rows, take the general kernel
-  static const struct { int items, block; } kForms[] = {{1, 64}, {2, 64}, {1, 256}, {2, 256}, {4, 256}, {8, 256}, {4, 1024}};
+  static const struct { int items, block; } kForms[] = {{1, 64}, {2, 64}, {1, 256}, {2, 256}, {2, 512}, {2, 1024}, {4, 1024}};
   const long long nv = (cols * x.isz + 15) / 16;
   const int gk = !gate ? 0 : a.g_col == 1 || cols == 1 ? 1 : a.g_col == 0 ? 2 : -1;
   for (const auto& f : kForms) {

@@ -210,14 +210,14 @@ __device__ __forceinline__ void kv_append_general_body(const KvAppendArgs& a) {
 template <typename T>
 __device__ __forceinline__ void kv_load8(const char* p, float* v) {
   if constexpr (sizeof(T) == 4) {
-    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 16);
+    const f32x4 a = __builtin_nontemporal_load((const f32x4*)p), b = __builtin_nontemporal_load((const f32x4*)(p + 16));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = a[e];
       v[4 + e] = b[e];
     }
   } else {
-    const u32x4 w = *(const u32x4*)p;
+    const u32x4 w = __builtin_nontemporal_load((const u32x4*)p);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint16_t b = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
@@ -225,7 +225,8 @@ __device__ __forceinline__ void kv_load8(const char* p, float* v) {
     }
   }
 }
-template <typename T>
+// ONCE: past the caches (a prompt's rows are far more than they hold)
+template <typename T, bool ONCE>
 __device__ __forceinline__ void kv_store8(char* p, const float* v) {
   if constexpr (sizeof(T) == 4) {
     *(f32x4*)p = (f32x4){v[0], v[1], v[2], v[3]};
@@ -239,7 +240,8 @@ __device__ __forceinline__ void kv_store8(char* p, const float* v) {
       else
         w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){v[2 * e], v[2 * e + 1]}, f16x2));
     }
-    *(u32x4*)p = w;
+    if constexpr (ONCE) __builtin_nontemporal_store(w, (u32x4*)p);
+    else *(u32x4*)p = w;
   }
 }
 
@@ -326,8 +328,8 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
       char* p = is_q ? (char*)a.q_out + (t * a.qo_st + h * a.qo_sh) * SZ
                      : is_v ? (char*)a.v_cache + (at.page * a.vc_p + at.row * a.vc_r + h * a.vc_h) * SZ
                             : (char*)a.k_cache + (at.page * a.kc_p + at.row * a.kc_r + h * a.kc_h) * SZ;
-      kv_store8<T>(p + u * 8 * SZ, x[0]);
-      kv_store8<T>(p + (D / 2 + u * 8) * SZ, x[1]);
+      kv_store8<T, !INT4>(p + u * 8 * SZ, x[0]);
+      kv_store8<T, !INT4>(p + (D / 2 + u * 8) * SZ, x[1]);
     }
     if constexpr (INT4) {
       if (g * RPW + RPW > a.Hq) {  // (uniform) some lane holds a key or value
@@ -361,7 +363,7 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
             for (int v = 0; v < 2; ++v) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) x[v][e] = kv_value(code[v][e], k);
-              kv_store8<T>(out + (v * D / 2 + u * 8) * SZ, x[v]);
+              kv_store8<T, false>(out + (v * D / 2 + u * 8) * SZ, x[v]);
             }
           }
           if (at.page >= 0) {

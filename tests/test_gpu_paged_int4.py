@@ -284,6 +284,8 @@ ATTEND = {
     "page48": dict(ql=[1, 2], kl=[400, 100], h=4, hk=4, d=128, page=48),
     "page1": dict(ql=[1, 2], kl=[70, 9], h=4, hk=2, d=64, page=1),
     "page10": dict(ql=[1, 2], kl=[170, 9], h=4, hk=2, d=128, page=10),
+    "wide": dict(ql=[1] * 32, kl=[1 + 37 * i for i in range(32)], h=16, hk=8, d=128, page=16),
+    "wide_d64": dict(ql=[1, 0, 1, 2] * 8, kl=[1100 - 31 * i for i in range(32)], h=8, hk=8, d=64, page=64),
     "odd_d": dict(ql=[2, 1], kl=[70, 300], h=4, hk=2, d=80, page=16),
     "d2": dict(ql=[2], kl=[70], h=2, hk=1, d=2, page=16),
 }
@@ -355,11 +357,17 @@ def check_attend(c, dt, o, lse):
     assert (err <= score + 2.0 ** -20 * (1 + np.abs(wl[f]))).all(), float(err.max())
 
 
+# the form that a case takes where it has one of its own to show
+FORMS = {"one_key": "_r1", "ranges": "_r1_merge", "rows32": "_r2", "d256": "_r1", "wide": "_r1w", "wide_d64": "_r1w",
+         "chunk": "_r2", "page1": "_general", "page10": "_general", "odd_d": "_general", "d2": "_general"}
+
+
 @pytest.mark.parametrize("dt", ["bfloat16", "float16"])
 @pytest.mark.parametrize("case", sorted(ATTEND))
 def test_attend(case, dt):
     c = attend_case(case, dt)
     check_attend(c, dt, *attend_run(c, dt))
+    assert rt.module().last_kernel.endswith(FORMS.get(case, ""))
 
 
 def test_attend_scores_climb():
