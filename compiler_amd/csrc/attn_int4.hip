@@ -125,12 +125,13 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
 // is therefore ever dequantised: the matrix cores multiply the codes, and scale and
 // offset enter where a tile has few numbers.
 //   * A word holds 8 codes; (w >> 4 i) & 0x000F000F | bias makes two of them
-//     numbers at once, 128 + c in bfloat16 or 1024 + c in float16 (the code lands in
-//     the low mantissa bits): 7 operations for 8 codes.
+//     numbers at once, 128 + c in bfloat16 or 64 + c in float16 (the code lands in the
+//     mantissa): 7 operations for 8 codes.
 //   * S = s (sum q c) + o sum q, c in -8 .. 7: the bias leaves through the MFMA's
 //     addend, -(bias + 8) sum q.  Exact products, fp32 sums.
 //   * O = sum (p s) c + sum p o: the probability carries V's scale, rounded to
-//     bfloat16 once (its range, as s may be any size); the bias leaves through one
+//     bfloat16 once, or to two bfloat16 terms in float16 models (its range, as s may be
+//     any size); the bias leaves through one
 //     more MFMA with a constant -136 in place of V, over the same rounded values, so
 //     that nothing of it is left.  p o and the softmax sum stay in fp32.
 //   * V^T needs keys along the contraction: a lane reads the same word of its four
@@ -176,18 +177,25 @@ __device__ __forceinline__ void int4_pair(uint32_t w, float& s, float& o) {
   }
 }
 
-// Two codes of a word as numbers, (w & 0x000F000F) | bias, in one operation: with
-// both constants as literals the compiler takes two, so they are kept in
-// registers that it cannot see through.  (Not the instruction itself in inline asm:
-// the wait states that an MFMA needs behind the writer of its operand are not
-// inserted behind asm.)
+// Two codes of a word as numbers, (shifted word & mask) | bias, in one operation beside
+// the shift: with both constants as literals the compiler takes two, so they are
+// kept in registers that it cannot see through.  (Not the instruction itself in inline
+// asm: the wait states that an MFMA needs behind the writer of its operand are not
+// inserted behind asm.)  bfloat16: the code in mantissa bits 0 .. 3 of 128; float16: bits
+// 4 .. 7 of 64 (bits 0 .. 3 of 1024 would cost the scores three more bits).
+template <bool F16>
 struct Int4Codes {
-  uint32_t mask = 0x000F000Fu, kbias, vbias = 0x43004300u;
-  __device__ __forceinline__ explicit Int4Codes(uint32_t kb) : kbias(kb) {
-    asm("" : "+s"(mask), "+v"(kbias), "+v"(vbias));
+  static constexpr float KOFF = F16 ? 72.0f : 136.0f;  // bias + 8 of K's codes
+  uint32_t kmask = F16 ? 0x00F000F0u : 0x000F000Fu, kbias = F16 ? 0x54005400u : 0x43004300u;
+  uint32_t vmask = 0x000F000Fu, vbias = 0x43004300u;
+  __device__ __forceinline__ Int4Codes() { asm("" : "+s"(kmask), "+v"(kbias), "+s"(vmask), "+v"(vbias)); }
+  // codes r and r + 4
+  __device__ __forceinline__ uint32_t k(uint32_t w, int r) const {
+    if constexpr (F16) w = r == 0 ? w << 4 : w >> (4 * (r - 1));
+    else w >>= 4 * r;
+    return (w & kmask) | kbias;
   }
-  __device__ __forceinline__ uint32_t k(uint32_t w) const { return (w & mask) | kbias; }
-  __device__ __forceinline__ uint32_t v(uint32_t w) const { return (w & mask) | vbias; }
+  __device__ __forceinline__ uint32_t v(uint32_t w, int r) const { return ((w >> (4 * r)) & vmask) | vbias; }
 };
 
 // 8 dims of a query row as pairs (r, r + 4), the order in which a word's codes are
@@ -333,8 +341,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr int VN = D == 64 ? 4 : 8;             // codes of each
   constexpr int NB = VW * VN;                     // 16-d blocks of O^T
   constexpr int ROWS = 16 * RT;
-  constexpr uint32_t KBIAS = F16 ? 0x64006400u : 0x43004300u;
-  constexpr float KOFF = F16 ? 1032.0f : 136.0f;
+  constexpr int PT = F16 ? 2 : 1;                 // bfloat16 terms of a probability
   constexpr int WLDS = RING > ROWS * D * 4 ? RING : ROWS * D * 4;  // a wave's LDS: its ring, then its partial O
   __shared__ __attribute__((aligned(1024))) char lds[NW * WLDS];
   __shared__ float ml[NW][ROWS][2];
@@ -447,7 +454,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   }
   const float unit = lane < 32 ? p.scale_log2 : 1.0f;
   const char* const pairs = ring + ST * TILE + 32 * g4;
-  const Int4Codes two(KBIAS);
+  const Int4Codes<F16> two;
   const int kperm = (l16 >> 2) + 4 * (l16 & 3);  // K row of S^T's row l16
   const uint32_t m136 = 0xC308C308u;             // -136 in bfloat16, twice
   const u32x4 unbias = {m136, m136, m136, m136};
@@ -485,14 +492,14 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
       f32x4 acc[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float q = -KOFF * qsum[rt];
+        const float q = -Int4Codes<F16>::KOFF * qsum[rt];
         acc[rt] = (f32x4){q, q, q, q};
       }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         u32x4 kf;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) kf[r] = two.k(kw[ks] >> (4 * r));
+        for (int r = 0; r < 4; ++r) kf[r] = two.k(kw[ks], r);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt] = int4_mfma<F16>(kf, qf[rt][ks], acc[rt]);
       }
@@ -516,7 +523,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
             if (!((alive >> t) & 1) || key < kmin[rt] || key > kmax[rt] || key >= hi) s[t][rt][e] = -__builtin_huge_valf();
           }
     }
-    u32x4 pf[RT];
+    u32x4 pf[RT][PT];
     float vs[2][4], vo[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -566,11 +573,22 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
         for (int e = 0; e < 4; ++e) zo[rt] = fmaf(pe[e], zp[e], zo[rt]);
         l[rt] += (pe[0] + pe[1]) + (pe[2] + pe[3]);
       }
-      auto pack = [](float a, float b) {
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
-      };
-      pf[rt] = (u32x4){pack(ps[0][0], ps[0][1]), pack(ps[0][2], ps[0][3]), pack(ps[1][0], ps[1][1]), pack(ps[1][2], ps[1][3])};
-      ob[rt] = int4_mfma<false>(unbias, pf[rt], ob[rt]);
+      // bfloat16 models: one rounding; float16 models: what the rounding left out as a
+      // second term (their outputs hold more bits than one term gives them)
+#pragma unroll
+      for (int n = 0; n < PT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float* two_p = &ps[j / 2][2 * (j & 1)];
+          const uint32_t pk = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){two_p[0], two_p[1]}, bf16x2));
+          pf[rt][n][j] = pk;
+          if (n + 1 < PT) {
+            two_p[0] -= __uint_as_float(pk << 16);
+            two_p[1] -= __uint_as_float(pk & 0xFFFF0000u);
+          }
+        }
+        ob[rt] = int4_mfma<false>(unbias, pf[rt][n], ob[rt]);
+      }
     }
     // V: words of keys g4 + 4 e of both halves, two keys side by side
     const char* vr = st + KT + g4 * RB + l16 * (D == 64 ? 2 : 4);
@@ -594,9 +612,11 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
       for (int n = 0; n < VN; ++n) {
         u32x4 vf;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) vf[r] = two.v(half[n / 4][r] >> (4 * (n & 3)));
+        for (int r = 0; r < 4; ++r) vf[r] = two.v(half[n / 4][r], n & 3);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][c * VN + n] = int4_mfma<false>(vf, pf[rt], o[rt][c * VN + n]);
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int m = 0; m < PT; ++m) o[rt][c * VN + n] = int4_mfma<false>(vf, pf[rt][m], o[rt][c * VN + n]);
       }
     }
     // this tile's LDS reads have returned before its slot is refilled
