@@ -455,6 +455,7 @@ def paged_attention_int4(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_s
     unless given."""
     import torch
     t, h, d = q.shape
+    seqlen_q, seqlen_k = int(seqlen_q), int(seqlen_k)
     o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
     lse = torch.empty((h, t), dtype=torch.float32, device=q.device) if lse is None else lse
     if workspace is None:

@@ -98,6 +98,24 @@ def test_block_norm_in_place_and_strided(cols):
     assert (wide[2][:, :3] == 7).all() and (wide[2][:, cols + 3:] == 7).all() and (wide[3][:, cols:] == 7).all()
 
 
+def test_block_norm_gate_of_other_strides():
+    """A gate that is neither contiguous along the row nor one per row."""
+    i = inputs(5, 3000, "bfloat16", "full")
+    t = {k: dev(v, "bfloat16") for k, v in i.items()}
+    y, n = ops.block_norm(t["x"], t["h"], t["w_pre"], 1e-6, w_post=t["w_post"], gate=t["gate"].t().contiguous().t(),
+                          gate_act="tanh", sync=True)
+    assert rt.module().last_kernel == "g950_block_norm_general"
+    check(i, "bfloat16", y, n, act="tanh")
+
+
+def test_block_norm_forms():
+    for cols, form in ((100, "i1_b64"), (900, "i2_b64"), (2000, "i1_b256"), (4096, "i2_b256"), (8192, "i2_b512"),
+                       (16000, "i2_b1024"), (30000, "i4_b1024")):
+        i = inputs(2, cols, "float16", "full")
+        check(i, "float16", *run(i, "float16", gate_act="sigmoid"), act="sigmoid")
+        assert rt.module().last_kernel == f"g950_block_norm_f16_{form}_g1"
+
+
 def test_block_norm_rows_keep_to_themselves():
     """A row of NaN, of infinities, of zeros: the others are as without it."""
     i = inputs(6, 3000, "bfloat16")

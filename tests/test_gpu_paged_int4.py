@@ -532,6 +532,152 @@ def test_append_then_attend_steps():
             at += n[i]
 
 
+def test_attend_parts_in_captured_graphs():
+    """Calls of several parts captured into two graphs (each with its own workspace,
+    from torch's allocator): replayed in turn, between eager calls of other
+    sizes, each gives its eager bits again."""
+    cases = [attend_case("ranges", "bfloat16"), attend_case("rows32", "bfloat16", seed=3)]
+    cases[1]["seqlen_k"] = 2000  # several parts
+    args = [attend_args(c, "bfloat16") for c in cases]
+    call = lambda i: ops.paged_attention_int4(*args[i], scale=cases[i]["scale"])  # noqa: E731
+    want = []
+    for i, c in enumerate(cases):
+        want.append([x.clone() for x in call(i)])
+        assert rt.module().last_kernel.endswith("_merge")
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(i))
+        graphs.append(g)
+    for _ in range(3):
+        for i in (0, 1):
+            for x in outs[i]:
+                x.zero_()
+            torch.cuda.synchronize()
+            graphs[i].replay()
+            ops.paged_attention_int4(*args[1 - i], scale=cases[1 - i]["scale"])
+            torch.cuda.synchronize()
+            n = cases[i]["q"].shape[0] - 3
+            assert torch.equal(outs[i][0][:n], want[i][0][:n]) and torch.equal(outs[i][1][:, :n], want[i][1][:, :n])
+
+
+def test_attend_streams_workspaces_and_prepared_calls():
+    """A Stream, its handle, the per-thread stream (which gets no workspace), a given
+    workspace of any length, a prepared call."""
+    c = attend_case("ranges", "bfloat16")
+    args = attend_args(c, "bfloat16")
+    n = c["q"].shape[0] - 3
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (side, side.cuda_stream, 0, 2):
+        o, lse = ops.paged_attention_int4(*args, scale=c["scale"], stream=stream, sync=True)
+        assert rt.module().last_kernel.endswith("_merge") == (stream != 2)
+        check_attend(c, "bfloat16", torch.cat([o[:n], torch.full_like(o[n:], 9)]),
+                     torch.cat([lse[:, :n], torch.full_like(lse[:, n:], 9)], 1))
+    need = rt.module().attention_int4_workspace(2, 32, 8, 128, 1, 1500)
+    assert need > 0
+    for floats in (0, 7, need // 2, need, need + 99):
+        o, lse = attend_run(c, "bfloat16", args, workspace=torch.empty(floats, device="cuda"))
+        assert rt.module().last_kernel.endswith("_merge") == (floats >= need // 2)
+        check_attend(c, "bfloat16", o, lse)
+    with pytest.raises(rt.G950Error, match="16-byte aligned"):
+        attend_run(c, "bfloat16", args, workspace=torch.empty(need + 1, device="cuda")[1:])
+    o = torch.full(c["q"].shape, 9.0, dtype=torch.bfloat16, device="cuda")
+    lse = torch.full((c["h"], n + 3), 9.0, device="cuda")
+    call = ops.paged_attention_int4_kernel(*args[:8], o, lse, torch.empty(need, device="cuda"), c["seqlen_q"], c["seqlen_k"],
+                                           c["scale"], True, -1, -1, prepare=True)
+    for _ in range(2):
+        call()
+    torch.cuda.synchronize()
+    check_attend(c, "bfloat16", o, lse)
+
+
+@pytest.mark.parametrize("d,dt", [(128, "bfloat16"), (64, "float16"), (80, "bfloat16")])
+def test_caches_past_32_bits(d, dt):
+    """Pages more than 2^31 (and 2^32) elements apart: append and attention by the
+    fast kernels and the general one."""
+    far = 3 << 30
+    rng = np.random.default_rng(3)
+    cu, used = np.array([0, 3, 4], np.int32), np.array([40, 17], np.int32)
+    table = np.array([[1, 0, 2], [3, 4, -1]], np.int32)
+    rows = 16 * 2 * (d // 2)
+    raw = [torch.zeros(4 * far + rows, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    codes = [x.as_strided((5, 16, 2, d // 2), (far, d, d // 2, 1)) for x in raw]
+    scales = [torch.zeros((5, 2, 16, 2), dtype=T[dt], device="cuda").transpose(1, 2) for _ in range(2)]
+    cos, sin = rope(40, d, rng)
+    rnd = ref.rounder(dt)
+    ks, vs = [], []
+    # the whole sequences appended as one prompt, then the last tokens attend
+    x = rnd(rng.standard_normal((57, 8, d)).astype(np.float32))
+    full = dev(np.array([0, 40, 57], np.int32))
+    q, kv, vv = ops.paged_append_int4(dev(x[:, :4], dt), dev(x[:, 4:6], dt), dev(x[:, 6:], dt), dev(cos), dev(sin), codes[0],
+                                      scales[0], codes[1], scales[1], dev(table), full, dev(used), values=True)
+    name = rt.module().last_kernel
+    assert name.endswith("general" if d == 80 else f"d{d}")
+    pick = [37, 38, 39, 56]
+    o, lse = ops.paged_attention_int4(q[pick].contiguous(), codes[0], scales[0], codes[1], scales[1], dev(table), dev(cu),
+                                      dev(used), 3, 40, sync=True)
+    assert rt.module().last_kernel.endswith("general" if d == 80 else "_r1")
+    for lo, hi in ((0, 40), (40, 57)):
+        ks.append(host(kv)[lo:hi].astype(np.float64))
+        vs.append(host(vv)[lo:hi].astype(np.float64))
+    wo, wl, _ = ref.attention(host(q)[pick], ks, vs, used, cu, 1 / math.sqrt(d), -1, 0, 3)
+    # the values that came back are rounded to 16 bits (2^-8 of up to 4.5 in keys and values)
+    assert np.abs(host(o) - wo).max() < 0.06 and np.abs(lse.cpu().numpy() - wl).max() < 0.06
+    # 16 bits
+    kc = torch.zeros(2 * far + 16 * 2 * d, dtype=T[dt], device="cuda").as_strided((3, 16, 2, d), (far, 2 * d, d, 1))
+    vc = torch.zeros((3, 16, 2, d), dtype=T[dt], device="cuda")
+    ops.paged_append(None, dev(x[:40, 4:6], dt), dev(x[:40, 6:], dt), dev(cos), dev(sin), kc, vc, dev(table[:1] % 3),
+                     dev(np.array([0, 40], np.int32)), dev(used[:1]), sync=True)
+    c1, s1 = cos[:40], sin[:40]
+    want = ref.rotate(x[:40, 4:6], c1, s1, False)
+    got = np.concatenate([host(kc[int(p) % 3]) for p in table[0]])[:40]
+    close(got, want, dt, rotation_error(x[:40, 4:6]))
+
+
+def test_no_sequences():
+    """b = 0: nothing is read or written, whatever the other extents."""
+    e = torch.empty((0, 3), dtype=torch.int32, device="cuda")
+    cu, used = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda")
+    for tokens in (0, 2):
+        q = torch.randn(tokens, 4, 128, device="cuda").bfloat16()
+        kc, ks = ops.int4_cache(2, 16, 2, 128, torch.bfloat16)
+        out = torch.full_like(q, 9.0)
+        cos = torch.ones(4, 64, device="cuda")
+        ops.paged_append_int4(q, q[:, :2], q[:, 2:], cos, cos, kc, ks, kc.clone(), ks.clone(), e, cu, used, out=out)
+        o, lse = ops.paged_attention_int4(q, kc, ks, kc, ks, e, cu, used, 1, 16, out=out, sync=True)
+        assert (out == 9.0).all() and (kc == 0).all() and o is out
+
+
+def test_other_calls_are_refused():
+    c = append_case("step", "bfloat16")
+    q = dev(c["q"], "bfloat16")
+    with pytest.raises(rt.G950Error, match="current device"):
+        ops.paged_append(q.cpu(), q[:, :2], q[:, :2], dev(c["cos"]), dev(c["sin"]), q, q, dev(c["table"]), dev(c["cu"]),
+                         dev(c["used"]))
+    with pytest.raises(rt.G950Error, match="be the input"):
+        kc, ks = ops.int4_cache(c["pool"], 64, 2, 128, torch.bfloat16)
+        k = q[:, :2]
+        ops.paged_append_int4(q, k, k, dev(c["cos"]), dev(c["sin"]), kc, ks, kc.clone(), ks.clone(), dev(c["table"]),
+                              dev(c["cu"]), dev(c["used"]), k_out=k, v_out=torch.empty_like(k))
+
+
+def test_append_int4_one_of_the_values():
+    c = append_case("prompt", "bfloat16")
+    both = append4(c, "bfloat16")
+    qkv = dev(c["x"], "bfloat16")
+    h, hk = c["h"], c["hk"]
+    for name, want in (("k_out", both[1]), ("v_out", both[2])):
+        kc, ks = ops.int4_cache(c["pool"], c["page"], hk, c["d"], torch.bfloat16)
+        out = torch.full(want.shape, 9.0, dtype=torch.bfloat16, device="cuda")
+        _, ko, vo = ops.paged_append_int4(qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:], dev(c["cos"]), dev(c["sin"]), kc, ks,
+                                          kc.clone(), ks.clone(), dev(c["table"]), dev(c["cu"]), dev(c["used"]), sync=True,
+                                          **{name: out})
+        assert (ko is None) == (name == "v_out") and (vo is None) == (name == "k_out")
+        assert torch.equal(out, want)
+
+
 def test_calls_from_two_threads_on_two_streams():
     c = attend_case("ranges", "bfloat16")
     args = attend_args(c, "bfloat16")
