@@ -11,6 +11,7 @@ torch = pytest.importorskip("torch")
 from compiler_amd import operators as ops  # noqa: E402
 from compiler_amd import runtime as rt  # noqa: E402
 from oracle import paged as ref  # noqa: E402
+from own_streams import own_stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -137,7 +138,7 @@ def test_block_norm_captured():
     want = [x.clone() for x in call()]
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.cuda.graph(graph, stream=own_stream()):
         out = call()
     for _ in range(3):
         for x in out:

@@ -21,6 +21,7 @@ torch = pytest.importorskip("torch")
 from compiler_amd import operators as ops  # noqa: E402
 from compiler_amd import runtime as rt  # noqa: E402
 from oracle import paged as ref  # noqa: E402
+from own_streams import own_stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -497,14 +498,14 @@ def test_append_then_attend_steps():
             o, _ = ops.paged_attention_int4(qr, kc, ks, vc, vs, table, cu, used, max(n), int(lens.max()))
             return qr, kv, vv, o
         if step == 2:
-            stream = torch.cuda.Stream()
+            stream = own_stream()
             stream.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(stream):
                 out = call()
             stream.synchronize()
         elif step == 3:
             graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
+            with torch.cuda.graph(graph, stream=own_stream()):
                 out = call()
             first = None
             for _ in range(3):
@@ -547,7 +548,7 @@ def test_attend_parts_in_captured_graphs():
     graphs, outs = [], []
     for i in range(2):
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with torch.cuda.graph(g, stream=own_stream()):
             outs.append(call(i))
         graphs.append(g)
     for _ in range(3):
@@ -568,7 +569,7 @@ def test_attend_streams_workspaces_and_prepared_calls():
     c = attend_case("ranges", "bfloat16")
     args = attend_args(c, "bfloat16")
     n = c["q"].shape[0] - 3
-    side = torch.cuda.Stream()
+    side = own_stream()
     torch.cuda.synchronize()
     for stream in (side, side.cuda_stream, 0, 2):
         o, lse = ops.paged_attention_int4(*args, scale=c["scale"], stream=stream, sync=True)
@@ -684,8 +685,8 @@ def test_calls_from_two_threads_on_two_streams():
     want = [x.clone() for x in attend_run(c, "bfloat16", args)]
     bad = []
 
-    def work():
-        s = torch.cuda.Stream()
+    def work(i):
+        s = own_stream(i)
         with torch.cuda.stream(s):
             for _ in range(20):
                 o, lse = ops.paged_attention_int4(*args, scale=c["scale"])
@@ -693,7 +694,8 @@ def test_calls_from_two_threads_on_two_streams():
                 n = c["q"].shape[0] - 3
                 if not (torch.equal(o[:n], want[0][:n]) and torch.equal(lse[:, :n], want[1][:, :n])):
                     bad.append(1)
-    th = [threading.Thread(target=work) for _ in range(2)]
+    own_stream(0), own_stream(1)
+    th = [threading.Thread(target=work, args=(i,)) for i in range(2)]
     for t in th:
         t.start()
     for t in th:
