@@ -1963,6 +1963,7 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
                     a.q_st % 8 == 0 && a.q_sh % 8 == 0 && o.addr() % 8 == 0 && a.o_st % 4 == 0 && a.o_sh % 4 == 0;
   if (fast && rows) {
     const Int4Shape f = int4_shape(m, a.B, H, HK, D, std::min(SQ, T), SK);
+    if (f.blocks > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
     if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
     // as many parts as the workspace holds records for
     a.row_blocks = (int)f.row_blocks;
@@ -2028,7 +2029,7 @@ int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const
   }
   if (gate && (g.v->dtype != x.v->dtype || g.shape[0] != x.shape[0] || g.shape[1] != cols))
     return fail(G950_USAGE, "block_norm: G must have X's shape (strides may be 0) and dtype");
-  if (!gate && act) return fail(G950_USAGE, "block_norm: gate_act without G");
+  if (!gate && act && x.shape[0]) return fail(G950_USAGE, "block_norm: gate_act without G");
   if (int rc = distinct(y, "block_norm")) return rc;
   BlockNormArgs a{};
   a.x = x.v->data; a.h = h.v->data; a.y = y.v->data;
@@ -2194,6 +2195,8 @@ size_t g950_paged_attention_int4_workspace(g950_module* m, int64_t b, int64_t h,
   if (b <= 0 || hk <= 0 || h < hk || h % hk || d <= 0 || seqlen_q <= 0 || seqlen_k <= 0 || b > most || h > 65536 || d > 256 ||
       seqlen_q > most || seqlen_k > most || (d != 64 && d != 128 && d != 256))
     return 0;
+  // (what has more blocks than a grid is refused by the launch)
+  if ((double)b * (double)h * (double)seqlen_q > 0x1p47) return 0;
   const Int4Shape f = int4_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
   return f.splits > 1 ? (size_t)(f.blocks * f.rows * f.splits * (d + 2)) * 4 : 0;
 }

@@ -207,9 +207,9 @@ typedef struct g950_scalar {
  *                      s = o = NaN.
  *   views   cos_ptr, cu_seqlens_q_ptr, k_cache_ptr u8[pages,block_size,HK,D/2],
  *           k_out_ptr[T,HK,D] or empty (the appended rows as the cache now holds
- *           them, rounded to T), k_ptr, k_scale_ptr[pages,block_size,HK,2],
- *           page_table_ptr, q_out_ptr, q_ptr, seqused_k_ptr, sin_ptr, v_cache_ptr,
- *           v_out_ptr, v_ptr, v_scale_ptr
+ *           them, rounded to T; apart from every input), k_ptr,
+ *           k_scale_ptr[pages,block_size,HK,2], page_table_ptr, q_out_ptr, q_ptr,
+ *           seqused_k_ptr, sin_ptr, v_cache_ptr, v_out_ptr, v_ptr, v_scale_ptr
  *   scalars interleaved
  * G950_OP_PAGED_ATTENTION_INT4  attention over that cache: GQA, query i of a
  *                      sequence with n of them sees keys j with i + seqused_k - n - left <= j

@@ -160,6 +160,20 @@ def test_block_norm_is_taken_and_refused():
     refused(norm(X=dict(strides=[512, 2])), rt.USAGE, "contiguous")
 
 
+def test_block_norm_without_rows_takes_a_gate():
+    for g in (dict(shape=[0, 256]), dict(shape=[0, 256], strides=[0, 1]), dict(shape=[0, 0])):
+        assert norm(rows=0, act=1, G=g)[0] == 0
+
+
+def test_attend_sizes_past_every_grid():
+    big = dict(t=(1 << 27) - 1, h=16, hk=16, b=(1 << 27) - 2, sq=(1 << 27) - 1, sk=5000)
+    refused(attend(**big), rt.USAGE, "grid too large")
+    size = lambda *a: rt.load_library().g950_paged_attention_int4_workspace(None, *a)  # noqa: E731
+    assert size(1 << 31, 65536, 65536, 128, 1 << 31, 1 << 31) == 0
+    assert size(0, 8, 8, 128, 1, 5000) == size(1, 8, 3, 128, 1, 5000) == size(1, 8, 8, 80, 1, 5000) == 0
+    assert size(1, 8, 8, 128, 1, 1000) == 0 < size(1, 8, 8, 128, 1, 5000)
+
+
 # ------------------------------------------------------- the oracle's own pins
 def test_oracle_quantize_bounds_and_special_rows():
     rng = np.random.default_rng(0)
