@@ -24,7 +24,8 @@ __device__ __forceinline__ Int4Seq int4_seq(const AttnInt4Args& p, int z) {
 }
 
 // One wave per (query row, head): any D, page size, stride and alignment.
-// Lanes take keys for the scores, dims for O.
+// Lanes take keys for the scores, dims for O.  A cache row is read once for every
+// query row and head, 64 rows apart: bound by the latency of its loads.
 __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
   __shared__ float qs[256];
   __shared__ float pr[64], vo[64];
@@ -117,13 +118,22 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
 // d 64, 128 or 256, pages of whole 16-key runs, 16-byte rows.  A workgroup owns
 // one (sequence, KV head, block of 16 RT query rows, key range); a query row is
 // (query, head of the group), so K and V are read once for the whole group.  Its
-// 4 (or 16) waves take 32-key tiles in turn and share nothing until the end: each fills
+// 4 or 16 waves take 32-key tiles in turn and share nothing until the end: each fills
 // its own LDS ring by direct global->LDS DMA and waits for its own loads only.
 //
-// What bounds it is the vector ALU beside the bytes: a tile of 32 keys is
-// 64 d values in 64 lanes and leaves HBM in about a thousand cycles of a SIMD.  No value
-// is therefore ever dequantised: the matrix cores multiply the codes, and scale and
-// offset enter where a tile has few numbers.
+// What bounds it is the vector ALU beside the bytes: a tile of 32 keys is 64 d values in
+// 64 lanes; its 4.4 KB (d 128) come from HBM in 0.75 us where all 1024 SIMDs load, and a
+// SIMD with four waves works on it for 0.63 us.  No value is therefore ever dequantised:
+// the matrix cores multiply the codes, and scale and offset enter where a tile has few
+// numbers.  Measured (32 query heads on 8 KV heads, d 128, bfloat16, pages of 64):
+//   64 sequences of 8192 keys   111 us + 5 joining parts, 5.1 TB/s (a plain copy: 6.0)
+//   3 of 65537 to 81920         52.4 + 5.3, 4.6 TB/s
+//   32 of 300 to 4096           25.7 (77 MB; the longest sequences' workgroups end last)
+//   1 of 1000                   11.6: 6.2 with a single key, then 0.6 per tile of a SIMD
+//   2 x 301 to 512 queries behind 3001 to 4096 keys: 120 us, 380 TFLOP/s; a tile's codes
+//     are unpacked again for every 32 query rows, and 72% of the CUs' time is used (800
+//     workgroups on 512 places)
+// 16 queries x 8 heads on one KV head, d 64, float16, up to 8192 keys: 11.6 + 3.9.
 //   * A word holds 8 codes; (w >> 4 i) & 0x000F000F | bias makes two of them
 //     numbers at once, 128 + c in bfloat16 or 64 + c in float16 (the code lands in the
 //     mantissa): 7 operations for 8 codes.
@@ -220,6 +230,13 @@ __device__ __forceinline__ float int4_row(float v) {
   return Op::apply(v, __shfl_xor(v, 32));
 }
 
+// the largest of three (fmaxf quiets each of its operands first: an operation more each)
+__device__ __forceinline__ float int4_max3(float a, float b, float c) {
+  float m;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+  return m;
+}
+
 // Keys of a sequence that its queries (those the grid covers) see, in tiles of 64:
 // from kbeg on, n of them; n = 0 where there is no query, else at least 1.
 struct Int4Span {
@@ -273,7 +290,7 @@ __device__ __forceinline__ Int4Part int4_deal(const AttnInt4Args& p, Int4Span& s
   return w;
 }
 
-// The four waves' partial rows of a workgroup joined: row r's O unnormalised in wave w's
+// The waves' partial rows of a workgroup joined: row r's O unnormalised in wave w's
 // LDS (16-byte chunks XOR-swizzled by the row), its maximum (log2 units) and sum in
 // ml[w][r].  Writes o and lse, or record rec0.
 template <int D, bool F16, int ROWS, int WLDS, int NW>
@@ -329,7 +346,8 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr int KT = I4_TK * RB;                  // bytes of a tile's K (or V)
   constexpr int TILE = 2 * KT + 256;              // K, V, 64 pairs
   constexpr int PAIRS = 512;                      // the pairs of one tile in fp32
-  // tiles in flight per wave: 35 KiB of LDS per workgroup with one row tile, 70 with two
+  // tiles in flight per wave: four workgroups share a CU's 160 KiB with one row tile (36 and
+  // 38 KiB at d 128 and 64), two with two row tiles or d 256 (65 to 70 KiB), one of 16 waves
   constexpr int ST = RT == 1 ? (D == 64 ? 4 : 2) : (D == 64 ? 7 : 4);
   constexpr int RING = ST * TILE + PAIRS;
   constexpr int DC = KT / 1024;                   // DMA instructions of a tile's K
@@ -400,6 +418,9 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   const int* table = p.table + (long long)w.z * p.table_s;
   const int ntiles = hi > lo ? (hi - lo + I4_TK - 1) / I4_TK : 0;
   const int nloc = ntiles > wave ? (ntiles - wave + NW - 1) / NW : 0;
+  // of this wave's tiles, those whose every key every row sees: free_from .. free_to - 1
+  auto own_tiles = [&](int keys) { return keys < 0 ? 0 : (keys / I4_TK - wave + NW - 1) / NW; };
+  const int free_from = own_tiles(all_from - lo + I4_TK - 1), free_to = own_tiles(min(all_to + 1, hi) - lo);
 
   // pages and rows of this wave's next 32 tiles, one 16-key half per lane; a half
   // without a page (or past the end) reads page 0 and is masked
@@ -422,10 +443,11 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     const int pr[2] = {__builtin_amdgcn_readlane(prow, at), __builtin_amdgcn_readlane(prow, at + 1)};
     const uint32_t dst = ring32 + (j % ST) * TILE;
     const char *ksrc[2], *vsrc[2];
+    // (unsigned halves: a 64-bit product of them is three scalar multiplies, or two)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      ksrc[t] = kbase + (long long)pg[t] * p.k_p + (long long)pr[t] * p.k_r;
-      vsrc[t] = vbase + (long long)pg[t] * p.v_p + (long long)pr[t] * p.v_r;
+      ksrc[t] = kbase + (uint32_t)pg[t] * (uint64_t)p.k_p + (uint64_t)(uint32_t)pr[t] * (uint32_t)p.k_r;
+      vsrc[t] = vbase + (uint32_t)pg[t] * (uint64_t)p.v_p + (uint64_t)(uint32_t)pr[t] * (uint32_t)p.v_r;
     }
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind)
@@ -511,7 +533,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
           s[t][rt][e] = fmaf(kp[e / 2][2 * (e & 1)], acc[rt][e], kp[e / 2][2 * (e & 1) + 1] * qsum[rt]);
     }
     const uint32_t alive = (uint32_t)(live[(i >> 5) & 1] >> (2 * (i & 31))) & 3;
-    const bool mask = alive != 3 || kv0 < all_from || kv0 + I4_TK - 1 > all_to || kv0 + I4_TK > hi;
+    const bool mask = alive != 3 || i < free_from || i >= free_to;
     if (mask) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -536,8 +558,9 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float mh = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
-                             fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
+      const float mh = int4_max3(int4_max3(s[0][rt][0], s[0][rt][1], s[0][rt][2]),
+                                 int4_max3(s[0][rt][3], s[1][rt][0], s[1][rt][1]),
+                                 int4_max3(s[1][rt][2], s[1][rt][3], s[1][rt][3]));
       if (__any(mh > ms[rt] + 8.0f)) {
         const float mt = int4_row<OpMax>(mh);
         const bool move = mt > ms[rt] + 8.0f;
@@ -624,7 +647,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
     if (i + ST < nloc) issue(i + ST);
   }
 
-  // ---- the four waves' partial rows: O through each wave's own ring (16-byte
+  // ---- the waves' partial rows: O through each wave's own ring (16-byte
   // chunks XOR-swizzled by the row), maxima and sums beside it.  Block b = c VN + n,
   // element e: dim 128 c + VN (4 g4 + e) + n.
 #pragma unroll
@@ -652,7 +675,10 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
 }
 
 // Joins the parts of a block of query rows: one wave per row, lane s holds part s's
-// maximum and sum (at most 64 parts), D / 64 outputs per lane.
+// maximum and sum (at most 64 parts), D / 64 outputs per lane.  Latency is all of it, so
+// the records are read before the lengths say how many of them there are (what lies
+// behind the last one is read and left), 32 loads at a time: 42 parts of 96 rows 5.3 us,
+// 6.1 with 8 at a time behind the lengths; 32 parts of 512 rows of 64 dims 3.9 and 4.5.
 template <int D, bool F16, int ROWS>
 __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
   const int lane = threadIdx.x & 63;
@@ -662,28 +688,32 @@ __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
   const int block = id % p.row_blocks, pair = id / p.row_blocks;
   const int z = pair / p.Hkv, hk = pair % p.Hkv;
   const int row = block * ROWS + r;
+  constexpr int E = D / 64, U = 32 / E;
+  using vec = float __attribute__((ext_vector_type(E)));
+  const long long rec = (long long)id * p.splits * ROWS + r;
+  const float* part = p.part + rec * D + lane * E;
+  const float* pair_ml = p.ml + 2 * (rec + (long long)min(lane, p.splits - 1) * ROWS);
+  float m = pair_ml[0], l = pair_ml[1];
+  vec v[U];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = *(const vec*)(part + (long long)min(s0 + u, p.splits - 1) * ROWS * D);
+  };
+  load(0);
   const Int4Span sp = int4_span(p, z);
   if (row >= sp.nq * p.group) return;
   const int c = int4_part(p, sp.n), count = (sp.n + c - 1) / c;
   if (count <= 1) return;  // its workgroup had all of it
-  const long long rec = (long long)id * p.splits * ROWS + r;
-  float m = -__builtin_huge_valf(), l = 0.0f;
-  if (lane < count) {
-    m = p.ml[2 * (rec + (long long)lane * ROWS)];
-    l = p.ml[2 * (rec + (long long)lane * ROWS) + 1];
+  if (lane >= count) {
+    m = -__builtin_huge_valf();
+    l = 0.0f;
   }
   const float mt = wave_reduce<OpMax>(m);
   // no finite score in a part: nothing seen (O = l = 0), or only NaN, which stays
   const float f = m == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(m - mt);
   const float lt = wave_reduce<OpSum>(f * l);
-  constexpr int E = D / 64, U = 8;
-  float acc[E] = {};
-  for (int s0 = 0; s0 < count; s0 += U) {
-    float v[U][E];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[u][e] = p.part[(rec + (long long)min(s0 + u, count - 1) * ROWS) * D + lane * E + e];
+  vec acc = {};
+  for (int s0 = 0;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s0 + u, 63)));
@@ -691,6 +721,8 @@ __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[u][e], acc[e]);
     }
+    if ((s0 += U) >= count) break;
+    load(s0);
   }
   const int i = row / p.group, h = hk * p.group + row % p.group;
   const bool empty = !(lt > 0.0f);  // zero or NaN
@@ -726,8 +758,8 @@ G950_INT4(g950_attn_int4_f16_d64, 64, true, 2)
 G950_INT4(g950_attn_int4_f16_d128, 128, true, 1)
 G950_INT4(g950_attn_int4_f16_d128, 128, true, 2)
 G950_INT4(g950_attn_int4_f16_d256, 256, true, 1)
-// 16 waves to a block (one workgroup per CU): where there are one to two blocks of many
-// keys per CU, and parts would only be joined again.
+// 16 waves to a block (one workgroup per CU): where a CU has a block or two of some
+// length, and parts would only be joined again.
 #define G950_INT4W(NAME, D, F16)                                                                   \
   extern "C" __global__ __launch_bounds__(1024) void NAME##_r1w(const g950::AttnInt4Args p) {     \
     g950::attn_int4_body<D, F16, 1, 16>(p);                                                        \

@@ -56,7 +56,12 @@ __device__ __forceinline__ void block_norm_general_body(const BlockNormArgs& a) 
   }
 }
 
-// ---- one workgroup per row, the row in registers
+// ---- one workgroup per row, the row in registers: x and h are read once, y and n
+// written once, so a large batch is bound by HBM: bfloat16 [8191, 3000] with a gate per
+// channel, 197 MB in 36.9 us, 5.3 TB/s; fp32 [4096, 4096] with a gate for every value, 335 MB
+// in 59.6 us, 5.6 TB/s (a plain copy: 6.0; the general kernel, which reads the row three
+// times over: 233 and 155 us).  16 rows of 4096 take 4.2 us: launch, load, two sums across
+// the workgroup.
 // 16 bytes of a row at any element alignment (the hardware takes unaligned
 // 16-byte accesses: rows of odd length and all alignments share one kernel)
 typedef uint32_t u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));

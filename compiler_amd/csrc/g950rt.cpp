@@ -1843,10 +1843,16 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   vec = vec && (int4 ? rows_at(kc, 4) && rows_at(vc, 4) && rows_at(ks, 4) && rows_at(vs, 4) && rows_at(ko, 16) && rows_at(vo, 16)
                      : rows_at(kc, 16) && rows_at(vc, 16));
   if (vec && rows) {
-    // a wave takes all heads of a token, or fewer while there are CUs without waves
+    // A wave's share of a token's heads (in groups of 1024 / d): two groups, three or more
+    // into 4 bits, where a wave has more to do before it starts (26 thousand tokens of 48 heads
+    // of 128, 6 groups: 112 us by one wave a token, 103 by three, 111 by six; of 80 heads 100, 86
+    // by five; of 32 heads of 256 155, 139 by four; 4 bits, 10 thousand tokens of 48 heads: 48.3,
+    // 47.0 by two, 52 by three; 24 heads of 64, two groups: 34.6 and 46.4 by one, 37.1 and 57.3 by
+    // two), and less while there are fewer than 16 waves for every CU (32 tokens of 48 heads:
+    // 6.8 us by one, 4.6 by four, 4.0 by six).
     const long long groups = (H + 2 * HK + 1024 / D - 1) / (1024 / D);
     const long long cus = m ? m->cus : 256;
-    a.chunks = (int)std::max(1ll, std::min(groups, 16 * cus / std::max(T, 1ll)));
+    a.chunks = (int)std::max({1ll, int4 ? groups / 3 : (groups + 1) / 2, std::min(groups, 16 * cus / std::max(T, 1ll))});
     const long long blocks = (T * a.chunks + 3) / 4;
     if (blocks > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
     char name[64];
@@ -1857,7 +1863,29 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
 }
 
 // How attention over the 4-bit cache cuts a call: blocks of 16 or 32 query rows per
-// (sequence, KV head), and parts of their keys, whose records need a workspace.
+// (sequence, KV head), and parts of their keys, whose records need a workspace.  All of it
+// by the greatest lengths alone; the keys of each sequence are cut by its own on the device.
+// Measured at d 128 in bfloat16, 32 query heads on 8 KV heads:
+//   * 32 rows share an unpacked key or value where there are more than 16 (two chunks of 301
+//     to 512 queries behind 3001 to 4096 keys: 120 us, 140 with 16 rows); d 256 has no
+//     registers for it.
+//   * Parts until there are four workgroups for every CU, of 256 keys or more: 32 sequences
+//     of 300 to 4096 keys 23.0 us, 26.6 with two for every CU, 24.8 and 26.0 with six and
+//     eight; 20 of 3000 to 6000, two queries, 26.7 against 29.4 with two.  8 sequences of
+//     2000 to 4096: 13.6 with parts of at least 128 or 256 keys, 15.1 with 1024.
+//   * Up to 1024 keys one part: 1000 keys of one sequence 13.3 us a call against 16.5 with
+//     parts and the second launch that joins them.
+//   * 16 waves in place of 4 (`wide`) where a CU has a block anyway, and some length for
+//     them: past 512 keys with at most a block per CU (1 sequence of 1000 keys 11.6 us against
+//     12.8, of 600 9.7 and 10.3; 32 of 1000 13.7 and 15.1; but 64 of 1000 24.6 and 19.1), and
+//     past 1024 with one or two per CU, in place of parts.  There a CU takes its next block
+//     when it has done one, which parts cut by the sequences' own lengths do not match where
+//     lengths differ: 32 of 300 to 4096 keys 25.7 us against 23.0 + 4.0 for joining, 40 of 300
+//     to 6000 37.2 and 38.2 + 4.2, 64 of 300 to 8192 63.6 and 77.4 + 4.8; of one length, 32 of
+//     8192 57.0 and 58.4 + 4.8, 64 of 8192 116 and 111 + 4.9; it loses where one or two blocks
+//     of one length do not fill the rounds: 48 of 4000 55.5 and 44.0 + 4.8, 64 of 2048 37.5
+//     and 32.2 + 4.1.  With fewer blocks parts reach more CUs: 1 of 8192 7.5 + 4.5 against
+//     38, 8 of 2000 to 4096 13.6 + 3.9 against 23.7.
 struct Int4Shape {
   long long rows;        // query rows of a block
   long long row_blocks;  // per (sequence, KV head)
@@ -1865,7 +1893,7 @@ struct Int4Shape {
   long long splits;      // parts wanted
   bool wide;             // 16 waves to a workgroup
 };
-constexpr long long kInt4Target = 4, kInt4MinKeys = 256, kInt4OneRange = 1024;
+constexpr long long kInt4Target = 4, kInt4MinKeys = 256, kInt4OneRange = 1024, kInt4WideKeys = 512;
 
 Int4Shape int4_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
                      long long seqlen_k) {
@@ -1875,7 +1903,8 @@ Int4Shape int4_shape(const g950_module* m, long long b, long long h, long long h
   f.row_blocks = (rows + f.rows - 1) / f.rows;
   f.blocks = b * hk * f.row_blocks;
   f.splits = 1;
-  f.wide = f.rows == 16 && d <= 128 && seqlen_k > kInt4OneRange && f.blocks >= cus && f.blocks <= 2 * cus;
+  f.wide = f.rows == 16 && d <= 128 && (seqlen_k > kInt4OneRange ? f.blocks >= cus && f.blocks <= 2 * cus
+                                                                  : seqlen_k > kInt4WideKeys && f.blocks <= cus);
   if (f.blocks && seqlen_k > kInt4OneRange && !f.wide)
     f.splits = std::max(1ll, std::min({kInt4Target * cus / f.blocks, (seqlen_k + kInt4MinKeys - 1) / kInt4MinKeys,
                                        64ll}));  // the merge holds a row's parts in one wave's lanes
@@ -2042,8 +2071,9 @@ int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const
   a.rows = (int)x.shape[0]; a.cols = (int)cols;
   a.act = (int)act; a.dtype = (int)x.v->dtype;
   a.alpha = (float)alpha; a.eps = (float)eps;
-  // the smallest form that holds a row; a gate that is neither contiguous along
-  // the row nor one per row, and longer rows, take the general kernel
+  // the smallest form that holds a row (bfloat16 [8191, 3000]: 256 threads 37.0 us, 512
+  // 50.8); a gate that is neither contiguous along the row nor one per row, and longer
+  // rows, take the general kernel
   static const struct { int items, block; } kForms[] = {{1, 64}, {2, 64}, {1, 256}, {2, 256}, {2, 512}, {2, 1024}, {4, 1024}};
   const long long nv = (cols * x.isz + 15) / 16;
   const int gk = !gate ? 0 : a.g_col == 1 || cols == 1 ? 1 : a.g_col == 0 ? 2 : -1;

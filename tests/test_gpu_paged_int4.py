@@ -287,6 +287,8 @@ ATTEND = {
     "page10": dict(ql=[1, 2], kl=[170, 9], h=4, hk=2, d=128, page=10),
     "wide": dict(ql=[1] * 32, kl=[1 + 37 * i for i in range(32)], h=16, hk=8, d=128, page=16),
     "wide_d64": dict(ql=[1, 0, 1, 2] * 8, kl=[1100 - 31 * i for i in range(32)], h=8, hk=8, d=64, page=64),
+    "wide_few": dict(ql=[3, 1, 2, 0], kl=[1024, 513, 30, 700], h=8, hk=2, d=128, page=16),
+    "wide_few_d64": dict(ql=[2, 5], kl=[2, 1000], h=6, hk=2, d=64, page=32, causal=False, window=(511, 2)),
     "odd_d": dict(ql=[2, 1], kl=[70, 300], h=4, hk=2, d=80, page=16),
     "d2": dict(ql=[2], kl=[70], h=2, hk=1, d=2, page=16),
 }
@@ -360,6 +362,7 @@ def check_attend(c, dt, o, lse):
 
 # the form that a case takes where it has one of its own to show
 FORMS = {"one_key": "_r1", "ranges": "_r1_merge", "rows32": "_r2", "d256": "_r1", "wide": "_r1w", "wide_d64": "_r1w",
+         "wide_few": "_r1w", "wide_few_d64": "_r1w", "local": "_r1w",
          "chunk": "_r2", "page1": "_general", "page10": "_general", "odd_d": "_general", "d2": "_general"}
 
 
@@ -384,7 +387,7 @@ def test_attend_scores_climb():
     check_attend(c, "bfloat16", *attend_run(c, "bfloat16"))
 
 
-@pytest.mark.parametrize("case", ["ranges", "chunk", "odd_d", "local"])
+@pytest.mark.parametrize("case", ["ranges", "chunk", "odd_d", "local", "wide_few", "wide_few_d64"])
 def test_attend_nothing_leaks_from_unseen_places(case):
     """NaN scales in every cache row that no query sees: behind the sequences'
     ends, in unused pages, and (for the causal queries) after them."""
@@ -414,7 +417,7 @@ def test_attend_nan_after_a_query_stays_there():
     assert torch.isnan(o[90:130]).all()
 
 
-@pytest.mark.parametrize("case", ["ranges", "chunk", "odd_d", "page10", "d256"])
+@pytest.mark.parametrize("case", ["ranges", "chunk", "odd_d", "page10", "d256", "wide_few"])
 def test_attend_bad_pages_count_as_no_keys(case):
     c = attend_case(case, "bfloat16")
     c["table"][0, 0], c["table"][0, -1], c["table"][-1, 0] = -1, c["pool"], 1 << 30
@@ -531,6 +534,21 @@ def test_append_then_attend_steps():
             # keys); the bars of the 16-bit kernels
             assert torch.allclose(o[at:at + n[i]].double(), w, rtol=2e-2, atol=4e-2)
             at += n[i]
+
+
+@pytest.mark.parametrize("case", ["ranges", "rows32", "d256", "ranges_d64"])
+def test_attend_workspace_may_hold_anything(case):
+    """The records of parts that a shorter sequence does not have count for nothing."""
+    c = attend_case(case, "bfloat16")
+    c["seqlen_k"] = 4096  # more parts than any sequence has
+    args = attend_args(c, "bfloat16")
+    size = rt.module().attention_int4_workspace(len(c["used"]), c["h"], c["hk"], c["d"], c["seqlen_q"], 4096)
+    got = []
+    for fill in (0.0, math.nan, math.inf):
+        got.append(attend_run(c, "bfloat16", args, workspace=torch.full((size,), fill, device="cuda")))
+        assert rt.module().last_kernel.endswith("_merge")
+    assert all(torch.equal(a, b) for g in got[1:] for a, b in zip(g, got[0]))
+    check_attend(c, "bfloat16", *got[0])
 
 
 def test_attend_parts_in_captured_graphs():
