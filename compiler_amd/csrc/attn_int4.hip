@@ -347,8 +347,9 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   constexpr int TILE = 2 * KT + 256;              // K, V, 64 pairs
   constexpr int PAIRS = 512;                      // the pairs of one tile in fp32
   // tiles in flight per wave: four workgroups share a CU's 160 KiB with one row tile (36 and
-  // 38 KiB at d 128 and 64), two with two row tiles or d 256 (65 to 70 KiB), one of 16 waves
-  constexpr int ST = RT == 1 ? (D == 64 ? 4 : 2) : (D == 64 ? 7 : 4);
+  // 38 KiB at d 128 and 64), three with two at d 64 (48), two at d 128 and with d 256 (69 and
+  // 70), one of 16 waves
+  constexpr int ST = RT == 1 ? (D == 64 ? 4 : 2) : (D == 64 ? 5 : 4);
   constexpr int RING = ST * TILE + PAIRS;
   constexpr int DC = KT / 1024;                   // DMA instructions of a tile's K
   constexpr int DPT = 2 * DC + 1;
@@ -740,9 +741,11 @@ __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
 extern "C" __global__ __launch_bounds__(64) void g950_attn_int4_general(const g950::AttnInt4Args p) {
   g950::attn_int4_general_body(p);
 }
-// Four workgroups per CU with one row tile (128 registers), else two.
+// Four workgroups per CU with one row tile (128 registers), three with two at d 64 (two
+// chunks of 301 to 512 queries behind 3001 to 4096 keys: 89 us, 98 with two and seven tiles
+// in flight), else two (at d 128 a third would spill: 206 us against 119).
 #define G950_INT4(NAME, D, F16, RT)                                                                    \
-  extern "C" __global__ __launch_bounds__(256, RT == 1 && D < 256 ? 4 : 2) void NAME##_r##RT(const g950::AttnInt4Args p) {      \
+  extern "C" __global__ __launch_bounds__(256, RT == 1 && D < 256 ? 4 : D == 64 ? 3 : 2) void NAME##_r##RT(const g950::AttnInt4Args p) {      \
     g950::attn_int4_body<D, F16, RT, 4>(p);                                                               \
   }                                                                                                    \
   extern "C" __global__ __launch_bounds__(256) void NAME##_r##RT##_merge(const g950::AttnInt4Args p) { \

@@ -417,6 +417,21 @@ def test_attend_nan_after_a_query_stays_there():
     assert torch.isnan(o[90:130]).all()
 
 
+@pytest.mark.parametrize("case", ["ranges", "chunk", "rows17", "wide_few", "odd_d", "d256"])
+def test_attend_bad_query_rows_stay_alone(case):
+    """NaN or infinities in one query row (one head of one token) leave the others' bits."""
+    c = attend_case(case, "bfloat16")
+    want = [x.clone() for x in attend_run(c, "bfloat16")]
+    t, h = 1, c["h"] - 1
+    keep = torch.ones(c["q"].shape[:2], dtype=torch.bool, device="cuda")
+    keep[t, h] = False
+    for bad in (np.nan, np.inf, -np.inf):
+        c["q"][t, h, 5] = bad
+        o, lse = attend_run(c, "bfloat16")
+        assert torch.equal(o[keep], want[0][keep]) and torch.equal(lse.t()[keep], want[1].t()[keep])
+        assert torch.isnan(o[t, h]).all()
+
+
 @pytest.mark.parametrize("case", ["ranges", "chunk", "odd_d", "page10", "d256", "wide_few"])
 def test_attend_bad_pages_count_as_no_keys(case):
     c = attend_case(case, "bfloat16")
