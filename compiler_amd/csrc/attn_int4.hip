@@ -125,15 +125,7 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
 // 64 lanes; its 4.4 KB (d 128) come from HBM in 0.75 us where all 1024 SIMDs load, and a
 // SIMD with four waves works on it for 0.63 us.  No value is therefore ever dequantised:
 // the matrix cores multiply the codes, and scale and offset enter where a tile has few
-// numbers.  Measured (32 query heads on 8 KV heads, d 128, bfloat16, pages of 64):
-//   64 sequences of 8192 keys   111 us + 5 joining parts, 5.1 TB/s (a plain copy: 6.0)
-//   3 of 65537 to 81920         52.4 + 5.3, 4.6 TB/s
-//   32 of 300 to 4096           25.7 (77 MB; the longest sequences' workgroups end last)
-//   1 of 1000                   11.6: 6.2 with a single key, then 0.6 per tile of a SIMD
-//   2 x 301 to 512 queries behind 3001 to 4096 keys: 120 us, 380 TFLOP/s; a tile's codes
-//     are unpacked again for every 32 query rows, and 72% of the CUs' time is used (800
-//     workgroups on 512 places)
-// 16 queries x 8 heads on one KV head, d 64, float16, up to 8192 keys: 11.6 + 3.9.
+// numbers.
 //   * A word holds 8 codes; (w >> 4 i) & 0x000F000F | bias makes two of them
 //     numbers at once, 128 + c in bfloat16 or 64 + c in float16 (the code lands in the
 //     mantissa): 7 operations for 8 codes.
@@ -150,6 +142,16 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
 //     four rows of a read lie in different LDS banks.
 //   * K's dims are taken in the order in which the words hold them; q's fragments
 //     are laid out to match, once.
+// Measured, in us (32 query heads on 8 KV heads, d 128, bfloat16, pages of 64):
+//   64 sequences of 8192 keys  114, 5.0 TB/s (a plain copy: 6.0)
+//   3 of 65537 to 81920        51.7 and 5.2 for joining the parts, 4.7 TB/s
+//   32 of 300 to 4096          25.5 (77 MB; the longest sequences' workgroups end last)
+//   1 of 1000                  11.5: 6.2 with a single key, then 0.6 per tile of a SIMD
+//   2 of 301 to 512 queries behind 3001 to 4096 keys: 120, 385 TFLOP/s; a tile's codes are
+//     unpacked again for every 32 query rows, and 72% of the CUs' time is used (800
+//     workgroups on 512 places)
+// 16 sequences of 4 queries, 8 heads on one KV head, d 64, float16, 511 to 8192 keys: 11.4
+// and 3.9.
 constexpr int I4_TK = 32;  // keys per tile of one wave
 
 __device__ __forceinline__ void dma_lane16(const char* src, uint32_t lds_dst) {
@@ -274,17 +276,20 @@ struct Int4Part {
   int z, hk, block, t0, t1, rec;
 };
 // tiles of a part, of n
-__device__ __forceinline__ int int4_part(const AttnInt4Args& p, int n) { return max((n + p.splits - 1) / p.splits, 4); }
+__device__ __forceinline__ int int4_part(const AttnInt4Args& p, int n) {
+  return max((int)((uint32_t)(n + p.splits - 1) / (uint32_t)p.splits), 4);
+}
 __device__ __forceinline__ Int4Part int4_deal(const AttnInt4Args& p, Int4Span& sp) {
-  const int pairs = p.B * p.Hkv, units = pairs * p.row_blocks;
-  const int split = blockIdx.x / units, unit = blockIdx.x % units;
+  // (unsigned: a division is a third shorter)
+  const uint32_t heads = p.Hkv, pairs = p.B * heads, units = pairs * p.row_blocks;
+  const uint32_t split = blockIdx.x / units, unit = blockIdx.x % units, pair = unit % pairs;
   Int4Part w;
-  w.z = (unit % pairs / p.Hkv + split * p.turn) % p.B;
-  w.hk = unit % p.Hkv;
-  w.block = p.row_blocks - 1 - unit / pairs;  // those that see most keys first
+  w.z = (pair / heads + split * (uint32_t)p.turn) % (uint32_t)p.B;
+  w.hk = pair % heads;
+  w.block = p.row_blocks - 1 - (int)(unit / pairs);  // those that see most keys first
   sp = int4_span(p, w.z);
   const int c = int4_part(p, sp.n);
-  w.t0 = split * c;
+  w.t0 = (int)split * c;
   w.t1 = min(sp.n, w.t0 + c);
   w.rec = sp.n <= c ? -1 : ((w.z * p.Hkv + w.hk) * p.row_blocks + w.block) * p.splits + split;
   return w;
@@ -296,7 +301,7 @@ __device__ __forceinline__ Int4Part int4_deal(const AttnInt4Args& p, Int4Span& s
 template <int D, bool F16, int ROWS, int WLDS, int NW>
 __device__ __forceinline__ void int4_finish(const AttnInt4Args& p, const char* lds, const float* ml, const Int4Seq& sq,
                                             int hk, int rec0, int row0, int nrows) {
-  const int G = p.group;
+  const uint32_t G = p.group;
   constexpr int CPR = D / 4;  // 16-byte chunks (4 d) per row
   for (int it = threadIdx.x; it < nrows * CPR; it += NW * 64) {
     const int r = it / CPR, c = it % CPR;
@@ -324,7 +329,7 @@ __device__ __forceinline__ void int4_finish(const AttnInt4Args& p, const char* l
       }
       continue;
     }
-    const int i = (row0 + r) / G, h = hk * G + (row0 + r) % G;
+    const int i = (uint32_t)(row0 + r) / G, h = hk * G + (uint32_t)(row0 + r) % G;
     const bool empty = !(lt > 0.0f);  // zero or NaN
     const float inv = empty ? 1.0f : 1.0f / lt;
     char* dst = (char*)p.o + 2 * ((long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + c * 4);
@@ -368,18 +373,18 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, l16 = lane & 15;
-  const int G = p.group;
+  const uint32_t G = p.group;
   Int4Span sp;
   const Int4Part w = int4_deal(p, sp);
   const int hk = w.hk;
   const Int4Seq& sq = sp.sq;
-  const int rows = sp.nq * G;  // of this sequence and KV head
+  const int rows = sp.nq * p.group;  // of this sequence and KV head
   const int row0 = w.block * ROWS;
   if (row0 >= rows || w.t0 >= sp.n) return;
   const int nrows = min(ROWS, rows - row0);
   auto first_key = [&](int i) { return sp.first_key(p, i); };
   auto last_key = [&](int i) { return sp.last_key(p, i); };
-  const int i_lo = row0 / G, i_hi = (row0 + nrows - 1) / G;
+  const int i_lo = (uint32_t)row0 / G, i_hi = (uint32_t)(row0 + nrows - 1) / G;
   const int all_from = first_key(i_hi), all_to = last_key(i_lo);  // keys every row sees
   const int lo = max(sp.kbeg + 64 * w.t0, first_key(i_lo) / I4_TK * I4_TK);
   const int hi = min(last_key(i_hi) + 1, w.t1 < sp.n ? sp.kbeg + 64 * w.t1 : 0x7FFFFFFF);
@@ -391,7 +396,7 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
   int kmin[RT], kmax[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = row0 + min(rt * 16 + l16, nrows - 1);
+    const uint32_t r = row0 + min(rt * 16 + l16, nrows - 1);
     const int i = r / G, h = hk * G + r % G;
     kmin[rt] = first_key(i);
     kmax[rt] = last_key(i);
@@ -683,11 +688,12 @@ __device__ __forceinline__ void attn_int4_body(const AttnInt4Args& p) {
 template <int D, bool F16, int ROWS>
 __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
   const int lane = threadIdx.x & 63;
-  const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int id = (int)(item / p.merge_rows), r = (int)(item % p.merge_rows);
-  if (id >= p.B * p.Hkv * p.row_blocks) return;
-  const int block = id % p.row_blocks, pair = id / p.row_blocks;
-  const int z = pair / p.Hkv, hk = pair % p.Hkv;
+  // (parts are wanted for a few blocks per CU only: 32 bits hold their rows)
+  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t id = item / (uint32_t)p.merge_rows, r = item % (uint32_t)p.merge_rows;
+  if (id >= (uint32_t)(p.B * p.Hkv * p.row_blocks)) return;
+  const uint32_t blocks = p.row_blocks, heads = p.Hkv, pair = id / blocks;
+  const int block = id % blocks, z = pair / heads, hk = pair % heads;
   const int row = block * ROWS + r;
   constexpr int E = D / 64, U = 32 / E;
   using vec = float __attribute__((ext_vector_type(E)));
@@ -725,7 +731,7 @@ __device__ __forceinline__ void attn_int4_merge_body(const AttnInt4Args& p) {
     if ((s0 += U) >= count) break;
     load(s0);
   }
-  const int i = row / p.group, h = hk * p.group + row % p.group;
+  const int i = (uint32_t)row / (uint32_t)p.group, h = hk * p.group + (uint32_t)row % (uint32_t)p.group;
   const bool empty = !(lt > 0.0f);  // zero or NaN
   const float inv = empty ? 1.0f : 1.0f / lt;
   uint16_t* dst = (uint16_t*)p.o + (long long)(sp.sq.q0 + i) * p.o_st + (long long)h * p.o_sh + lane * E;
