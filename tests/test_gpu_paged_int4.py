@@ -73,6 +73,7 @@ APPEND = {
     "page1": dict(ql=[6, 2], kl=[6, 3], h=4, hk=2, d=64, page=1),
     "many_sequences": dict(ql=[1, 0, 2] * 60, kl=[1 + i for i in range(180)], h=2, hk=1, d=64, page=16),
     "no_queries": dict(ql=[3, 4], kl=[3, 40], h=0, hk=2, d=128, page=16),
+    "many_tokens": dict(ql=[1403, 0, 697], kl=[1410, 3, 697], h=43, hk=6, d=128, page=64),  # several groups of heads a wave
 }
 
 
