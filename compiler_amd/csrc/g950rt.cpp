@@ -1831,14 +1831,14 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   a.interleaved = interleaved ? 1 : 0;
   a.dtype = (int)dt; a.table_dtype = (int)cos.v->dtype; a.int4 = int4 ? 1 : 0;
   const long long rows = a.B ? T * (H + 2 * HK) : 0;
-  // whole vectors: rows of 32 to 256 dims (a power of two) that turn as a whole or
-  // not at all, 16-byte rows everywhere (4-byte code words and pairs)
+  // whole vectors: rows of 32 to 256 dims (a power of two), a multiple of 16 of which
+  // turn, 16-byte rows everywhere (4-byte code words and pairs)
   auto rows_at = [&](const View& w, int bytes) {
     bool ok = w.addr() % bytes == 0;
     for (int d = 0; d + 1 < w.nd; ++d) ok = ok && w.stride[d] * w.isz % bytes == 0;
     return ok || no_elements(w);
   };
-  bool vec = (D == 32 || D == 64 || D == 128 || D == 256) && (R == 0 || R == D) && rows_at(q, 16) && rows_at(k, 16) &&
+  bool vec = (D == 32 || D == 64 || D == 128 || D == 256) && R % 16 == 0 && rows_at(q, 16) && rows_at(k, 16) &&
              rows_at(v, 16) && rows_at(qo, 16) && (R == 0 || (rows_at(cos, 16) && rows_at(sin, 16)));
   vec = vec && (int4 ? rows_at(kc, 4) && rows_at(vc, 4) && rows_at(ks, 4) && rows_at(vs, 4) && rows_at(ko, 16) && rows_at(vo, 16)
                      : rows_at(kc, 16) && rows_at(vc, 16));

@@ -205,19 +205,22 @@ __device__ __forceinline__ void kv_append_general_body(const KvAppendArgs& a) {
   }
 }
 
-// ---- whole vectors: D = 16 L dims, L a power of two; all of them turn or none
+// ---- whole vectors: D = 16 L dims, L a power of two; a multiple of 16 of them turn
 // A wave takes a token's heads, 64 / L at a time (queries, then keys, then
-// values); lane u of a head holds dims 8 u .. and D / 2 + 8 u .., so that both
-// members of a pair (i, i + D / 2), or of two pairs (2i, 2i + 1), are its own, and
+// values); lane u of a head holds 8 dims of either half of those that turn (u < R /
+// 16: dims 8 u .. and R / 2 + 8 u ..) or of the rest, so that both members of a pair
+// (i, i + R / 2), or of pairs (2i, 2i + 1), are its own, and
 // a row's cos and sin are loaded once for all heads.  The first heads' loads
 // are issued before the token's place is looked up (three dependent loads), the
 // next heads' before these are stored.
 //
 // A prompt is bound by HBM: 8 prompts of 2304 to 4096 tokens, 32 + 8 + 8 heads of 128
 // dims in bfloat16, 631 MB in and out in 103 us, 6.1 TB/s (a plain copy reaches 6.0 on this
-// card); into 4 bits, values wanted, 245 MB in 47 us, 5.2 TB/s.  Loads and stores pass
+// card); into 4 bits, values wanted, 245 MB in 45 us, 5.4 TB/s.  Loads and stores pass
 // the caches where a row is used once: a tenth longer without (4 bits: no difference, so
-// only the loads do).  A decoding step is bound by its chain of loads: 32 tokens 3.9 us, 13
+// only the loads do).  Where fewer dims turn a head is read in shorter runs: 16 thousand
+// tokens of the same heads take 68 us where 128 dims turn, 84 where 64 and 96 where 32 do
+// (the general kernel, with 24: 726).  A decoding step is bound by its chain of loads: 32 tokens 3.9 us, 13
 // sequences of 1 to 5 tokens into 4 bits 5.5 us.
 template <typename T>
 __device__ __forceinline__ void kv_load8(const char* p, float* v) {
@@ -277,6 +280,8 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
   const int t = (int)(w / a.chunks), chunk = (int)(w % a.chunks);
   if (t >= a.T) return;
   const int slots = a.Hq + 2 * a.Hkv, groups = (slots + RPW - 1) / RPW;
+  const bool turns = u < a.R / 16;
+  const int from[2] = {turns ? 8 * u : a.R + 8 * (u - a.R / 16), turns ? a.R / 2 + 8 * u : (a.R + D) / 2 + 8 * (u - a.R / 16)};
   const char* qrow = (const char*)a.q + t * a.q_st * SZ;
   const char* krow = (const char*)a.k + t * a.k_st * SZ;
   const char* vrow = (const char*)a.v + t * a.v_st * SZ;
@@ -285,17 +290,17 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
     const int s = min(g * RPW + sub, slots - 1);
     const char* p = s < a.Hq ? qrow + s * a.q_sh * SZ
                              : s < a.Hq + a.Hkv ? krow + (s - a.Hq) * a.k_sh * SZ : vrow + (s - a.Hq - a.Hkv) * a.v_sh * SZ;
-    kv_load8<T>(p + u * 8 * SZ, x[0]);
-    kv_load8<T>(p + (D / 2 + u * 8) * SZ, x[1]);
+    kv_load8<T>(p + from[0] * SZ, x[0]);
+    kv_load8<T>(p + from[1] * SZ, x[1]);
   };
   float x[2][8];
   load(chunk, x);
   const KvPlace at = kv_place(a, t);
   if (at.seq < 0) return;
-  float c[8], s[8];
-  if (a.R) {
-    // half-split: pairs 8 u .. + 7; interleaved: 4 u .. + 3 and D / 4 + 4 u .. + 3
-    const int i0 = a.interleaved ? 4 * u : 8 * u, i1 = a.interleaved ? D / 4 + 4 * u : 8 * u + 4;
+  float c[8] = {}, s[8] = {};
+  if (turns) {
+    // half-split: pairs 8 u .. + 7; interleaved: 4 u .. + 3 and R / 4 + 4 u .. + 3
+    const int i0 = a.interleaved ? 4 * u : 8 * u, i1 = a.interleaved ? a.R / 4 + 4 * u : 8 * u + 4;
     const long long co = at.pos * a.cos_s, so = at.pos * a.sin_s;
     if (a.table_dtype == DT_F32) {
       const f32x4 c0 = *(const f32x4*)((const float*)a.cos + co + i0), c1 = *(const f32x4*)((const float*)a.cos + co + i1);
@@ -334,14 +339,14 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
 #pragma unroll
       for (int v = 0; v < 2; ++v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[v][e] = is_v ? x[v][e] : y[v][e];
+        for (int e = 0; e < 8; ++e) x[v][e] = is_v || !turns ? x[v][e] : y[v][e];
     }
     if (slot < slots && (is_q || (!INT4 && at.page >= 0))) {
       char* p = is_q ? (char*)a.q_out + (t * a.qo_st + h * a.qo_sh) * SZ
                      : is_v ? (char*)a.v_cache + (at.page * a.vc_p + at.row * a.vc_r + h * a.vc_h) * SZ
                             : (char*)a.k_cache + (at.page * a.kc_p + at.row * a.kc_r + h * a.kc_h) * SZ;
-      kv_store8<T, !INT4>(p + u * 8 * SZ, x[0]);
-      kv_store8<T, !INT4>(p + (D / 2 + u * 8) * SZ, x[1]);
+      kv_store8<T, !INT4>(p + from[0] * SZ, x[0]);
+      kv_store8<T, !INT4>(p + from[1] * SZ, x[1]);
     }
     if constexpr (INT4) {
       if (g * RPW + RPW > a.Hq) {  // (uniform) some lane holds a key or value
@@ -375,14 +380,14 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
             for (int v = 0; v < 2; ++v) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) x[v][e] = kv_value(code[v][e], k);
-              kv_store8<T, false>(out + (v * D / 2 + u * 8) * SZ, x[v]);
+              kv_store8<T, false>(out + from[v] * SZ, x[v]);
             }
           }
           if (at.page >= 0) {
             char* dst = is_v ? (char*)a.v_cache + (at.page * a.vc_p + at.row * a.vc_r + h * a.vc_h)
                              : (char*)a.k_cache + (at.page * a.kc_p + at.row * a.kc_r + h * a.kc_h);
-            *(uint32_t*)(dst + 4 * u) = word[0];
-            *(uint32_t*)(dst + D / 4 + 4 * u) = word[1];
+            *(uint32_t*)(dst + from[0] / 2) = word[0];
+            *(uint32_t*)(dst + from[1] / 2) = word[1];
             if (u == 0) {
               char* sc = is_v ? (char*)a.v_scale + 2 * (at.page * a.vs_p + at.row * a.vs_r + h * a.vs_h)
                               : (char*)a.k_scale + 2 * (at.page * a.ks_p + at.row * a.ks_r + h * a.ks_h);

@@ -76,6 +76,8 @@ def test_append_is_taken(four):
         assert rc == 0 and name.startswith("g950_kv_append"), (kw, err)
     if not four:
         assert append(dt=F32)[0] == 0 and append(d=300)[0] == 0
+    for r, general in ((128, False), (0, False), (16, False), (96, False), (32, False), (24, True), (2, True)):
+        assert append(four, r=r)[1].endswith("_general") == general, r
 
 
 @pytest.mark.parametrize("four", [False, True])

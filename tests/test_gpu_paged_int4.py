@@ -65,6 +65,9 @@ APPEND = {
     "empty_sequences": dict(ql=[0, 4, 0, 0, 2, 0], kl=[9, 4, 0, 7, 30, 1], h=4, hk=2, d=128, page=16),
     "partial": dict(ql=[5, 6], kl=[5, 20], h=4, hk=2, d=128, page=16, r=32),
     "partial_interleaved": dict(ql=[5, 6], kl=[5, 20], h=4, hk=2, d=64, page=16, r=32, interleaved=True),
+    "partial_96": dict(ql=[5, 6], kl=[5, 20], h=4, hk=2, d=256, page=16, r=96),
+    "partial_16_interleaved": dict(ql=[5, 6], kl=[9, 20], h=4, hk=2, d=32, page=16, r=16, interleaved=True),
+    "partial_odd": dict(ql=[5, 6], kl=[5, 20], h=4, hk=2, d=128, page=16, r=26),
     "unturned": dict(ql=[5, 6], kl=[5, 20], h=4, hk=2, d=128, page=16, r=0),
     "odd_d": dict(ql=[4, 3], kl=[4, 11], h=3, hk=3, d=80, page=7),
     "d96": dict(ql=[4, 3], kl=[4, 11], h=6, hk=2, d=96, page=16),
