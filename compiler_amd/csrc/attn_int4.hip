@@ -751,8 +751,9 @@ extern "C" __global__ __launch_bounds__(64) void g950_attn_int4_general(const g9
 // chunks of 301 to 512 queries behind 3001 to 4096 keys: 89 us, 98 with two and seven tiles
 // in flight), else two (at d 128 a third would spill: 206 us against 119).
 #define G950_INT4(NAME, D, F16, RT)                                                                    \
-  extern "C" __global__ __launch_bounds__(256, RT == 1 && D < 256 ? 4 : D == 64 ? 3 : 2) void NAME##_r##RT(const g950::AttnInt4Args p) {      \
-    g950::attn_int4_body<D, F16, RT, 4>(p);                                                               \
+  extern "C" __global__ __launch_bounds__(256, RT == 1 && D < 256 ? 4 : D == 64 ? 3 : 2) void           \
+      NAME##_r##RT(const g950::AttnInt4Args p) {                                                       \
+    g950::attn_int4_body<D, F16, RT, 4>(p);                                                            \
   }                                                                                                    \
   extern "C" __global__ __launch_bounds__(256) void NAME##_r##RT##_merge(const g950::AttnInt4Args p) { \
     g950::attn_int4_merge_body<D, F16, 16 * RT>(p);                                                    \

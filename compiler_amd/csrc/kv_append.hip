@@ -127,7 +127,7 @@ __device__ __forceinline__ float kv_value(int c, const KvScale& k) {
 
 // One wave per (token, head) row: any D, R, stride and alignment.  Each row looks its
 // place up and each element reads its own cos and sin: 988 us where the vector kernel
-// takes 103 (26 thousand tokens, below), 489 against 47 into 4 bits.
+// takes 103 (26 thousand tokens, below), 489 against 44 into 4 bits.
 __device__ __forceinline__ void kv_append_general_body(const KvAppendArgs& a) {
   const int lane = threadIdx.x & 63;
   const int slots = a.Hq + 2 * a.Hkv;
@@ -216,7 +216,7 @@ __device__ __forceinline__ void kv_append_general_body(const KvAppendArgs& a) {
 //
 // A prompt is bound by HBM: 8 prompts of 2304 to 4096 tokens, 32 + 8 + 8 heads of 128
 // dims in bfloat16, 631 MB in and out in 103 us, 6.1 TB/s (a plain copy reaches 6.0 on this
-// card); into 4 bits, values wanted, 245 MB in 45 us, 5.4 TB/s.  Loads and stores pass
+// card); into 4 bits, values wanted, 245 MB in 44 us, 5.5 TB/s.  Loads and stores pass
 // the caches where a row is used once: a tenth longer without (4 bits: no difference, so
 // only the loads do).  Where fewer dims turn a head is read in shorter runs: 16 thousand
 // tokens of the same heads take 68 us where 128 dims turn, 84 where 64 and 96 where 32 do
