@@ -2037,7 +2037,8 @@ int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const
   };
   for (const View* w : {&x, &h, &y})
     if (int rc = rows_as_x(*w)) return rc;
-  if (x.shape[0] > 0x7FFFFFFF || x.shape[1] > 0x7FFFFFFF) return fail(G950_USAGE, "block_norm: extent too large");
+  // (columns: the general kernel's 32-bit position goes a step of 256 past the last)
+  if (x.shape[0] > 0x7FFFFFFF || x.shape[1] > 0x7FFFFFFF - 255) return fail(G950_USAGE, "block_norm: extent too large");
   double eps, alpha;
   long long act;
   if (int rc = scalar_float(&sc[0], "eps", eps)) return rc;

@@ -229,7 +229,8 @@ typedef struct g950_scalar {
  * G950_OP_BLOCK_NORM   the norms around a block with its gate and residual:
  *                      u = H rsqrt(mean(H^2) + eps) W_post (H itself without W_post),
  *                      Y = residual_scale X + act(G) u, N = Y rsqrt(mean(Y^2) + eps) W_pre
- *                      of Y before its rounding.  Y may be X and N may be H.
+ *                      of Y before its rounding.  Y may be X and N may be H.  C is at
+ *                      most 2^31 - 256.
  *   views   G[R,C] (strides may be 0) or empty, H[R,C], N[R,C] (empty without
  *           W_pre), W_post[C] or empty, W_pre[C] or empty, X[R,C], Y[R,C]: one
  *           float dtype

@@ -176,6 +176,15 @@ def test_attend_sizes_past_every_grid():
     assert size(1, 8, 8, 128, 1, 1000) == 0 < size(1, 8, 8, 128, 1, 5000)
 
 
+def test_block_norm_longest_rows():
+    """Positions of a row count on by 256 in 32 bits until they pass its end."""
+    for dt in (BF, F32):
+        long = dict(rows=1, dt=dt, W_post=dict(shape=[0]), W_pre=dict(shape=[0]), N=dict(shape=[0, 0]))
+        assert norm(cols=2 ** 31 - 256, **long)[:2] == (0, "g950_block_norm_general")
+        for cols in (2 ** 31 - 255, 2 ** 31 - 1, 2 ** 31):
+            refused(norm(cols=cols, **long), rt.USAGE, "extent too large")
+
+
 # ------------------------------------------------------- the oracle's own pins
 def test_oracle_quantize_bounds_and_special_rows():
     rng = np.random.default_rng(0)
