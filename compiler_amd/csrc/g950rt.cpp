@@ -225,11 +225,17 @@ hipFunction_t function(g950_module* m, const std::string& name) {
   return f;
 }
 
+// Most workgroups of one launch: its work-items are counted in 32 bits.
+constexpr unsigned max_grid(unsigned block) { return 0xFFFFFFFFu / block; }
+
 template <class Args>
 int launch(g950_module* m, const std::string& name, unsigned grid, unsigned block, Args& args,
            void* stream) {
   t_form = t_next_form;
   t_next_form = "";
+  if (grid > max_grid(block))
+    return fail(G950_USAGE, "%s: grid too large (%u workgroups of %u; a launch counts its work-items in 32 bits)",
+                name.c_str(), grid, block);
   if (!m) {  // validation only (g950_validate): report the choice, launch nothing
     t_kernel = name;
     return G950_OK;
@@ -1854,10 +1860,12 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
     const long long cus = m ? m->cus : 256;
     a.chunks = (int)std::max({1ll, int4 ? groups / 3 : (groups + 1) / 2, std::min(groups, 16 * cus / std::max(T, 1ll))});
     const long long blocks = (T * a.chunks + 3) / 4;
-    if (blocks > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
-    char name[64];
-    snprintf(name, sizeof name, "g950_kv_append%s_%s_d%lld", int4 ? "_int4" : "", rr_dtype(dt), D);
-    return launch(m, name, (unsigned)blocks, 256u, a, stream);
+    // (past 2^26 waves the general kernel, whose waves take several rows)
+    if (blocks <= max_grid(256)) {
+      char name[64];
+      snprintf(name, sizeof name, "g950_kv_append%s_%s_d%lld", int4 ? "_int4" : "", rr_dtype(dt), D);
+      return launch(m, name, (unsigned)blocks, 256u, a, stream);
+    }
   }
   return launch(m, "g950_kv_append_general", (unsigned)std::min((rows + 3) / 4, 1ll << 20), 256u, a, stream);
 }
@@ -2078,13 +2086,25 @@ int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const
   static const struct { int items, block; } kForms[] = {{1, 64}, {2, 64}, {1, 256}, {2, 256}, {2, 512}, {2, 1024}, {4, 1024}};
   const long long nv = (cols * x.isz + 15) / 16;
   const int gk = !gate ? 0 : a.g_col == 1 || cols == 1 ? 1 : a.g_col == 0 ? 2 : -1;
+  char name[64] = "g950_block_norm_general";
+  unsigned block = 256;
   for (const auto& f : kForms) {
     if (gk < 0 || nv > (long long)f.items * f.block) continue;
-    char name[64];
     snprintf(name, sizeof name, "g950_block_norm_%s_i%d_b%d_g%d", rr_dtype(x.v->dtype), f.items, f.block, gk);
-    return launch(m, name, (unsigned)a.rows, (unsigned)f.block, a, stream);
+    block = (unsigned)f.block;
+    break;
   }
-  return launch(m, "g950_block_norm_general", (unsigned)a.rows, 256u, a, stream);
+  // a workgroup per row: more rows than a launch counts take several
+  for (long long left = a.rows;;) {
+    const long long n = std::min<long long>(left, max_grid(block));
+    a.rows = (int)n;
+    if (int rc = launch(m, name, (unsigned)n, block, a, stream)) return rc;
+    if ((left -= n) == 0) return G950_OK;
+    auto on = [&](auto& p, long long row) {
+      if (p) p = (char*)p + n * row * x.isz;
+    };
+    on(a.x, a.x_row); on(a.h, a.h_row); on(a.gate, a.g_row); on(a.y, a.y_row); on(a.n, a.n_row);
+  }
 }
 
 // ------------------------------------------------------------------- copy

@@ -185,6 +185,24 @@ def test_block_norm_longest_rows():
             refused(norm(cols=cols, **long), rt.USAGE, "extent too large")
 
 
+def test_grids_past_32_bits_of_work_items():
+    """A launch counts its work-items (workgroups x threads) in 32 bits.  Norms take
+    several launches then, appends the general kernel; attention is refused."""
+    edge = 2 ** 26 - 1  # waves of one launch
+    for rows in (edge, edge + 1, 2 ** 31 - 1):
+        assert norm(rows=rows, cols=64)[:2] == (0, "g950_block_norm_bf16_i1_b64_g0")
+        assert norm(rows=rows, cols=40000)[:2] == (0, "g950_block_norm_general")
+    for four in (False, True):
+        name = "g950_kv_append%s_bf16_d128" % ("_int4" if four else "")
+        assert append(four, t=edge // 4 * 4, h=1, hk=1)[:2] == (0, name)
+        assert append(four, t=edge // 4 * 4 + 1, h=1, hk=1)[:2] == (0, "g950_kv_append_general")
+    assert attend(t=edge // 2, h=2, hk=2, d=80, sq=5)[:2] == (0, "g950_attn_int4_general")
+    refused(attend(t=edge // 2 + 1, h=2, hk=2, d=80, sq=5), rt.USAGE, "grid too large")
+    long = dict(t=2 ** 27 - 1, sq=2 ** 27 - 1, h=1, hk=1)
+    assert attend(b=3, **long)[:2] == (0, "g950_attn_int4_bf16_d128_r2")
+    refused(attend(b=4, **long), rt.USAGE, "grid too large")
+
+
 # ------------------------------------------------------- the oracle's own pins
 def test_oracle_quantize_bounds_and_special_rows():
     rng = np.random.default_rng(0)

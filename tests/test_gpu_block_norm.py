@@ -150,3 +150,18 @@ def test_block_norm_captured():
         assert all(torch.equal(a, b) for a, b in zip(call(), want))
     with rt.no_alloc():
         assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
+@pytest.mark.parametrize("cols", [1, 3])
+def test_block_norm_rows_past_one_launch(cols):
+    """2^26 - 1 workgroups of 64 threads fill a launch: the rows behind them."""
+    rows = 2 ** 26 + 70
+    x = torch.randn(rows, cols, device="cuda").bfloat16()
+    h = torch.randn(rows, cols, device="cuda").bfloat16()
+    gate = torch.randn(rows, 1, device="cuda").bfloat16()
+    w = torch.randn(cols, device="cuda").bfloat16()
+    y, n = ops.block_norm(x, h, w, 1e-6, w_post=w, gate=gate, sync=True)
+    for s in (slice(0, 100), slice(2 ** 26 - 100, 2 ** 26 + 70)):
+        some = [t[s].clone() for t in (x, h, gate)]
+        sy, sn = ops.block_norm(some[0], some[1], w, 1e-6, w_post=w, gate=some[2], sync=True)
+        assert torch.equal(y[s], sy) and torch.equal(n[s], sn)
