@@ -436,9 +436,13 @@ def paged_append_int4(q, k, v, cos, sin, k_cache, k_scale, v_cache, v_scale, pag
 def _workspace(floats, like, stream):
     """Memory for one call on ``stream`` (None: the current one), which torch
     may hand on when the call returns: to later work of that stream.  None for
-    hipStreamPerThread (handle 2), which names a stream of every thread."""
+    hipStreamPerThread (handle 2, also as torch's current stream), which names a
+    stream of every thread."""
     import torch
-    handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
+    if stream is None:
+        handle = rt._raw_stream(rt.module().device)
+    else:
+        handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
     if stream is None or not floats or handle == 2:
         return torch.empty(0 if handle == 2 else floats, dtype=torch.float32, device=like.device)
     if not hasattr(stream, "cuda_stream"):
