@@ -393,13 +393,45 @@ def _none(dtype, device, rank):
     return torch.empty((0,) * rank, dtype=dtype, device=device)
 
 
+def _torch_stream(stream):
+    """torch's object for a call's ``stream`` (a Stream or a handle); None for
+    hipStreamPerThread (handle 2), whose memory torch would hand on between threads."""
+    import torch
+    if hasattr(stream, "cuda_stream"):
+        return None if stream.cuda_stream == 2 else stream
+    if stream == 2:
+        return None
+    return torch.cuda.ExternalStream(stream) if stream not in (0, 1) else torch.cuda.default_stream()
+
+
+def _on_stream(stream, make):
+    """``make`` (torch.empty, torch.empty_like) for outputs of a call on ``stream``:
+    memory that no other stream's pending work still uses, and that is not handed on
+    before the current stream, where the caller may read it, is done with it."""
+    import torch
+    stream = _torch_stream(stream)
+    if stream is None:
+        return make
+    here = torch.cuda.current_stream()
+
+    def made(*args, **kw):
+        with torch.cuda.stream(stream):
+            t = make(*args, **kw)
+        if stream.cuda_stream != here.cuda_stream and t.numel():
+            t.record_stream(here)
+        return t
+    return made
+
+
 def paged_append(q, k, v, cos, sin, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, interleaved=False,
                  out=None, **kw):
     """Appends k and v to the cache and returns the rotated q (``out=q``: in
     place; q may be None).  See paged_append_kernel."""
     import torch
+    stream = kw.get("stream")
+    empty_like = torch.empty_like if stream is None else _on_stream(stream, torch.empty_like)
     q = k.new_empty((k.shape[0], 0, k.shape[2])) if q is None else q
-    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    out = empty_like(q, memory_format=torch.contiguous_format) if out is None else out
     paged_append_kernel(q, k, v, cos, sin, out, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k,
                         bool(interleaved), **kw)
     return out
@@ -421,11 +453,13 @@ def paged_append_int4(q, k, v, cos, sin, k_cache, k_scale, v_cache, v_scale, pag
     and, with ``values`` (or k_out / v_out given), the appended keys and values
     as the cache holds them; else None for both."""
     import torch
+    stream = kw.get("stream")
+    empty_like = torch.empty_like if stream is None else _on_stream(stream, torch.empty_like)
     q = k.new_empty((k.shape[0], 0, k.shape[2])) if q is None else q
-    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    out = empty_like(q, memory_format=torch.contiguous_format) if out is None else out
     if values:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
-        v_out = torch.empty_like(v, memory_format=torch.contiguous_format) if v_out is None else v_out
+        k_out = empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
+        v_out = empty_like(v, memory_format=torch.contiguous_format) if v_out is None else v_out
     none = _none(k.dtype, k.device, 3)
     paged_append_int4_kernel(q, k, v, cos, sin, out, none if k_out is None else k_out, none if v_out is None else v_out,
                              k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, bool(interleaved),
@@ -440,13 +474,12 @@ def _workspace(floats, like, stream):
     stream of every thread."""
     import torch
     if stream is None:
-        handle = rt._raw_stream(rt.module().device)
+        per_thread = rt._raw_stream(rt.module().device) == 2
     else:
-        handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
-    if stream is None or not floats or handle == 2:
-        return torch.empty(0 if handle == 2 else floats, dtype=torch.float32, device=like.device)
-    if not hasattr(stream, "cuda_stream"):
-        stream = torch.cuda.ExternalStream(handle) if handle else torch.cuda.default_stream()
+        stream = _torch_stream(stream)
+        per_thread = stream is None
+    if stream is None or not floats:
+        return torch.empty(0 if per_thread else floats, dtype=torch.float32, device=like.device)
     with torch.cuda.stream(stream):
         return torch.empty(floats, dtype=torch.float32, device=like.device)
 
@@ -460,11 +493,18 @@ def paged_attention_int4(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_s
     import torch
     t, h, d = q.shape
     seqlen_q, seqlen_k = int(seqlen_q), int(seqlen_k)
-    o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    lse = torch.empty((h, t), dtype=torch.float32, device=q.device) if lse is None else lse
+    stream = kw.get("stream")
+    if out is None:
+        o = (torch.empty_like if stream is None else _on_stream(stream, torch.empty_like))(
+            q, memory_format=torch.contiguous_format)
+    else:
+        o = out
+    if lse is None:
+        lse = (torch.empty if stream is None else _on_stream(stream, torch.empty))(
+            (h, t), dtype=torch.float32, device=q.device)
     if workspace is None:
         workspace = _workspace(rt.module().attention_int4_workspace(
-            cu_seqlens_q.shape[0] - 1, h, k_cache.shape[2], d, min(seqlen_q, t), seqlen_k), q, kw.get("stream"))
+            cu_seqlens_q.shape[0] - 1, h, k_cache.shape[2], d, min(seqlen_q, t), seqlen_k), q, stream)
     paged_attention_int4_kernel(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_seqlens_q, seqused_k, o, lse,
                                 workspace, seqlen_q, seqlen_k, 1.0 / math.sqrt(d) if scale is None else float(scale),
                                 bool(causal), int(window[0]), int(window[1]), **kw)
@@ -482,10 +522,12 @@ def block_norm(x, h, w_pre, eps, w_post=None, gate=None, gate_act=None, residual
     import torch
     if gate_act not in _GATE_ACTS:
         raise rt.G950Error(rt.USAGE, f"block_norm: unknown gate_act {gate_act!r}")
-    y = torch.empty_like(x) if out is None else out
+    stream = kw.get("stream")
+    empty_like = torch.empty_like if stream is None else _on_stream(stream, torch.empty_like)
+    y = empty_like(x) if out is None else out
     n = None
     if w_pre is not None:
-        n = torch.empty_like(x) if norm_out is None else norm_out
+        n = empty_like(x) if norm_out is None else norm_out
     none = _none(x.dtype, x.device, 1)
     if gate is not None and gate.shape != x.shape:
         gate = gate.expand(x.shape)
