@@ -1717,6 +1717,47 @@ int distinct(const View& v, const char* op) {
   return G950_OK;
 }
 
+// Whether the host can see that two views share no byte: their reaches are apart, or
+// interleave with some stride's period (heads of one row of a projection).
+bool apart(const View& a, const View& b) {
+  if (no_elements(a) || no_elements(b)) return true;
+  struct Span { long long lo, len; };  // bytes, without the extents that step by multiples of `period`
+  auto span = [](const View& v, long long period) {
+    Span s{(long long)v.addr(), v.isz};
+    for (int i = 0; i < v.nd; ++i) {
+      const long long step = v.stride[i] * v.isz;
+      if (v.shape[i] == 1 || (period && step % period == 0)) continue;
+      s.len += std::abs(step) * (v.shape[i] - 1);
+      if (step < 0) s.lo += step * (v.shape[i] - 1);
+    }
+    return s;
+  };
+  auto clear = [&](long long period) {
+    const Span p = span(a, period), q = span(b, period);
+    if (!period) return p.lo + p.len <= q.lo || q.lo + q.len <= p.lo;
+    const long long d = ((q.lo - p.lo) % period + period) % period;
+    return p.len <= d && d + q.len <= period;
+  };
+  if (clear(0)) return true;
+  for (const View* v : {&a, &b})
+    for (int i = 0; i < v->nd; ++i)
+      if (v->shape[i] > 1 && v->stride[i] && clear(std::abs((long long)v->stride[i] * v->isz))) return true;
+  return false;
+}
+
+// The same elements in the same places.
+bool same_view(const View& a, const View& b) {
+  bool same = a.addr() == b.addr() && a.nd == b.nd && a.isz == b.isz;
+  for (int i = 0; i < a.nd && same; ++i)
+    same = a.shape[i] == b.shape[i] && (a.shape[i] <= 1 || a.stride[i] == b.stride[i]);
+  return same;
+}
+
+int keep_apart(const View& out, const View& other, const char* op) {
+  if (!apart(out, other)) return fail(G950_USAGE, "%s: %s overlaps %s", op, out.name, other.name);
+  return G950_OK;
+}
+
 int last_contiguous(const View& v, const char* op) {
   if (!no_elements(v) && v.shape[v.nd - 1] > 1 && v.stride[v.nd - 1] != 1)
     return fail(G950_USAGE, "%s: the last axis of %s must be contiguous", op, v.name);
@@ -1799,6 +1840,10 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   if (int rc = paged_cache(vc, kc, HK, int4 ? D / 2 : D, cdt, op)) return rc;
   for (const View* w : {&qo, &kc, &vc})
     if (int rc = distinct(*w, op)) return rc;
+  if (!same_view(qo, q))
+    if (int rc = keep_apart(qo, q, op)) return rc;
+  for (const View* w : {&k, &v})
+    if (int rc = keep_apart(qo, *w, op)) return rc;
   KvAppendArgs a{};
   if (int4) {
     for (View* w : {&ks, &vs}) {
@@ -1813,7 +1858,10 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
         return fail(G950_USAGE, "%s: %s may not be the input it comes from", op, w->name);
       if (int rc = last_contiguous(*w, op)) return rc;
       if (int rc = distinct(*w, op)) return rc;
+      for (const View* in : {&q, &k, &v, &qo})
+        if (int rc = keep_apart(*w, *in, op)) return rc;
     }
+    if (int rc = keep_apart(ko, vo, op)) return rc;
     a.k_out = no_elements(ko) ? nullptr : ko.v->data;
     a.v_out = no_elements(vo) ? nullptr : vo.v->data;
     a.ko_st = ko.stride[0]; a.ko_sh = ko.stride[1]; a.vo_st = vo.stride[0]; a.vo_sh = vo.stride[1];
@@ -2069,6 +2117,15 @@ int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const
     return fail(G950_USAGE, "block_norm: G must have X's shape (strides may be 0) and dtype");
   if (!gate && act && x.shape[0]) return fail(G950_USAGE, "block_norm: gate_act without G");
   if (int rc = distinct(y, "block_norm")) return rc;
+  // elements are read before the thread that writes them does: the same view, or none of it
+  for (const View* w : {&x, &h, &g}) {
+    if (!same_view(y, *w))
+      if (int rc = keep_apart(y, *w, "block_norm")) return rc;
+    if (pre && !same_view(n, *w))
+      if (int rc = keep_apart(n, *w, "block_norm")) return rc;
+  }
+  if (pre)
+    if (int rc = keep_apart(n, y, "block_norm")) return rc;
   BlockNormArgs a{};
   a.x = x.v->data; a.h = h.v->data; a.y = y.v->data;
   a.w_post = post ? wo.v->data : nullptr;

@@ -187,11 +187,13 @@ typedef struct g950_scalar {
  *                      sin tables (R / 2 columns: the first R dims turn, pairs
  *                      (i, i + R / 2) or, interleaved, (2i, 2i + 1)), k and v
  *                      appended to the paged cache; fp32 arithmetic, one rounding.
- *                      q_out_ptr may be q_ptr itself (same strides), else they may
- *                      not overlap.  A token at a position below 0 or past the
+ *                      q_out_ptr may be q_ptr itself (same strides), else it overlaps
+ *                      neither q_ptr nor k_ptr or v_ptr (refused where the views may).
+ *                      A token at a position below 0 or past the
  *                      tables is left out; a key page that the table or the pool
- *                      does not hold drops only its cache row.  Cache rows that two
- *                      tokens of a call name end as either.
+ *                      does not hold drops only its cache row.  A cache row that two
+ *                      tokens of a call name is undefined: a mix of both, in 4 bits also
+ *                      one's codes under the other's scale.
  *   views   cos_ptr[P,R/2], cu_seqlens_q_ptr i32[B+1], k_cache_ptr[pages,
  *           block_size,HK,D], k_ptr[T,HK,D], page_table_ptr i32[B,max_pages],
  *           q_out_ptr[T,H,D], q_ptr[T,H,D] (H may be 0), seqused_k_ptr i32[B],
@@ -207,7 +209,8 @@ typedef struct g950_scalar {
  *                      s = o = NaN.
  *   views   cos_ptr, cu_seqlens_q_ptr, k_cache_ptr u8[pages,block_size,HK,D/2],
  *           k_out_ptr[T,HK,D] or empty (the appended rows as the cache now holds
- *           them, rounded to T; apart from every input), k_ptr,
+ *           them, rounded to T; refused where they may overlap q_ptr, k_ptr, v_ptr,
+ *           q_out_ptr or each other), k_ptr,
  *           k_scale_ptr[pages,block_size,HK,2], page_table_ptr, q_out_ptr, q_ptr,
  *           seqused_k_ptr, sin_ptr, v_cache_ptr, v_out_ptr, v_ptr, v_scale_ptr
  *   scalars interleaved
@@ -230,8 +233,10 @@ typedef struct g950_scalar {
  * G950_OP_BLOCK_NORM   the norms around a block with its gate and residual:
  *                      u = H rsqrt(mean(H^2) + eps) W_post (H itself without W_post),
  *                      Y = residual_scale X + act(G) u, N = Y rsqrt(mean(Y^2) + eps) W_pre
- *                      of Y before its rounding.  Y may be X and N may be H.  C is at
- *                      most 2^31 - 256.
+ *                      of Y before its rounding.  Y and N may each be X, H or G
+ *                      itself (same strides), else they overlap none of them, nor
+ *                      each other (refused where the views may).  C is at most
+ *                      2^31 - 256.
  *   views   G[R,C] (strides may be 0) or empty, H[R,C], N[R,C] (empty without
  *           W_pre), W_post[C] or empty, W_pre[C] or empty, X[R,C], Y[R,C]: one
  *           float dtype
