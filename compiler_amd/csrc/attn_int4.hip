@@ -142,12 +142,14 @@ __device__ __forceinline__ void attn_int4_general_body(const AttnInt4Args& p) {
 //     four rows of a read lie in different LDS banks.
 //   * K's dims are taken in the order in which the words hold them; q's fragments
 //     are laid out to match, once.
-// Measured, in us (32 query heads on 8 KV heads, d 128, bfloat16, pages of 64):
+// Measured, in us (32 query heads on 8 KV heads, d 128, bfloat16, pages of 64), in runs of 23
+// launches after a pause; in a run of thousands what the vector ALU bounds takes a tenth less
+// (the 32 sequences 23.8, the chunks 108.6, 426 TFLOP/s), the rest as long:
 //   64 sequences of 8192 keys  114, 5.0 TB/s (a plain copy: 6.0)
 //   3 of 65537 to 81920        51.7 and 5.2 for joining the parts, 4.7 TB/s
 //   32 of 300 to 4096          25.5 (77 MB; the longest sequences' workgroups end last)
 //   1 of 1000                  11.5: 6.2 with a single key, then 0.6 per tile of a SIMD
-//   2 of 301 to 512 queries behind 3001 to 4096 keys: 120, 385 TFLOP/s; a tile's codes are
+//   2 of 301 to 512 queries behind 3001 to 4096 keys: 120, 386 TFLOP/s; a tile's codes are
 //     unpacked again for every 32 query rows, and 72% of the CUs' time is used (800
 //     workgroups on 512 places)
 // 16 sequences of 4 queries, 8 heads on one KV head, d 64, float16, 511 to 8192 keys: 11.4

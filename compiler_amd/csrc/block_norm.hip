@@ -8,7 +8,7 @@ namespace g950 {
 
 // sigmoid(g) = 1 / (1 + e^-g); tanh(g) = (1 - e^-2|g|) / (1 + e^-2|g|) with g's
 // sign, near 0 (where the difference cancels) the odd series to g^7 (next term
-// 62 / 2835 g^9: below 2e-8 of g for |g| < 0.18)
+// 62 / 2835 g^9: below 2.5e-8 of g for |g| < 0.18)
 __device__ __forceinline__ float gate_act(float g, int act) {
   if (act == 0) return g;
   if (act == 1) return 1.0f / (1.0f + __expf(-g));

@@ -1921,7 +1921,7 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
 // How attention over the 4-bit cache cuts a call: blocks of 16 or 32 query rows per
 // (sequence, KV head), and parts of their keys, whose records need a workspace.  All of it
 // by the greatest lengths alone; the keys of each sequence are cut by its own on the device.
-// Measured at d 128 in bfloat16, 32 query heads on 8 KV heads:
+// Measured at d 128 in bfloat16, 32 query heads on 8 KV heads, in short runs:
 //   * 32 rows share an unpacked key or value where there are more than 16 (two chunks of 301
 //     to 512 queries behind 3001 to 4096 keys: 120 us, 140 with 16 rows); d 256 has no
 //     registers for it.

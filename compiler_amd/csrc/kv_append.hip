@@ -12,12 +12,15 @@
 //
 // 4-bit rows: a (token, head) row x of D dims, after the rotation and before
 // any rounding, is held as
-//   s = T((max - min) / 15), o = T(min + 8 s), c = clamp(rint((x - o) / s) + 8, 0, 15)
+//   s = T((max - min) / 15), o = T(min + 8 s), c = clamp(rint((x - o) (1 / s)) + 8, 0, 15)
 // and stands for (c - 8) s + o; T is the model's type.  Byte i holds dims 2i
 // (low half) and 2i + 1.  A row whose spread rounds to nothing has s = 0 and o = its
 // value; a row that holds NaN or infinities (or whose spread passes fp32) has s = o = NaN.
-// s and o round once, as they are kept, and the codes are taken against the rounded pair:
-// its rounding moves the codes, not the values behind them.
+// s and o round once, as they are kept, and the codes are taken against the rounded pair, so
+// that its rounding moves the codes and the values stay within half a step s; but at the row's
+// ends the codes clamp, and a value is off by up to o's rounding and 15 of s's (2^-8 of each
+// in bfloat16, 2^-11 in float16) where that is more: rows far from 0 beside their
+// spread lose one end.
 //
 // Nothing is written for tokens past cu[B] or of a sequence whose rows are not
 // rows of q; nor, at a position below 0 or past the tables; a page that the
