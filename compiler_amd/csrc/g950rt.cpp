@@ -2009,6 +2009,8 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
   if (int rc = paged_cache(vs, k, HK, 2, dt, op)) return rc;
   if (int rc = distinct(o, op)) return rc;
   if (int rc = distinct(lse, op)) return rc;
+  if (!same_view(o, q))  // (in place: who read a row of q writes that row of o, or the joining launch does)
+    if (int rc = keep_apart(o, q, op)) return rc;
   if (ws.v->dtype != G950_DTYPE_FLOAT32) return fail(G950_USAGE, "%s: workspace_ptr must be float32", op);
   if (int rc = last_contiguous(ws, op)) return rc;
   AttnInt4Args a{};

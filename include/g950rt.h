@@ -219,7 +219,8 @@ typedef struct g950_scalar {
  *                      <= i + seqused_k - n + right (window sizes below 0: no limit; causal:
  *                      right = 0) whose page the pool holds; queries from seqlen_q on are
  *                      left alone; O = 0 and LSE = +inf for a row without keys (and, as
- *                      in G950_OP_FLASH_VARLEN, LSE = +inf where the sum is NaN).  Calls
+ *                      in G950_OP_FLASH_VARLEN, LSE = +inf where the sum is NaN).  O may
+ *                      be Q itself (same strides), else they may not overlap.  Calls
  *                      of more work-items than a launch counts (2^32) are refused
  *   views   cu_seqlens_q_ptr, k_cache_ptr, k_scale_ptr, o_ptr[T,H,D],
  *           page_table_ptr, q_ptr[T,H,D], seqused_k_ptr, softmax_lse_ptr f32[H,T],

@@ -1,4 +1,4 @@
-"""Outputs that lie over inputs: what the paged appends and the norms around a
+"""Outputs that lie over inputs: what the paged operators and the norms around a
 block take and refuse (g950_validate, no device).  Views are numpy views of host
 buffers, which validation compares and never reads."""
 import ctypes
@@ -9,7 +9,8 @@ import pytest
 from compiler_amd import runtime as rt
 
 T, H, HK, D = 7, 8, 2, 64
-OUTS = {"k_cache_ptr", "v_cache_ptr", "q_out_ptr", "k_out_ptr", "v_out_ptr", "k_scale_ptr", "v_scale_ptr", "Y", "N"}
+OUTS = {"k_cache_ptr", "v_cache_ptr", "q_out_ptr", "k_out_ptr", "v_out_ptr", "k_scale_ptr", "v_scale_ptr", "Y", "N",
+        "o_ptr", "softmax_lse_ptr", "workspace_ptr"}
 CODES = {np.dtype(np.uint16): rt.DT_BF16, np.dtype(np.float32): rt.DT_F32, np.dtype(np.int32): rt.DT_INT32,
          np.dtype(np.uint8): rt.DT_UINT8}
 
@@ -95,6 +96,21 @@ def test_append_held_values_over_inputs():
     refused(append(True, **base, k_out_ptr=ko, v_out_ptr=ko), "k_out_ptr overlaps v_out_ptr")
     out = half(T, H, D)
     refused(append(True, **base, q_out_ptr=out, k_out_ptr=out[:, :HK], v_out_ptr=vo), "k_out_ptr overlaps q_out_ptr")
+
+
+def test_attend_over_queries():
+    def attend(q, o):
+        cache, pairs = np.zeros((9, 16, HK, D // 2), np.uint8), half(9, 16, HK, 2)
+        v = {"cu_seqlens_q_ptr": np.zeros(4, np.int32), "seqused_k_ptr": np.zeros(3, np.int32),
+             "page_table_ptr": np.zeros((3, 4), np.int32), "q_ptr": q, "o_ptr": o, "k_cache_ptr": cache,
+             "v_cache_ptr": cache.copy(), "k_scale_ptr": pairs, "v_scale_ptr": pairs.copy(),
+             "softmax_lse_ptr": np.zeros((H, T), np.float32), "workspace_ptr": np.zeros(0, np.float32)}
+        return validate(rt.OP_PAGED_ATTENTION_INT4, v, [True, 0.1, 64, 3, -1, -1])
+    qkv = half(T, 2 * H, D)
+    assert attend(qkv[:, :H], half(T, H, D))[0] == attend(qkv[:, :H], qkv[:, :H])[0] == attend(qkv[:, :H], qkv[:, H:])[0] == 0
+    refused(attend(qkv[:, :H], qkv[:, 1:H + 1]), "o_ptr overlaps q_ptr")
+    rows = half(T + 1, H, D)
+    refused(attend(rows[:T], rows[1:]), "o_ptr overlaps q_ptr")
 
 
 def norm(**views):

@@ -7,6 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import paged_bars as bars  # noqa: E402
+from compiler_amd import operators as ops  # noqa: E402
 from compiler_amd import runtime as rt  # noqa: E402
 from test_gpu_paged_int4 import ATTEND, attend_args, attend_run  # noqa: E402
 
@@ -25,6 +26,18 @@ def test_attend_within_bars(name, dt, aimed):
     for _ in range(2):
         again = attend_run(c, dt, args)
         assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("name", ["blocks_parts", "chunk_d64", "parts_window", "wide_few", "rows33", "d256", "page10"])
+def test_attend_in_the_place_of_its_queries(name):
+    c = bars.case(name, "bfloat16")
+    args = list(attend_args(c, "bfloat16"))
+    args[0][c["cu"][-1]:] = 9.0
+    lse = torch.full((c["h"], c["q"].shape[0]), 9.0, device="cuda")
+    o, _ = ops.paged_attention_int4(*args, scale=c["scale"], causal=c["causal"], window=c["window"], out=args[0], lse=lse,
+                                    sync=True)
+    assert o is args[0]
+    bars.check(bars.attend(c, "bfloat16"), o.double().cpu().numpy(), lse.double().cpu().numpy())
 
 
 @pytest.mark.parametrize("dt", ["bfloat16", "float16"])
