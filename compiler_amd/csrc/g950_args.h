@@ -186,6 +186,74 @@ struct KvAppendArgs {
   int dtype, table_dtype;   // of q / k / v, of cos / sin
   int int4;
   int chunks;               // vector kernel: parts a token's heads are dealt over
+  const int* parent;        // trees: [tokens] each node's parent within its sequence
+};
+
+// Moving a tree's accepted path to its place in the cache (kv_keep.hip).
+struct KvKeepArgs {
+  char* k;                  // [layers, pages, block_size, Hkv, D]
+  char* v;
+  const int* cu;            // [B + 1]
+  const int* used;          // [B]
+  const int* table;         // [B, max_pages]
+  const int* path;          // [B, L]
+  const int* count;         // [B]
+  int* used_out;            // [B]
+  long long k_l, k_p, k_r, k_h, v_l, v_p, v_r, v_h;  // bytes
+  long long table_s, path_z, count_z, out_z;         // elements
+  int T, B, L, Hkv;
+  int pages, block_size, max_pages;
+  int words;                // pieces (of the kernel's word) of a head's row
+  int blocks;               // workgroups of a sequence and layer
+};
+
+// nodes of a drafted tree that attention and verification take at most
+constexpr int TREE_NODES = 1024;
+
+// Attention of drafted trees over a paged cache (attn_tree.hip).
+struct AttnTreeArgs {
+  const void* q;            // [T, Hq, D]
+  void* o;
+  float* lse;               // [Hq, T]
+  const void* k;            // [pages, block_size, Hkv, D]
+  const void* v;
+  const int* cu;            // [B + 1]
+  const int* used;          // [B]
+  const int* table;         // [B, max_pages]
+  const int* parent;        // [T]
+  long long q_st, q_sh, o_st, o_sh, lse_h, lse_t;
+  long long k_p, k_r, k_h, v_p, v_r, v_h;  // elements
+  long long table_s;
+  int T, Hq, Hkv, D, B;
+  int pages, block_size, max_pages;
+  float scale_log2;         // scale * log2(e)
+  int left;                 // window; < 0: unbounded
+  int dtype;
+  int group;                // query heads per KV head
+  int seqlen_q;             // nodes per sequence that take part
+  int row_blocks;           // blocks of rows (node x head of the group) per (sequence, KV head)
+  int splits;               // parts that a block's keys are cut into at most
+  int turn;                 // sequences to move on by from one part to the next
+  int merge_rows;           // rows of a block that any sequence can have
+  float* part;              // [blocks * splits][rows][D] unnormalised O
+  float* ml;                // [blocks * splits][rows][2] maximum (log2 units), sum
+};
+
+// Verification of drafted trees (verify_tree.hip).
+struct VerifyArgs {
+  const void* target;       // [T, V] the target's distribution after each node
+  const void* draft;        // [T, V] what each node's children were drawn from, or null
+  const void* tokens;       // [T] int32 or int64
+  const int* parent;        // [T]
+  const float* u;           // [T]
+  const float* last;        // [B]
+  const int* cu;            // [B + 1]
+  int* path;                // [B, L]
+  int* count;               // [B]
+  void* next;               // [B] like tokens
+  long long t_row, d_row, path_z, count_z, next_z;
+  int T, B, V, L;
+  int token64, distinct;
 };
 
 // Attention over a paged cache of 4-bit rows (attn_int4.hip).

@@ -9,3 +9,6 @@
 #include "kv_append.hip"
 #include "attn_int4.hip"
 #include "block_norm.hip"
+#include "attn_tree.hip"
+#include "kv_keep.hip"
+#include "verify_tree.hip"

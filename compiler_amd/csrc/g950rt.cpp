@@ -1788,13 +1788,20 @@ int paged_cache(const View& c, const View& like, long long heads, long long last
   return last_contiguous(c, op);
 }
 
+// A tree's parents, one per token.
+int tree_list(const View& parent, long long T, const char* op) {
+  if (parent.v->dtype != G950_DTYPE_INT32 || parent.shape[0] != T)
+    return fail(G950_USAGE, "%s: %s must be int32 [tokens]", op, parent.name);
+  return last_contiguous(parent, op);
+}
+
 int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
-                    bool int4, void* stream) {
-  const char* op = int4 ? "paged_append_int4" : "paged_append";
-  if (nviews != (int4 ? 15u : 11u) || nsc != 1)
-    return fail(G950_USAGE, "%s: needs %d views (cos_ptr .. %s) and the scalar interleaved", op, int4 ? 15 : 11,
+                    bool int4, bool tree, void* stream) {
+  const char* op = int4 ? "paged_append_int4" : tree ? "paged_append_tree" : "paged_append";
+  if (nviews != (int4 ? 15u : tree ? 12u : 11u) || nsc != 1)
+    return fail(G950_USAGE, "%s: needs %d views (cos_ptr .. %s) and the scalar interleaved", op, int4 ? 15 : tree ? 12 : 11,
                 int4 ? "v_scale_ptr" : "v_ptr");
-  View cos, cu, kc, ko, k, ks, table, qo, q, used, sin, vc, vo, v, vs;
+  View cos, cu, kc, ko, k, ks, table, parent, qo, q, used, sin, vc, vo, v, vs;
   uint32_t i = 0;
   auto next = [&](const char* name, int nd, View& w, bool out) { return check_view(views, i++, name, nd, w, out); };
   if (int rc = next("cos_ptr", 2, cos, false)) return rc;
@@ -1804,6 +1811,7 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   if (int rc = next("k_ptr", 3, k, false)) return rc;
   if (int4) if (int rc = next("k_scale_ptr", 4, ks, true)) return rc;
   if (int rc = next("page_table_ptr", 2, table, false)) return rc;
+  if (tree) if (int rc = next("parent_ptr", 1, parent, false)) return rc;
   if (int rc = next("q_out_ptr", 3, qo, true)) return rc;
   if (int rc = next("q_ptr", 3, q, false)) return rc;
   if (int rc = next("seqused_k_ptr", 1, used, false)) return rc;
@@ -1835,6 +1843,8 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   if (R > D) return fail(G950_USAGE, "%s: the tables turn %lld dims, rows have %lld", op, R, D);
   if (cos.shape[0] > 0x7FFFFFFF) return fail(G950_USAGE, "%s: extent too large", op);
   if (int rc = paged_lists(cu, used, table, op)) return rc;
+  if (tree)
+    if (int rc = tree_list(parent, T, op)) return rc;
   const uint32_t cdt = int4 ? (uint32_t)G950_DTYPE_UINT8 : dt;
   if (int rc = paged_cache(kc, kc, HK, int4 ? D / 2 : D, cdt, op)) return rc;
   if (int rc = paged_cache(vc, kc, HK, int4 ? D / 2 : D, cdt, op)) return rc;
@@ -1845,6 +1855,16 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
   for (const View* w : {&k, &v})
     if (int rc = keep_apart(qo, *w, op)) return rc;
   KvAppendArgs a{};
+  if (tree) {
+    a.parent = (const int*)parent.v->data;
+    for (const View* out : {&qo, &kc, &vc})
+      for (const View* in : {&cos, &sin, &cu, &used, &table, &parent, &k, &v})
+        if (int rc = keep_apart(*out, *in, op)) return rc;
+    for (const View* w : {&q, &qo, &vc})
+      if (int rc = keep_apart(kc, *w, op)) return rc;
+    for (const View* w : {&q, &qo})
+      if (int rc = keep_apart(vc, *w, op)) return rc;
+  }
   if (int4) {
     for (View* w : {&ks, &vs}) {
       if (int rc = paged_cache(*w, kc, HK, 2, dt, op)) return rc;
@@ -1911,11 +1931,11 @@ int op_paged_append(g950_module* m, const g950_view* views, uint32_t nviews, con
     // (past 2^26 waves the general kernel, whose waves take several rows)
     if (blocks <= max_grid(256)) {
       char name[64];
-      snprintf(name, sizeof name, "g950_kv_append%s_%s_d%lld", int4 ? "_int4" : "", rr_dtype(dt), D);
+      snprintf(name, sizeof name, "g950_kv_append%s_%s_d%lld", int4 ? "_int4" : tree ? "_tree" : "", rr_dtype(dt), D);
       return launch(m, name, (unsigned)blocks, 256u, a, stream);
     }
   }
-  return launch(m, "g950_kv_append_general", (unsigned)std::min((rows + 3) / 4, 1ll << 20), 256u, a, stream);
+  return launch(m, tree ? "g950_kv_append_tree_general" : "g950_kv_append_general", (unsigned)std::min((rows + 3) / 4, 1ll << 20), 256u, a, stream);
 }
 
 // How attention over the 4-bit cache cuts a call: blocks of 16 or 32 query rows per
@@ -2074,6 +2094,201 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
 }
 
 // --------------------------------------------------- norms around a block
+// ------------------------------------------------------------ drafted trees
+constexpr long long kTreeNodes = G950_TREE_NODES;
+static_assert(kTreeNodes == TREE_NODES, "the header's limit is the kernels'");
+
+int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
+                            void* stream) {
+  const char* op = "paged_attention_tree";
+  if (nviews != 10 || nsc != 4)
+    return fail(G950_USAGE, "%s: needs 10 views (cu_seqlens_q_ptr .. workspace_ptr) and 4 scalars", op);
+  View cu, k, o, table, parent, q, used, lse, v, ws;
+  const struct { View* w; const char* name; int nd; bool out; } vw[10] = {
+      {&cu, "cu_seqlens_q_ptr", 1, false}, {&k, "k_cache_ptr", 4, false}, {&o, "o_ptr", 3, true},
+      {&table, "page_table_ptr", 2, false}, {&parent, "parent_ptr", 1, false}, {&q, "q_ptr", 3, false},
+      {&used, "seqused_k_ptr", 1, false}, {&lse, "softmax_lse_ptr", 2, true}, {&v, "v_cache_ptr", 4, false},
+      {&ws, "workspace_ptr", 1, true}};
+  for (uint32_t i = 0; i < 10; ++i)
+    if (int rc = check_view(views, i, vw[i].name, vw[i].nd, *vw[i].w, vw[i].out)) return rc;
+  double scale;
+  long long SK, SQ, left;
+  if (int rc = scalar_float(&sc[0], "scale_softmax", scale)) return rc;
+  if (int rc = scalar_int(&sc[1], "seqlen_k", SK)) return rc;
+  if (int rc = scalar_int(&sc[2], "seqlen_q", SQ)) return rc;
+  if (int rc = scalar_int(&sc[3], "window_size_left", left)) return rc;
+  const uint32_t dt = q.v->dtype;
+  if (!is_float(dt) || o.v->dtype != dt)
+    return fail(G950_USAGE, "%s: q and o must share one dtype (float32, bfloat16, float16)", op);
+  const long long T = q.shape[0], H = q.shape[1], D = q.shape[2], HK = k.shape[2];
+  if (HK < 1 || H < 1 || H % HK) return fail(G950_USAGE, "%s: %lld query heads on %lld KV heads", op, H, HK);
+  if (D < 1 || D > 256) return fail(G950_USAGE, "%s: d must be at most 256", op);
+  if (T > 0x7FFFFFFF || H > 65536) return fail(G950_USAGE, "%s: extent too large", op);
+  if (SQ < 0 || SQ > kTreeNodes) return fail(G950_USAGE, "%s: seqlen_q must be 0 .. %lld", op, kTreeNodes);
+  if (SK < 0 || SK > 0x7FFFFFFF) return fail(G950_USAGE, "%s: seqlen_k out of range", op);
+  if (!std::isfinite(scale)) return fail(G950_USAGE, "%s: scale_softmax must be finite", op);
+  for (int d = 0; d < 3; ++d)
+    if (o.shape[d] != q.shape[d]) return fail(G950_USAGE, "%s: o_ptr must have q's shape", op);
+  if (lse.v->dtype != G950_DTYPE_FLOAT32 || lse.shape[0] != H || lse.shape[1] != T)
+    return fail(G950_USAGE, "%s: softmax_lse_ptr must be float32 [h, tokens]", op);
+  if (int rc = last_contiguous(q, op)) return rc;
+  if (int rc = last_contiguous(o, op)) return rc;
+  if (int rc = paged_lists(cu, used, table, op)) return rc;
+  if (int rc = tree_list(parent, T, op)) return rc;
+  if (int rc = paged_cache(k, k, HK, D, dt, op)) return rc;
+  if (int rc = paged_cache(v, k, HK, D, dt, op)) return rc;
+  if (ws.v->dtype != G950_DTYPE_FLOAT32) return fail(G950_USAGE, "%s: workspace_ptr must be float32", op);
+  if (int rc = last_contiguous(ws, op)) return rc;
+  // (o in place of q: who reads a row of q writes that row of o, or the joining launch does)
+  for (const View* out : {&o, &lse, &ws}) {
+    if (int rc = distinct(*out, op)) return rc;
+    for (const View* w : {&cu, &k, &table, &parent, &q, &used, &v})
+      if (!(out == &o && w == &q && same_view(o, q)))
+        if (int rc = keep_apart(*out, *w, op)) return rc;
+  }
+  if (int rc = keep_apart(o, lse, op)) return rc;
+  for (const View* w : {&o, &lse})
+    if (int rc = keep_apart(ws, *w, op)) return rc;
+  AttnTreeArgs a{};
+  a.q = q.v->data; a.o = o.v->data; a.lse = (float*)lse.v->data; a.k = k.v->data; a.v = v.v->data;
+  a.cu = (const int*)cu.v->data; a.used = (const int*)used.v->data; a.table = (const int*)table.v->data;
+  a.parent = (const int*)parent.v->data;
+  a.q_st = q.stride[0]; a.q_sh = q.stride[1]; a.o_st = o.stride[0]; a.o_sh = o.stride[1];
+  a.lse_h = lse.stride[0]; a.lse_t = lse.stride[1];
+  a.k_p = k.stride[0]; a.k_r = k.stride[1]; a.k_h = k.stride[2];
+  a.v_p = v.stride[0]; a.v_r = v.stride[1]; a.v_h = v.stride[2];
+  a.table_s = table.stride[0];
+  a.T = (int)T; a.Hq = (int)H; a.Hkv = (int)HK; a.D = (int)D; a.B = (int)used.shape[0];
+  a.pages = (int)k.shape[0]; a.block_size = (int)k.shape[1]; a.max_pages = (int)table.shape[1];
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.left = left < 0 ? -1 : (int)std::min(left, 0x7FFFFFFFll);
+  a.dtype = (int)dt; a.group = (int)(H / HK); a.seqlen_q = (int)SQ;
+  const long long rows = a.B && SQ ? T * H : 0;
+  if (rows > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+  return launch(m, "g950_attn_tree_general", (unsigned)rows, 64u, a, stream);
+}
+
+int op_verify_tree(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
+                   void* stream) {
+  const char* op = "verify_tree";
+  if (nviews != 10 || nsc != 1)
+    return fail(G950_USAGE, "%s: needs 10 views (count_ptr .. uniform_ptr) and the scalar distinct", op);
+  View count, cu, draft, next, parent, path, target, tokens, last, u;
+  const struct { View* w; const char* name; int nd; bool out; } vw[10] = {
+      {&count, "count_ptr", 1, true}, {&cu, "cu_seqlens_q_ptr", 1, false}, {&draft, "draft_probs_ptr", 2, false},
+      {&next, "next_ptr", 1, true}, {&parent, "parent_ptr", 1, false}, {&path, "path_ptr", 2, true},
+      {&target, "target_probs_ptr", 2, false}, {&tokens, "tokens_ptr", 1, false},
+      {&last, "uniform_next_ptr", 1, false}, {&u, "uniform_ptr", 1, false}};
+  for (uint32_t i = 0; i < 10; ++i)
+    if (int rc = check_view(views, i, vw[i].name, vw[i].nd, *vw[i].w, vw[i].out)) return rc;
+  long long distinct_;
+  if (int rc = scalar_int(&sc[0], "distinct", distinct_)) return rc;
+  const uint32_t dt = target.v->dtype;
+  if (!is_float(dt)) return fail(G950_USAGE, "%s: target_probs_ptr must be float32, bfloat16 or float16", op);
+  const long long T = target.shape[0], V = target.shape[1], B = count.shape[0], L = path.shape[1];
+  if (V < 1 || V > 0x7FFFFFFF || T > 0x7FFFFFFF || B > 0x7FFFFFF || L > 0x7FFFFFFF)
+    return fail(G950_USAGE, "%s: extent empty or too large", op);
+  if (L < 1) return fail(G950_USAGE, "%s: path_ptr [b, most] needs a place for the root", op);
+  const bool drawn = draft.shape[0] != 0 && draft.shape[1] != 0;
+  if (drawn && (draft.v->dtype != dt || draft.shape[0] != T || draft.shape[1] != V))
+    return fail(G950_USAGE, "%s: draft_probs_ptr must be empty or have target_probs_ptr's shape and dtype", op);
+  const uint32_t tk = tokens.v->dtype;
+  if ((tk != G950_DTYPE_INT32 && tk != G950_DTYPE_INT64) || next.v->dtype != tk)
+    return fail(G950_USAGE, "%s: tokens_ptr and next_ptr must both be int32 or int64", op);
+  if (tokens.shape[0] != T || u.shape[0] != T || u.v->dtype != G950_DTYPE_FLOAT32)
+    return fail(G950_USAGE, "%s: tokens_ptr [tokens], uniform_ptr float32 [tokens] and target_probs_ptr disagree", op);
+  if (int rc = tree_list(parent, T, op)) return rc;
+  if (cu.v->dtype != G950_DTYPE_INT32 || cu.shape[0] != B + 1 || count.v->dtype != G950_DTYPE_INT32 ||
+      path.v->dtype != G950_DTYPE_INT32 || path.shape[0] != B || next.shape[0] != B || last.shape[0] != B ||
+      last.v->dtype != G950_DTYPE_FLOAT32)
+    return fail(G950_USAGE, "%s: count_ptr int32 [b], cu_seqlens_q_ptr int32 [b + 1], path_ptr int32 [b, most], next_ptr [b] "
+                            "and uniform_next_ptr float32 [b] disagree", op);
+  for (const View* w : {&target, &draft, &tokens, &u, &last, &cu, &path})
+    if (int rc = last_contiguous(*w, op)) return rc;
+  for (const View* out : {&count, &next, &path}) {
+    if (int rc = distinct(*out, op)) return rc;
+    for (const View* w : {&cu, &draft, &parent, &target, &tokens, &last, &u, &count, &next, &path})
+      if (out != w)
+        if (int rc = keep_apart(*out, *w, op)) return rc;
+  }
+  VerifyArgs a{};
+  a.target = target.v->data; a.draft = drawn ? draft.v->data : nullptr; a.tokens = tokens.v->data;
+  a.parent = (const int*)parent.v->data; a.u = (const float*)u.v->data; a.last = (const float*)last.v->data;
+  a.cu = (const int*)cu.v->data; a.path = (int*)path.v->data; a.count = (int*)count.v->data; a.next = next.v->data;
+  a.t_row = target.stride[0]; a.d_row = draft.stride[0]; a.path_z = path.stride[0];
+  a.count_z = count.stride[0]; a.next_z = next.stride[0];
+  a.T = (int)T; a.B = (int)B; a.V = (int)V; a.L = (int)L;
+  a.token64 = tk == G950_DTYPE_INT64; a.distinct = distinct_ ? 1 : 0;
+  return launch(m, std::string("g950_verify_tree_") + rr_dtype(dt), (unsigned)B, 1024u, a, stream);
+}
+
+int op_paged_keep_path(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar*, uint32_t nsc,
+                       void* stream) {
+  const char* op = "paged_keep_path";
+  if (nviews != 8 || nsc != 0) return fail(G950_USAGE, "%s: needs 8 views (count_ptr .. v_cache_ptr) and no scalars", op);
+  View count, cu, k, table, path, out, used, v;
+  if (int rc = check_view(views, 0, "count_ptr", 1, count, false)) return rc;
+  if (int rc = check_view(views, 1, "cu_seqlens_q_ptr", 1, cu, false)) return rc;
+  if (int rc = check_view(views, 2, "k_cache_ptr", -1, k, true)) return rc;
+  if (int rc = check_view(views, 3, "page_table_ptr", 2, table, false)) return rc;
+  if (int rc = check_view(views, 4, "path_ptr", 2, path, false)) return rc;
+  if (int rc = check_view(views, 5, "seqused_k_ptr", 1, used, false)) return rc;
+  if (int rc = check_view(views, 6, "seqused_out_ptr", 1, out, true)) return rc;
+  if (int rc = check_view(views, 7, "v_cache_ptr", -1, v, true)) return rc;
+  if (int rc = paged_lists(cu, used, table, op)) return rc;
+  const long long B = used.shape[0], L = path.shape[1];
+  if (path.v->dtype != G950_DTYPE_INT32 || count.v->dtype != G950_DTYPE_INT32 || out.v->dtype != G950_DTYPE_INT32 ||
+      path.shape[0] != B || count.shape[0] != B || out.shape[0] != B || L > 0x7FFFFFFF)
+    return fail(G950_USAGE, "%s: count_ptr, path_ptr [b, most] and seqused_out_ptr must be int32 and agree on b", op);
+  if (int rc = last_contiguous(path, op)) return rc;
+  if ((k.nd != 4 && k.nd != 5) || v.nd != k.nd)
+    return fail(G950_USAGE, "%s: the caches must both be [pages, block_size, hk, d] or [layers, pages, block_size, hk, d]", op);
+  if (!is_float(k.v->dtype) || v.v->dtype != k.v->dtype)
+    return fail(G950_USAGE, "%s: the caches must share one dtype (float32, bfloat16, float16)", op);
+  const int at = k.nd - 4;  // the axis of pages
+  for (int d = 0; d < k.nd; ++d) {
+    if (k.shape[d] != v.shape[d]) return fail(G950_USAGE, "%s: the caches differ in shape", op);
+    if (k.shape[d] > (d < at ? 65536 : 0x7FFFFFFF)) return fail(G950_USAGE, "%s: extent too large", op);
+  }
+  const long long layers = at ? k.shape[0] : 1, HK = k.shape[at + 2], D = k.shape[at + 3];
+  if (HK < 1 || D < 1 || HK > 65536 || D > 65536) return fail(G950_USAGE, "%s: extent empty or too large", op);
+  if (k.shape[at + 1] < 1) return fail(G950_USAGE, "%s: pages of no keys", op);
+  for (const View* w : {&k, &v}) {
+    if (int rc = last_contiguous(*w, op)) return rc;
+    if (int rc = distinct(*w, op)) return rc;
+    for (const View* in : {&count, &cu, &table, &path, &used, &out})
+      if (int rc = keep_apart(*w, *in, op)) return rc;
+  }
+  if (int rc = keep_apart(k, v, op)) return rc;
+  if (int rc = distinct(out, op)) return rc;
+  for (const View* in : {&count, &cu, &table, &path, &used})
+    if (int rc = keep_apart(out, *in, op)) return rc;
+  KvKeepArgs a{};
+  a.k = (char*)k.v->data; a.v = (char*)v.v->data;
+  a.cu = (const int*)cu.v->data; a.used = (const int*)used.v->data; a.table = (const int*)table.v->data;
+  a.path = (const int*)path.v->data; a.count = (const int*)count.v->data; a.used_out = (int*)out.v->data;
+  // (an axis of one element is not stepped along, whatever its stride)
+  auto step = [](const View& w, int d) { return w.shape[d] > 1 ? (long long)w.stride[d] * w.isz : 0; };
+  a.k_l = at ? step(k, 0) : 0; a.k_p = step(k, at); a.k_r = step(k, at + 1); a.k_h = step(k, at + 2);
+  a.v_l = at ? step(v, 0) : 0; a.v_p = step(v, at); a.v_r = step(v, at + 1); a.v_h = step(v, at + 2);
+  a.table_s = table.stride[0]; a.path_z = path.stride[0]; a.count_z = count.stride[0]; a.out_z = out.stride[0];
+  a.T = 0x7FFFFFFF; a.B = (int)B; a.L = (int)L; a.Hkv = (int)HK;
+  a.pages = (int)k.shape[at]; a.block_size = (int)k.shape[at + 1]; a.max_pages = (int)table.shape[1];
+  // the widest word that every head's row is made of
+  int word = k.isz;
+  for (int w : {4, 16}) {
+    bool fits = D * k.isz % w == 0;
+    for (const View* c : {&k, &v})
+      for (int d = -1; d < c->nd - 1; ++d) fits = fits && (d < 0 ? (long long)(c->addr() % w) : step(*c, d) % w) == 0;
+    if (fits) word = w;
+  }
+  const long long words = D * k.isz / word, blocks = (2 * HK * words + 255) / 256;
+  if (2 * HK * words > 0x7FFFFF00 || B * blocks * layers > (long long)max_grid(256))
+    return fail(G950_USAGE, "%s: grid too large", op);
+  a.words = (int)words; a.blocks = (int)blocks;
+  return launch(m, "g950_kv_keep_w" + std::to_string(word), (unsigned)(B * blocks * layers), 256u, a, stream);
+}
+
 int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
                   void* stream) {
   if (nviews != 7 || nsc != 3)
@@ -2248,11 +2463,16 @@ int dispatch(g950_module* m, uint32_t op, const g950_view* views, uint32_t nview
       case G950_OP_SOFTMAX_INNER: return op_softmax_inner(m, views, nviews, scalars, nscalars, stream);
       case G950_OP_LAYERNORM_ROW: return op_layernorm_row(m, views, nviews, scalars, nscalars, stream);
       case G950_OP_GQA: return op_gqa(m, views, nviews, scalars, nscalars, stream);
-      case G950_OP_PAGED_APPEND: return op_paged_append(m, views, nviews, scalars, nscalars, false, stream);
-      case G950_OP_PAGED_APPEND_INT4: return op_paged_append(m, views, nviews, scalars, nscalars, true, stream);
+      case G950_OP_PAGED_APPEND: return op_paged_append(m, views, nviews, scalars, nscalars, false, false, stream);
+      case G950_OP_PAGED_APPEND_INT4: return op_paged_append(m, views, nviews, scalars, nscalars, true, false, stream);
       case G950_OP_PAGED_ATTENTION_INT4:
         return op_paged_attention_int4(m, views, nviews, scalars, nscalars, stream);
       case G950_OP_BLOCK_NORM: return op_block_norm(m, views, nviews, scalars, nscalars, stream);
+      case G950_OP_PAGED_APPEND_TREE: return op_paged_append(m, views, nviews, scalars, nscalars, false, true, stream);
+      case G950_OP_PAGED_ATTENTION_TREE:
+        return op_paged_attention_tree(m, views, nviews, scalars, nscalars, stream);
+      case G950_OP_VERIFY_TREE: return op_verify_tree(m, views, nviews, scalars, nscalars, stream);
+      case G950_OP_PAGED_KEEP_PATH: return op_paged_keep_path(m, views, nviews, scalars, nscalars, stream);
       default: return fail(G950_USAGE, "g950_launch: unknown operator contract %u", op);
     }
   } catch (...) {
@@ -2309,6 +2529,10 @@ size_t g950_paged_attention_int4_workspace(g950_module* m, int64_t b, int64_t h,
   if ((double)b * (double)h * (double)seqlen_q > 0x1p47) return 0;
   const Int4Shape f = int4_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
   return f.splits > 1 ? (size_t)(f.blocks * f.rows * f.splits * (d + 2)) * 4 : 0;
+}
+
+size_t g950_paged_attention_tree_workspace(g950_module*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) {
+  return 0;
 }
 
 int g950_sync(void* stream) {

@@ -22,6 +22,10 @@
 // in bfloat16, 2^-11 in float16) where that is more: rows far from 0 beside their
 // spread lose one end.
 //
+// Trees of drafted tokens (TREE): node i of a sequence has a parent among the nodes before
+// it, or none (any other value); it goes to the cache row of position used - n + i, n the
+// sequence's nodes, and stands at position used - n + depth, where the rotation is concerned.
+//
 // Nothing is written for tokens past cu[B] or of a sequence whose rows are not
 // rows of q; nor, at a position below 0 or past the tables; a page that the
 // table or the pool does not hold drops only the cache row.
@@ -58,6 +62,25 @@ __device__ __forceinline__ int kv_sequence(const int* cu, int B, int T, int t, i
   return b0 >= 0 && t >= b0 && t < b1 && b1 <= T ? b : -1;
 }
 
+// Levels above node i of the tree whose parents begin at `parent`: the way to its root
+// through 64 parents at a time, one per lane (a node's parent lies below it; all
+// arguments are wave-uniform).
+__device__ __forceinline__ int kv_depth(const int* parent, int i) {
+  const int lane = threadIdx.x & 63;
+  int depth = 0, from = i + 1, up = 0;
+  for (;;) {
+    if (i < from) {
+      from = max(i - 63, 0);
+      up = parent[min(from + lane, i)];
+    }
+    const int p = __builtin_amdgcn_readlane(up, i - from);
+    if (p < 0 || p >= i) return depth;
+    ++depth;
+    i = p;
+  }
+}
+
+template <bool TREE>
 __device__ __forceinline__ KvPlace kv_place(const KvAppendArgs& a, int t) {
   KvPlace w;
   w.pos = w.row = 0;
@@ -65,14 +88,19 @@ __device__ __forceinline__ KvPlace kv_place(const KvAppendArgs& a, int t) {
   int b0 = 0, b1 = 0;
   w.seq = __builtin_amdgcn_readfirstlane(kv_sequence(a.cu, a.B, a.T, t, b0, b1));
   if (w.seq < 0) return w;
-  const long long pos = (long long)a.used[w.seq] - (b1 - b0) + (t - b0);
+  long long pos = (long long)a.used[w.seq] - (b1 - b0) + (t - b0);
+  const int slot = __builtin_amdgcn_readfirstlane((int)pos);
+  if constexpr (TREE) {
+    b0 = __builtin_amdgcn_readfirstlane(b0);
+    pos += kv_depth(a.parent + b0, t - b0) - (t - b0);
+  }
   if (pos < 0 || (a.R && pos >= a.positions)) {
     w.seq = -1;
     return w;
   }
   w.pos = __builtin_amdgcn_readfirstlane((int)pos);
-  const int e = w.pos / a.block_size;
-  w.row = w.pos % a.block_size;
+  const int e = slot / a.block_size;
+  w.row = slot % a.block_size;
   if (e < a.max_pages) {
     const int ph = a.table[(long long)w.seq * a.table_s + e];
     w.page = ph >= 0 && ph < a.pages ? ph : -1;
@@ -131,6 +159,7 @@ __device__ __forceinline__ float kv_value(int c, const KvScale& k) {
 // One wave per (token, head) row: any D, R, stride and alignment.  Each row looks its
 // place up and each element reads its own cos and sin: 988 us where the vector kernel
 // takes 103 (26 thousand tokens, below), 489 against 44 into 4 bits.
+template <bool TREE>
 __device__ __forceinline__ void kv_append_general_body(const KvAppendArgs& a) {
   const int lane = threadIdx.x & 63;
   const int slots = a.Hq + 2 * a.Hkv;
@@ -139,7 +168,7 @@ __device__ __forceinline__ void kv_append_general_body(const KvAppendArgs& a) {
   for (long long task = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); task < tasks; task += (long long)gridDim.x * 4) {
     const int t = __builtin_amdgcn_readfirstlane((int)(task / slots));
     const int slot = __builtin_amdgcn_readfirstlane((int)(task % slots));
-    const KvPlace w = kv_place(a, t);
+    const KvPlace w = kv_place<TREE>(a, t);
     if (w.seq < 0) continue;
     const bool is_q = slot < a.Hq, is_v = slot >= a.Hq + a.Hkv;
     const int h = is_q ? slot : is_v ? slot - a.Hq - a.Hkv : slot - a.Hq;
@@ -274,7 +303,7 @@ __device__ __forceinline__ float kv_row(float v) {
   return v;
 }
 
-template <typename T, int L, bool INT4>
+template <typename T, int L, bool INT4, bool TREE>
 __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
   constexpr int D = 16 * L, RPW = 64 / L, SZ = (int)sizeof(T);
   constexpr int DT = SZ == 4 ? DT_F32 : std::is_same_v<T, bf16_t> ? DT_BF16 : DT_F16;
@@ -298,7 +327,7 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
   };
   float x[2][8];
   load(chunk, x);
-  const KvPlace at = kv_place(a, t);
+  const KvPlace at = kv_place<TREE>(a, t);
   if (at.seq < 0) return;
   float c[8] = {}, s[8] = {};
   if (turns) {
@@ -415,16 +444,23 @@ __device__ __forceinline__ void kv_append_body(const KvAppendArgs& a) {
 }  // namespace g950
 
 extern "C" __global__ __launch_bounds__(256) void g950_kv_append_general(const g950::KvAppendArgs a) {
-  g950::kv_append_general_body(a);
+  g950::kv_append_general_body<false>(a);
+}
+extern "C" __global__ __launch_bounds__(256) void g950_kv_append_tree_general(const g950::KvAppendArgs a) {
+  g950::kv_append_general_body<true>(a);
 }
 
 #define G950_KV(TNAME, T, D)                                                                             \
   extern "C" __global__ __launch_bounds__(256) void g950_kv_append_##TNAME##_d##D(const g950::KvAppendArgs a) { \
-    g950::kv_append_body<T, D / 16, false>(a);                                                           \
+    g950::kv_append_body<T, D / 16, false, false>(a);                                                    \
+  }
+#define G950_KVT(TNAME, T, D)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256) void g950_kv_append_tree_##TNAME##_d##D(const g950::KvAppendArgs a) { \
+    g950::kv_append_body<T, D / 16, false, true>(a);                                                          \
   }
 #define G950_KV4(TNAME, T, D)                                                                                 \
   extern "C" __global__ __launch_bounds__(256) void g950_kv_append_int4_##TNAME##_d##D(const g950::KvAppendArgs a) { \
-    g950::kv_append_body<T, D / 16, true>(a);                                                                 \
+    g950::kv_append_body<T, D / 16, true, false>(a);                                                          \
   }
 #define G950_KV_SET(M, TNAME, T) \
   M(TNAME, T, 32)                \
@@ -436,3 +472,6 @@ G950_KV_SET(G950_KV, bf16, g950::bf16_t)
 G950_KV_SET(G950_KV, f16, g950::f16_t)
 G950_KV_SET(G950_KV4, bf16, g950::bf16_t)
 G950_KV_SET(G950_KV4, f16, g950::f16_t)
+G950_KV_SET(G950_KVT, f32, float)
+G950_KV_SET(G950_KVT, bf16, g950::bf16_t)
+G950_KV_SET(G950_KVT, f16, g950::f16_t)

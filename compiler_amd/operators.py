@@ -306,6 +306,62 @@ def block_norm_kernel(X, H, W_post, G, W_pre, Y, N, eps, gate_act, residual_scal
                           prepare)
 
 
+def paged_append_tree_kernel(q_ptr, k_ptr, v_ptr, cos_ptr, sin_ptr, q_out_ptr, k_cache_ptr, v_cache_ptr, page_table_ptr,
+                             cu_seqlens_q_ptr, seqused_k_ptr, parent_ptr, interleaved, *, stream=None, sync=False,
+                             prepare=False):
+    """paged_append_kernel for drafted trees (G950_OP_PAGED_APPEND_TREE; no
+    reference counterpart): a sequence's tokens are the nodes of a tree, parent
+    int32 [tokens] their parents within the sequence (below their own index; else
+    none).  Node i goes to the cache row of position base + i and turns as position base + its
+    depth, base = seqused_k - nodes."""
+    return _launch_sorted(rt.OP_PAGED_APPEND_TREE,
+                          (cos_ptr, cu_seqlens_q_ptr, k_cache_ptr, k_ptr, page_table_ptr, parent_ptr, q_out_ptr, q_ptr,
+                           seqused_k_ptr, sin_ptr, v_cache_ptr, v_ptr),
+                          (False, False, True, False, False, False, True, False, False, False, True, False),
+                          (interleaved,), stream, sync, prepare)
+
+
+def paged_attention_tree_kernel(q_ptr, k_cache_ptr, v_cache_ptr, page_table_ptr, cu_seqlens_q_ptr, seqused_k_ptr,
+                                parent_ptr, o_ptr, softmax_lse_ptr, workspace_ptr, seqlen_q, seqlen_k, scale_softmax,
+                                window_size_left, *, stream=None, sync=False, prepare=False):
+    """Attention of drafted trees over a paged cache (G950_OP_PAGED_ATTENTION_TREE;
+    no reference counterpart): q/o [tokens, h, d], lse float32 [h, tokens], the cache
+    [pages, block_size, hk, d] and its lists as paged_append_tree_kernel fills them.
+    A node sees the keys before the tree, its own and those above it."""
+    return _launch_sorted(rt.OP_PAGED_ATTENTION_TREE,
+                          (cu_seqlens_q_ptr, k_cache_ptr, o_ptr, page_table_ptr, parent_ptr, q_ptr, seqused_k_ptr,
+                           softmax_lse_ptr, v_cache_ptr, workspace_ptr),
+                          (False, False, True, False, False, False, False, True, False, True),
+                          (scale_softmax, seqlen_k, seqlen_q, window_size_left), stream, sync, prepare)
+
+
+def verify_tree_kernel(target_probs_ptr, draft_probs_ptr, tokens_ptr, parent_ptr, uniform_ptr, uniform_next_ptr,
+                       cu_seqlens_q_ptr, path_ptr, count_ptr, next_ptr, distinct, *, stream=None, sync=False,
+                       prepare=False):
+    """Drafted trees verified against the target's probabilities
+    (G950_OP_VERIFY_TREE; no reference counterpart): probabilities [tokens, v]
+    after each node (draft: those that its children were drawn from, or empty), tokens and
+    parent [tokens], uniform float32 [tokens] and [b]; path int32 [b, most], count int32
+    [b] and the next token [b] come out."""
+    return _launch_sorted(rt.OP_VERIFY_TREE,
+                          (count_ptr, cu_seqlens_q_ptr, draft_probs_ptr, next_ptr, parent_ptr, path_ptr, target_probs_ptr,
+                           tokens_ptr, uniform_next_ptr, uniform_ptr),
+                          (True, False, False, True, False, True, False, False, False, False), (distinct,), stream, sync,
+                          prepare)
+
+
+def paged_keep_path_kernel(k_cache_ptr, v_cache_ptr, page_table_ptr, cu_seqlens_q_ptr, seqused_k_ptr, path_ptr, count_ptr,
+                           seqused_out_ptr, *, stream=None, sync=False, prepare=False):
+    """An accepted path's cache rows moved behind the keys before the tree
+    (G950_OP_PAGED_KEEP_PATH; no reference counterpart): row base + i gets row base +
+    path[b, i], i < count[b]; caches [pages, block_size, hk, d] or with the layers in
+    front; seqused_out int32 [b] is base + count."""
+    return _launch_sorted(rt.OP_PAGED_KEEP_PATH,
+                          (count_ptr, cu_seqlens_q_ptr, k_cache_ptr, page_table_ptr, path_ptr, seqused_k_ptr,
+                           seqused_out_ptr, v_cache_ptr), (False, False, True, False, False, False, True, True), (), stream,
+                          sync, prepare)
+
+
 def stream_copy(x, y, *, stream=None, sync=False, prepare=False):
     """y = x through the streaming-copy kernel (nontemporal 16-byte loads and
     stores, the row kernels' memory path); used to calibrate HBM counters."""
@@ -509,6 +565,79 @@ def paged_attention_int4(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_s
                                 workspace, seqlen_q, seqlen_k, 1.0 / math.sqrt(d) if scale is None else float(scale),
                                 bool(causal), int(window[0]), int(window[1]), **kw)
     return o, lse
+
+
+def paged_append_tree(q, k, v, cos, sin, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, parent,
+                      interleaved=False, out=None, **kw):
+    """paged_append for drafted trees: ``parent`` holds each token's parent within its
+    sequence.  See paged_append_tree_kernel."""
+    import torch
+    stream = kw.get("stream")
+    empty_like = torch.empty_like if stream is None else _on_stream(stream, torch.empty_like)
+    q = k.new_empty((k.shape[0], 0, k.shape[2])) if q is None else q
+    out = empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    paged_append_tree_kernel(q, k, v, cos, sin, out, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, parent,
+                             bool(interleaved), **kw)
+    return out
+
+
+def paged_attention_tree(q, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, parent, seqlen_q, seqlen_k, scale=None,
+                         window_left=-1, out=None, lse=None, workspace=None, **kw):
+    """Attention of drafted trees over a paged cache; seqlen_q is the most nodes (up
+    to 1024), seqlen_k the most keys of a sequence.  Returns o and lse [h,
+    tokens].  The workspace (float32) comes from torch's allocator, on the
+    call's stream, unless given."""
+    import torch
+    t, h, d = q.shape
+    seqlen_q, seqlen_k = int(seqlen_q), int(seqlen_k)
+    stream = kw.get("stream")
+    if out is None:
+        o = (torch.empty_like if stream is None else _on_stream(stream, torch.empty_like))(
+            q, memory_format=torch.contiguous_format)
+    else:
+        o = out
+    if lse is None:
+        lse = (torch.empty if stream is None else _on_stream(stream, torch.empty))(
+            (h, t), dtype=torch.float32, device=q.device)
+    if workspace is None:
+        floats = 0
+        if q.dtype != torch.float32:
+            floats = rt.module().attention_tree_workspace(cu_seqlens_q.shape[0] - 1, h, k_cache.shape[2], d,
+                                                          min(seqlen_q, t), seqlen_k)
+        workspace = _workspace(floats, q, stream)
+    paged_attention_tree_kernel(q, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, parent, o, lse, workspace,
+                                seqlen_q, seqlen_k, 1.0 / math.sqrt(d) if scale is None else float(scale),
+                                int(window_left), **kw)
+    return o, lse
+
+
+def verify_tree(target_probs, draft_probs, tokens, parent, uniform, uniform_next, cu_seqlens_q, most, distinct=False,
+                path=None, count=None, next_token=None, **kw):
+    """Drafted trees verified (verify_tree_kernel); draft_probs None: the drafts were
+    chosen, not drawn; ``distinct``: siblings were drawn without replacement.  Returns
+    path [b, most] (the accepted nodes, root first, then -1), count [b] and the
+    next token [b]."""
+    import torch
+    b, stream = cu_seqlens_q.shape[0] - 1, kw.get("stream")
+    empty = torch.empty if stream is None else _on_stream(stream, torch.empty)
+    path = empty((b, int(most)), dtype=torch.int32, device=tokens.device) if path is None else path
+    count = empty((b,), dtype=torch.int32, device=tokens.device) if count is None else count
+    next_token = empty((b,), dtype=tokens.dtype, device=tokens.device) if next_token is None else next_token
+    draft = _none(target_probs.dtype, target_probs.device, 2) if draft_probs is None else draft_probs
+    verify_tree_kernel(target_probs, draft, tokens, parent, uniform, uniform_next, cu_seqlens_q, path, count, next_token,
+                       bool(distinct), **kw)
+    return path, count, next_token
+
+
+def paged_keep_path(k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, path, count, out=None, **kw):
+    """Moves the accepted paths' cache rows (paged_keep_path_kernel) and returns the
+    keys that each sequence has now [b]."""
+    import torch
+    stream = kw.get("stream")
+    empty_like = torch.empty_like if stream is None else _on_stream(stream, torch.empty_like)
+    out = empty_like(seqused_k) if out is None else out
+    paged_keep_path_kernel(k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, path, count, out, **kw)
+    return out
 
 
 _GATE_ACTS = {None: 0, "none": 0, "sigmoid": 1, "tanh": 2}

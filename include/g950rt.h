@@ -242,6 +242,68 @@ typedef struct g950_scalar {
  *           W_pre), W_post[C] or empty, W_pre[C] or empty, X[R,C], Y[R,C]: one
  *           float dtype
  *   scalars eps, gate_act (0 none, 1 sigmoid, 2 tanh), residual_scale
+ *
+ * Trees of drafted tokens over the 16-bit (or fp32) paged cache: the tokens of
+ * sequence b, above, are the n nodes of a tree; parent_ptr i32[T] holds each node's
+ * parent as an index among its sequence's nodes, less than its own; any other
+ * value: none (a root).  With base = seqused_k[b] - n keys before them, node i's key lies in cache
+ * row base + i and stands at position base + depth(i), a root's depth being 0.  One
+ * node is the ordinary token; a chain (parent i - 1) ordinary drafts.
+ *
+ * G950_OP_PAGED_APPEND_TREE  G950_OP_PAGED_APPEND with these rows and positions.
+ *                      Outputs overlap no input but q_out_ptr q_ptr (same strides)
+ *   views   cos_ptr, cu_seqlens_q_ptr, k_cache_ptr, k_ptr, page_table_ptr, parent_ptr,
+ *           q_out_ptr, q_ptr, seqused_k_ptr, sin_ptr, v_cache_ptr, v_ptr
+ *   scalars interleaved
+ * G950_OP_PAGED_ATTENTION_TREE  attention of the nodes (GQA): node i sees the keys
+ *                      before the tree, its own and those of the nodes above it, whose
+ *                      page the pool holds; with window_size_left >= 0 those of them at
+ *                      positions from base + depth(i) - window_size_left on.  What a node does
+ *                      not see may hold anything, NaN included.  Nodes from seqlen_q (at
+ *                      most G950_TREE_NODES) on are left alone; O = 0 and LSE =
+ *                      +inf for a node without keys (LSE = +inf where the sum is NaN).
+ *                      O may be Q itself (same strides); else outputs overlap nothing
+ *   views   cu_seqlens_q_ptr, k_cache_ptr[pages,block_size,HK,D], o_ptr[T,H,D],
+ *           page_table_ptr, parent_ptr, q_ptr[T,H,D], seqused_k_ptr, softmax_lse_ptr
+ *           f32[H,T], v_cache_ptr, workspace_ptr f32 (as in
+ *           G950_OP_PAGED_ATTENTION_INT4, of g950_paged_attention_tree_workspace bytes):
+ *           f32 | bf16 | f16 (same), D at most 256
+ *   scalars scale_softmax, seqlen_k (about the longest sequence's keys: shapes the
+ *           key ranges only), seqlen_q, window_size_left
+ * G950_OP_VERIFY_TREE  the drafts of each tree accepted or refused, so that what is
+ *                      kept is distributed as the target's own tokens.  Row t of
+ *                      target_probs_ptr is its distribution p after node t, of draft_probs_ptr
+ *                      the q that node t's children were drawn from (independently; with
+ *                      `distinct` siblings without replacement).  From node 0 on, of the node
+ *                      reached the children are tested in order: with A = 0, S = Q = 1
+ *                      at first (rows count as normalised), child x with its u = uniform_ptr in
+ *                      [0, 1) is the next node if u q(x) S < max(p(x) - A q(x), 0) Q;
+ *                      else A += S / Q, S = sum_v max(p(v) - A q(v), 0) and, with
+ *                      `distinct`, Q = max(Q - q(x), 2^-24).  draft_probs_ptr empty:
+ *                      children were chosen, not drawn (q = 1 at x): u S < p(x), else S -= p(x) and
+ *                      x is out.  The next token is the first v whose sum of what is left of p
+ *                      (max(p - A q, 0); p without the tokens that are out) passes
+ *                      uniform_next_ptr[b] times the whole; where nothing is left,
+ *                      p's.  Sums are held in 64 bits; entries below 0 and NaN count as 0,
+ *                      tokens outside 0 .. V - 1 have probability 0 (and are refused).  Nodes from
+ *                      G950_TREE_NODES on are not looked at; a path that fills its row of
+ *                      path_ptr ends there.  Outputs overlap nothing
+ *   views   count_ptr i32[B] (nodes of the path), cu_seqlens_q_ptr i32[B+1],
+ *           draft_probs_ptr[T,V] or empty, next_ptr[B], parent_ptr i32[T], path_ptr
+ *           i32[B,most] (the path's nodes, root first, then -1), target_probs_ptr[T,V]
+ *           f32 | bf16 | f16 (draft the same), tokens_ptr[T] i32 | i64 (next the same),
+ *           uniform_next_ptr f32[B], uniform_ptr f32[T].  A sequence without nodes: count 0,
+ *           path and next -1
+ *   scalars distinct
+ * G950_OP_PAGED_KEEP_PATH  the path's rows moved to where its tokens belong: cache row base
+ *                      + i gets what row base + path[b,i] held, for i < count[b] and i <=
+ *                      path[b,i] < n, pages the pool holds (a path that increases is such
+ *                      a one); all others are left alone.  Outputs overlap nothing
+ *   views   count_ptr i32[B], cu_seqlens_q_ptr, k_cache_ptr[pages,block_size,HK,D] or
+ *           [layers,pages,block_size,HK,D] (all layers at once), page_table_ptr, path_ptr
+ *           i32[B,most], seqused_k_ptr, seqused_out_ptr i32[B] (base + count: the
+ *           keys that are left), v_cache_ptr: f32 | bf16 | f16
+ *   scalars none
  */
 enum g950_op {
   G950_OP_SOFTMAX = 1,
@@ -263,8 +325,16 @@ enum g950_op {
   G950_OP_PAGED_APPEND = 17,
   G950_OP_PAGED_APPEND_INT4 = 18,
   G950_OP_PAGED_ATTENTION_INT4 = 19,
-  G950_OP_BLOCK_NORM = 20
+  G950_OP_BLOCK_NORM = 20,
+  G950_OP_PAGED_APPEND_TREE = 21,
+  G950_OP_PAGED_ATTENTION_TREE = 22,
+  G950_OP_VERIFY_TREE = 23,
+  G950_OP_PAGED_KEEP_PATH = 24
 };
+
+/* Nodes of one drafted tree that G950_OP_PAGED_ATTENTION_TREE (seqlen_q) and
+ * G950_OP_VERIFY_TREE take at most. */
+#define G950_TREE_NODES 1024
 
 typedef struct g950_module g950_module;
 
@@ -319,6 +389,11 @@ size_t g950_workspace_bytes(g950_module *module, void *stream);
  * outputs: calls that may overlap (streams, graphs) need one each.  `module`
  * (for the device's size) may be NULL. */
 size_t g950_paged_attention_int4_workspace(g950_module *module, int64_t b, int64_t h, int64_t hk, int64_t d,
+                                           int64_t seqlen_q, int64_t seqlen_k);
+
+/* The same for G950_OP_PAGED_ATTENTION_TREE: b trees of at most seqlen_q nodes over
+ * seqlen_k keys. */
+size_t g950_paged_attention_tree_workspace(g950_module *module, int64_t b, int64_t h, int64_t hk, int64_t d,
                                            int64_t seqlen_q, int64_t seqlen_k);
 
 /* Run every contract check and the kernel choice of g950_launch without
