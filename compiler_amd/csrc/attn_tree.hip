@@ -11,7 +11,7 @@ namespace g950 {
 
 struct TreeSeq {
   int q0, n, nq;  // first row, nodes, those of them that take part
-  int base;       // keys before the tree; -n: none of the sequence's keys exist
+  int base;       // keys before the tree; below 0: the first nodes have no cache row
 };
 __device__ __forceinline__ TreeSeq tree_seq(const int* cu, const int* used, int T, int most, int z) {
   TreeSeq s;
@@ -19,7 +19,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const int* cu, const int* used, int 
   s.q0 = b0;
   s.n = b0 >= 0 && b1 >= b0 && b1 <= T ? b1 - b0 : 0;
   s.nq = min(s.n, most);
-  s.base = max(used[z], 0) - s.n;
+  s.base = max(max(used[z], 0) - s.n, -(1 << 20));  // (no node that takes part has a key below that)
   return s;
 }
 // a node's parent, -1 if it has none
@@ -123,8 +123,502 @@ __device__ __forceinline__ void attn_tree_general_body(const AttnTreeArgs& p) {
         empty ? __builtin_huge_valf() : (m + __log2f(l)) * 0.69314718055994530942f;
 }
 
+// ---------------------------------------------------------------- fast form
+// bfloat16 and float16, d 64, 128 or 256, pages of whole 16-key runs, 16-byte rows.  A row is
+// (node, head of the group).  A workgroup owns one (sequence, KV head, block of 32 RW
+// rows, key range); its 4 waves are RW blocks of 32 rows times KW = 4 / RW shares of the
+// keys, so that K and V are read once for all rows of a block, whatever their number.
+//   * S^T = K.Q^T on v_mfma_f32_32x32x16: a lane holds 16 of 32 keys' scores of ONE row, so
+//     the softmax's running maximum and sum are per lane (two lanes a row).  Its keys 4 g .. + 3
+//     and 8 + 4 g .. + 3 of every 16 are the contraction slots that its own probabilities
+//     feed in O^T = V^T.P^T; V^T's fragments of the same keys come from transposing LDS reads.
+//   * K and V come by direct global->LDS DMA into a ring of stages, TKS keys each, issued NS
+//     stages ahead.  16-byte pieces are swizzled on the way (the source address is the
+//     lane's): K's by the key, so that the 16 keys of a read lie in all 64 banks, V's
+//     by 64 bytes, so that the four keys of a transposing read do.
+//   * Stages are taken from the last to the first: the tree's keys come first, and a lane
+//     meets the nodes above its own one as it walks to the root, parents from LDS;
+//     each 32-key tile of the tree costs it a word of visible keys.  Tiles that every row
+//     sees whole (all but a few) skip that.
+//   * What a row does not see may hold anything: scores are replaced, and where V of a
+//     masked tile is not finite, 0 V would not be 0; such a tile's V is taken apart into
+//     its finite values and the signs of its infinities (NaN: both), which are joined where
+//     a row sees them.
+struct TreeSpan {
+  TreeSeq sq;
+  int kend;     // keys past the last that can be seen
+  int kbeg, n;  // tiles of 64 keys from kbeg on; 0 where no node takes part, else at least 1
+};
+__device__ __forceinline__ TreeSpan tree_span(const AttnTreeArgs& p, int z) {
+  TreeSpan s;
+  s.sq = tree_seq(p.cu, p.used, p.T, p.seqlen_q, z);
+  const long long held = p.pages > 0 ? (long long)p.max_pages * p.block_size : 0;
+  s.kend = (int)min((long long)max(s.sq.base + s.sq.nq, 0), held);
+  s.kbeg = p.left < 0 ? 0 : max(0ll, (long long)s.sq.base - p.left) / 64 * 64;
+  s.n = s.sq.nq > 0 ? max(1, (s.kend - s.kbeg + 63) / 64) : 0;
+  return s;
+}
+
+// What a workgroup does: tiles t0 .. t1 - 1 of a block of rows of a (sequence, KV head); rec:
+// where its partial rows go, -1 if it has all the tiles.  A sequence's tiles are cut into at most
+// `splits` parts of at least 4 by its own length; the sequence moves on with the part, so
+// that workgroups sharing a CU differ in length where the batch does.
+struct TreePart {
+  int z, hk, block, t0, t1, rec;
+};
+__device__ __forceinline__ int tree_part(const AttnTreeArgs& p, int n) {
+  return max((int)((uint32_t)(n + p.splits - 1) / (uint32_t)p.splits), 4);
+}
+__device__ __forceinline__ TreePart tree_deal(const AttnTreeArgs& p, TreeSpan& sp) {
+  const uint32_t heads = p.Hkv, pairs = p.B * heads, units = pairs * p.row_blocks;
+  const uint32_t split = blockIdx.x / units, unit = blockIdx.x % units, pair = unit % pairs;
+  TreePart w;
+  w.z = (pair / heads + split * (uint32_t)p.turn) % (uint32_t)p.B;
+  w.hk = pair % heads;
+  w.block = unit / pairs;
+  sp = tree_span(p, w.z);
+  const int c = tree_part(p, sp.n);
+  w.t0 = (int)split * c;
+  w.t1 = min(sp.n, w.t0 + c);
+  w.rec = sp.n <= c ? -1 : ((w.z * p.Hkv + w.hk) * p.row_blocks + w.block) * p.splits + split;
+  return w;
+}
+
+// value of `v` combined over the two lanes holding one row
+template <class Op>
+__device__ __forceinline__ float tree_row(float v) {
+  return Op::apply(v, __shfl_xor(v, 32));
+}
+
+__device__ __forceinline__ void tree_barrier() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// a V fragment's infinities (+: 1, else 0) and NaN (1) as numbers of the type
+template <bool F16>
+__device__ __forceinline__ uint32_t tree_odd(uint32_t w, uint32_t sign) {
+  constexpr uint32_t EXP = F16 ? 0x7C00u : 0x7F80u, ONE = F16 ? 0x3C00u : 0x3F80u;
+  uint32_t r = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t x = (w >> (16 * h)) & 0xFFFFu;
+    const bool odd = (x & EXP) == EXP && ((x & 0x7FFFu) != EXP || (x >> 15) == sign);
+    r |= (odd ? ONE : 0u) << (16 * h);
+  }
+  return r;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t tree_finite(uint32_t w) {
+  constexpr uint32_t EXP = F16 ? 0x7C00u : 0x7F80u;
+  if ((w & EXP) == EXP) w &= 0xFFFF0000u;
+  if ((w >> 16 & EXP) == EXP) w &= 0xFFFFu;
+  return w;
+}
+template <bool F16>
+__device__ __forceinline__ bool tree_is_odd(uint32_t w) {
+  constexpr uint32_t EXP = F16 ? 0x7C00u : 0x7F80u;
+  return (w & EXP) == EXP || (w >> 16 & EXP) == EXP;
+}
+
+template <int D, int RW>
+struct TreeCfg {
+  static constexpr int KW = 4 / RW;
+  static constexpr int SUB = KW == 1 ? 2 : 1;           // 32-key tiles of a wave in a stage
+  static constexpr int TKS = 32 * KW * SUB;             // keys of a stage
+  static constexpr int ROW = 2 * D, KT = TKS * ROW, STAGE = 2 * KT;
+  static constexpr int NS = STAGE <= 16384 ? 4 : 2;
+  static constexpr int ROWS = 32 * RW;
+  static constexpr int LDS = NS * STAGE;
+  static_assert(LDS >= 4 * 32 * D * 4, "the waves' partial O fits the ring");
+};
+
+template <int D, bool F16, int RW>
+__device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
+  using C = TreeCfg<D, RW>;
+  constexpr int KW = C::KW, SUB = C::SUB, TKS = C::TKS, ROW = C::ROW, KT = C::KT, NS = C::NS, ROWS = C::ROWS;
+  constexpr int KPI = 1024 / ROW, CH = ROW / 16;  // keys of a DMA instruction, 16-byte pieces of a row
+  constexpr int DI = 16 / KPI;                    // DMA instructions of 16 keys' K
+  constexpr int RUNS = TKS / 16, RPW = RUNS / 4;  // 16-key runs of a stage, of a wave's loads
+  constexpr int SB = 64 / RUNS;                   // stages of which the lanes hold the runs' pages
+  constexpr int DPT = RPW * 2 * DI;               // DMA instructions of a wave and stage
+  constexpr int DS = D / 16, DB = D / 32;
+  __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+  __shared__ short par[TREE_NODES];
+  __shared__ float ml[4][32][2];
+  if (blockDim.x != 256) return;  // launch shape must match the kernel
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = wave / KW, kw = wave % KW;
+  const int g = lane >> 5, r32 = lane & 31;
+  const uint32_t G = p.group;
+  TreeSpan sp;
+  const TreePart w = tree_deal(p, sp);
+  const TreeSeq& sq = sp.sq;
+  const int rows = sq.nq * p.group, row0 = w.block * ROWS;
+  if (row0 >= rows || w.t0 >= sp.n) return;
+  const int nrows = min(ROWS, rows - row0);
+  const bool busy = rw * 32 < nrows;
+  const int lo = sp.kbeg + 64 * w.t0, hi = min(sp.kend, sp.kbeg + 64 * w.t1);
+  const int nst = hi > lo ? (hi - lo + TKS - 1) / TKS : 0;
+
+  // this lane's row: its node, its query
+  const uint32_t row = row0 + min(rw * 32 + r32, nrows - 1);
+  const int node = row / G;
+  u32x4 qf[DS];
+  {
+    const char* src = (const char*)p.q + 2 * ((long long)(sq.q0 + node) * p.q_st + (long long)(w.hk * G + row % G) * p.q_sh + 8 * g);
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks) qf[ks] = *(const u32x4*)(src + 32 * ks);
+  }
+  const bool tree = hi > sq.base || p.left >= 0;
+  if (tree)
+    for (int i = tid; i < sq.nq; i += 256) par[i] = (short)tree_parent(p.parent, sq, i);
+
+  const uint32_t ring32 = lds_addr(lds);
+  const char* kbase = (const char*)p.k + 2 * (long long)w.hk * p.k_h;
+  const char* vbase = (const char*)p.v + 2 * (long long)w.hk * p.v_h;
+  auto kswz = [](int key) { return D == 64 ? (key >> 1) & 7 : key & 15; };
+  auto vswz = [](int key) { return D == 64 ? (key >> 1) & 1 : key & 3; };
+  const uint32_t k_r = 2 * (uint32_t)p.k_r, v_r = 2 * (uint32_t)p.v_r;
+  const int dkey = lane / CH, dpos = lane % CH;
+  uint32_t koff[DI], voff[DI];
+#pragma unroll
+  for (int u = 0; u < DI; ++u) {
+    const int key = u * KPI + dkey;
+    koff[u] = key * k_r + ((dpos ^ kswz(key)) << 4);
+    voff[u] = key * v_r + ((dpos ^ (vswz(key) << 2)) << 4);
+  }
+  // pages and rows of the runs of the next SB stages, one per lane; a run without a page (or
+  // past the end) reads page 0 and is masked
+  const int* table = p.table + (long long)w.z * p.table_s;
+  int pages = 0, prow = 0;
+  uint64_t live[2] = {0, 0};  // by the parity of the batch of SB stages
+  auto issue = [&](int j) {
+    if (j % SB == 0) {
+      const int key = lo + TKS * (nst - 1 - (j + lane / RUNS)) + 16 * (lane % RUNS);
+      int ph = -1;
+      if (key >= lo && key < hi) {
+        const int e = (uint32_t)key / (uint32_t)p.block_size;
+        ph = e < p.max_pages ? table[e] : -1;
+        ph = ph < p.pages ? ph : -1;
+        prow = ph < 0 ? 0 : key - e * p.block_size;
+      } else {
+        prow = 0;
+      }
+      const uint64_t m = __ballot(ph >= 0);
+      if ((j / SB) & 1) live[1] = m;
+      else live[0] = m;
+      pages = max(ph, 0);
+    }
+    const uint32_t dst = ring32 + (j % NS) * C::STAGE;
+#pragma unroll
+    for (int x = 0; x < RPW; ++x) {
+      const int run = wave + 4 * x, at = j % SB * RUNS + run;
+      const uint32_t pg = __builtin_amdgcn_readlane(pages, at), pr = __builtin_amdgcn_readlane(prow, at);
+      const char* ks = kbase + 2 * (pg * (uint64_t)p.k_p) + (uint64_t)pr * k_r;
+      const char* vs = vbase + 2 * (pg * (uint64_t)p.v_p) + (uint64_t)pr * v_r;
+#pragma unroll
+      for (int u = 0; u < DI; ++u) dma_base16(ks, koff[u], dst + run * 16 * ROW + u * 1024);
+#pragma unroll
+      for (int u = 0; u < DI; ++u) dma_base16(vs, voff[u], dst + KT + run * 16 * ROW + u * 1024);
+    }
+  };
+
+  __syncthreads();  // parents
+  int first = 0;    // first key before the tree that the row sees
+  if (p.left >= 0) {
+    int depth = 0;
+    for (int c = par[node]; c >= 0; c = par[c]) ++depth;
+    first = max(0ll, (long long)sq.base + depth - p.left);
+  }
+  int cur = node, up = 0;  // next node of the way to the root, levels above the own
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
+  float ms = -__builtin_huge_valf(), l = 0.0f;
+  const float c2 = p.scale_log2;
+  // operand reads: K of key r32, V of keys 4 g + (lane & 15) / 4 .. of a 16-d half block
+  const int kread = r32 * ROW, kx = (g ^ kswz(r32)) << 4;
+  const int j16 = lane & 15;
+  const int vread = (4 * g + (j16 >> 2)) * ROW + 32 * ((lane >> 4) & 1) + 8 * (j16 & 3), vx = vswz(j16 >> 2) << 6;
+  for (int j = 0; j < NS && j < nst; ++j) issue(j);
+  for (int i = 0; i < nst; ++i) {
+    // stage i has landed once at most the later stages' loads are in flight
+    if (i + NS <= nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * DPT) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    tree_barrier();
+    if (busy) {
+      const char* st = lds + (i % NS) * C::STAGE + kw * 32 * SUB * ROW;
+      const int kv0 = lo + TKS * (nst - 1 - i) + 32 * SUB * kw;
+      f32x16 s[SUB];
+#pragma unroll
+      for (int t = 0; t < SUB; ++t) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < DS; ++ks) {
+          const u32x4 kf = *(const u32x4*)(st + t * 32 * ROW + kread + (kx ^ (ks << 5)));
+          s[t] = mfma16<F16>(kf, qf[ks], s[t]);
+        }
+      }
+      const uint32_t alive = (uint32_t)(live[(i / SB) & 1] >> (i % SB * RUNS + 2 * SUB * kw)) & ((1u << (2 * SUB)) - 1);
+      const bool mask = alive != (1u << (2 * SUB)) - 1 || kv0 + 32 * SUB > min(sq.base, hi) || __any(first > kv0);
+      uint32_t vis[SUB];  // the row's visible keys of each tile, from 4 g on
+      if (mask) {
+#pragma unroll
+        for (int t = SUB - 1; t >= 0; --t) {
+          const int k0 = kv0 + 32 * t, n0 = k0 - sq.base;  // first key, and as a node
+          uint32_t v = n0 <= -32 ? ~0u : n0 < 0 ? (1u << -n0) - 1 : 0u;
+          if (first > k0) v &= first - k0 < 32 ? ~0u << (first - k0) : 0u;
+          if (n0 > -32)
+            while (cur >= max(n0, 0)) {
+              if (cur - n0 < 32 && (p.left < 0 || up <= p.left)) v |= 1u << (cur - n0);
+              cur = par[cur];
+              ++up;
+            }
+          if (hi - k0 < 32) v &= hi > k0 ? (1u << (hi - k0)) - 1 : 0u;
+          if (!(alive >> (2 * t) & 1)) v &= 0xFFFF0000u;
+          if (!(alive >> (2 * t + 1) & 1)) v &= 0xFFFFu;
+          vis[t] = v >> (4 * g);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!(vis[t] >> (8 * (e >> 2) + (e & 3)) & 1)) s[t][e] = -__builtin_huge_valf();
+        }
+      }
+      float mh = s[0][0];
+#pragma unroll
+      for (int t = 0; t < SUB; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) mh = vmax3(mh, s[t][e], s[t][e + 1]);
+      mh *= c2;
+      if (__any(mh > ms + 8.0f)) {
+        const float mt = tree_row<OpMax>(mh);
+        const bool move = mt > ms + 8.0f;
+        const float alpha = move ? __builtin_amdgcn_exp2f(ms - mt) : 1.0f;
+        l *= alpha;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[b] *= alpha;
+        ms = move ? mt : ms;
+      }
+      // rows without a visible key so far: exponent base 0, exp2(-inf) = 0
+      const float mb = ms == -__builtin_huge_valf() ? 0.0f : ms;
+      u32x4 pf[SUB][2];
+#pragma unroll
+      for (int t = 0; t < SUB; ++t) {
+        float pe[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pe[e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c2, -mb));
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) l += (pe[e] + pe[e + 1]) + (pe[e + 2] + pe[e + 3]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pf[t][e >> 2][e & 3] = pack2(pe[2 * e], pe[2 * e + 1], F16);
+      }
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      auto vfrag = [&](int t, int k2, int b) {
+        u32x4 f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(st + KT + (32 * t + 16 * k2 + 8 * h) * ROW + vread + ((b << 6) ^ vx))));
+          f[2 * h] = x[0];
+          f[2 * h + 1] = x[1];
+        }
+        return f;
+      };
+      bool odd = false;  // something in V that is not finite
+      if (mask) {
+        for (int x = 0; x < 32 * SUB * ROW / 1024; ++x) {
+          const u32x4 f = *(const u32x4*)(st + KT + x * 1024 + lane * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= tree_is_odd<F16>(f[e]);
+        }
+        odd = __any(odd);
+      }
+      if (!odd) {
+#pragma unroll
+        for (int t = 0; t < SUB; ++t)
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+            for (int b = 0; b < DB; ++b) o[b] = mfma16<F16>(vfrag(t, k2, b), pf[t][k2], o[b]);
+      } else {
+        constexpr uint32_t ONE = F16 ? 0x3C00u : 0x3F80u;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int sign = 0; sign < 2; ++sign) {
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16 seen;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) seen[e] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < SUB; ++t)
+#pragma unroll
+              for (int k2 = 0; k2 < 2; ++k2) {
+                const u32x4 f = vfrag(t, k2, b);
+                u32x4 x, see;
+                uint32_t v = vis[t];
+                asm volatile("" : "+v"(v));  // (kept as a word, not as all its bits)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  x[e] = tree_odd<F16>(f[e], sign);
+                  const int at = 16 * k2 + 8 * (e >> 1) + 2 * (e & 1);
+                  see[e] = (v >> at & 1 ? ONE : 0u) | (v >> (at + 1) & 1 ? ONE << 16 : 0u);
+                }
+                seen = mfma16<F16>(x, see, seen);
+                if (sign) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = tree_finite<F16>(f[e]);
+                o[b] = mfma16<F16>(x, pf[t][k2], o[b]);
+              }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (seen[e] > 0.0f) o[b][e] += sign ? -__builtin_huge_valf() : __builtin_huge_valf();
+          }
+      }
+    }
+    // every wave's LDS reads have returned before the stage's slot is refilled
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    tree_barrier();
+    if (i + NS < nst) issue(i + NS);
+  }
+
+  // ---- the waves' partial rows through the ring (16-byte pieces XOR-swizzled by the row),
+  // maxima and sums beside it
+  char* mine = lds + wave * 32 * D * 4;
+  const float ls = tree_row<OpSum>(l);
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *(f32x4*)(mine + r32 * D * 4 + (((8 * b + 2 * e + g) ^ (r32 & 15)) << 4)) =
+          (f32x4){o[b][4 * e], o[b][4 * e + 1], o[b][4 * e + 2], o[b][4 * e + 3]};
+  if (g == 0) {
+    ml[wave][r32][0] = ms;
+    ml[wave][r32][1] = ls;
+  }
+  __syncthreads();
+  constexpr int CPR = D / 4;  // 16-byte pieces (4 d) of a row
+  for (int it = tid; it < nrows * CPR; it += 256) {
+    const int r = it / CPR, c = it % CPR, w0 = r / 32 * KW, rr = r % 32;
+    float m = ml[w0][rr][0];
+#pragma unroll
+    for (int x = 1; x < KW; ++x) m = fmaxf(m, ml[w0 + x][rr][0]);
+    f32x4 sum = {};
+    float lt = 0.0f;
+#pragma unroll
+    for (int x = 0; x < KW; ++x) {
+      const float mw = ml[w0 + x][rr][0], lw = ml[w0 + x][rr][1];
+      // no finite score: no key of this row (l = 0), or only NaN ones
+      const float f = mw == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      lt = fmaf(f, lw, lt);
+      const f32x4 ow = *(const f32x4*)(lds + (w0 + x) * 32 * D * 4 + rr * D * 4 + ((c ^ (rr & 15)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, ow[e], sum[e]);
+    }
+    if (w.rec >= 0) {
+      const long long rec = (long long)w.rec * ROWS + r;
+      *(f32x4*)(p.part + rec * D + c * 4) = sum;
+      if (c == 0) {
+        p.ml[2 * rec] = m;
+        p.ml[2 * rec + 1] = lt;
+      }
+      continue;
+    }
+    const int i = (uint32_t)(row0 + r) / G, h = w.hk * G + (uint32_t)(row0 + r) % G;
+    const bool empty = !(lt > 0.0f);  // zero or NaN
+    const float inv = empty ? 1.0f : 1.0f / lt;
+    char* dst = (char*)p.o + 2 * ((long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + c * 4);
+    *(u32x2*)dst = (u32x2){pack2(sum[0] * inv, sum[1] * inv, F16), pack2(sum[2] * inv, sum[3] * inv, F16)};
+    if (c == 0)
+      p.lse[(long long)h * p.lse_h + (long long)(sq.q0 + i) * p.lse_t] =
+          empty ? __builtin_huge_valf() : (m + __log2f(lt)) * 0.69314718055994530942f;
+  }
+}
+
+// Joins the parts of a block of rows: one wave per row, lane s holds part s's maximum and
+// sum (at most 64 parts), D / 64 outputs per lane; the records are read before the lengths
+// say how many of them there are (what lies behind the last one is read and left).
+template <int D, bool F16, int ROWS>
+__device__ __forceinline__ void attn_tree_merge_body(const AttnTreeArgs& p) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t id = item / (uint32_t)p.merge_rows, r = item % (uint32_t)p.merge_rows;
+  if (id >= (uint32_t)(p.B * p.Hkv * p.row_blocks)) return;
+  const uint32_t blocks = p.row_blocks, heads = p.Hkv, pair = id / blocks;
+  const int block = id % blocks, z = pair / heads, hk = pair % heads;
+  const int row = block * ROWS + r;
+  constexpr int E = D / 64, U = 32 / E;
+  using vec = float __attribute__((ext_vector_type(E)));
+  const long long rec = (long long)id * p.splits * ROWS + r;
+  const float* part = p.part + rec * D + lane * E;
+  const float* pair_ml = p.ml + 2 * (rec + (long long)min(lane, p.splits - 1) * ROWS);
+  float m = pair_ml[0], l = pair_ml[1];
+  vec v[U];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = *(const vec*)(part + (long long)min(s0 + u, p.splits - 1) * ROWS * D);
+  };
+  load(0);
+  const TreeSpan sp = tree_span(p, z);
+  if (row >= sp.sq.nq * p.group) return;
+  const int c = tree_part(p, sp.n), count = (sp.n + c - 1) / c;
+  if (count <= 1) return;  // its workgroup had all of it
+  if (lane >= count) {
+    m = -__builtin_huge_valf();
+    l = 0.0f;
+  }
+  const float mt = wave_reduce<OpMax>(m);
+  // no finite score in a part: nothing seen (O = l = 0), or only NaN, which stays
+  const float f = m == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(m - mt);
+  const float lt = wave_reduce<OpSum>(f * l);
+  vec acc = {};
+  for (int s0 = 0;;) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s0 + u, 63)));
+      if (s0 + u < count)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(x, v[u][e], acc[e]);
+    }
+    if ((s0 += U) >= count) break;
+    load(s0);
+  }
+  const int i = (uint32_t)row / (uint32_t)p.group, h = hk * p.group + (uint32_t)row % (uint32_t)p.group;
+  const bool empty = !(lt > 0.0f);  // zero or NaN
+  const float inv = empty ? 1.0f : 1.0f / lt;
+  uint16_t* dst = (uint16_t*)p.o + (long long)(sp.sq.q0 + i) * p.o_st + (long long)h * p.o_sh + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = F16 ? f32_to_f16(acc[e] * inv) : f32_to_bf16(acc[e] * inv);
+  if (lane == 0)
+    p.lse[(long long)h * p.lse_h + (long long)(sp.sq.q0 + i) * p.lse_t] =
+        empty ? __builtin_huge_valf() : (mt + __log2f(lt)) * 0.69314718055994530942f;
+}
+
 }  // namespace g950
 
 extern "C" __global__ __launch_bounds__(64) void g950_attn_tree_general(const g950::AttnTreeArgs p) {
   g950::attn_tree_general_body(p);
 }
+#define G950_TREE(NAME, D, F16, RW, PER_CU)                                                                 \
+  extern "C" __global__ __launch_bounds__(256, PER_CU) void NAME##_r##RW(const g950::AttnTreeArgs p) {      \
+    g950::attn_tree_body<D, F16, RW>(p);                                                                    \
+  }                                                                                                         \
+  extern "C" __global__ __launch_bounds__(256) void NAME##_r##RW##_merge(const g950::AttnTreeArgs p) {      \
+    g950::attn_tree_merge_body<D, F16, 32 * RW>(p);                                                         \
+  }
+#define G950_TREE_SET(TNAME, F16)                          \
+  G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 1, 2)   \
+  G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 2, 2)   \
+  G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 4, 2)   \
+  G950_TREE(g950_attn_tree_##TNAME##_d128, 128, F16, 1, 1) \
+  G950_TREE(g950_attn_tree_##TNAME##_d128, 128, F16, 2, 2) \
+  G950_TREE(g950_attn_tree_##TNAME##_d128, 128, F16, 4, 2) \
+  G950_TREE(g950_attn_tree_##TNAME##_d256, 256, F16, 2, 1) \
+  G950_TREE(g950_attn_tree_##TNAME##_d256, 256, F16, 4, 1)
+G950_TREE_SET(bf16, false)
+G950_TREE_SET(f16, true)

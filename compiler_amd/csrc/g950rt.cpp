@@ -2098,6 +2098,30 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
 constexpr long long kTreeNodes = G950_TREE_NODES;
 static_assert(kTreeNodes == TREE_NODES, "the header's limit is the kernels'");
 
+// How attention of trees cuts a call: blocks of rows (node x head of the group) per
+// (sequence, KV head), and parts of their keys, whose records need a workspace.
+struct TreeShape {
+  long long rw;          // 32-row tiles of a block
+  long long row_blocks;  // per (sequence, KV head)
+  long long blocks;      // of the call
+  long long splits;      // parts wanted
+};
+constexpr long long kTreeTarget = 4, kTreeMinKeys = 256, kTreeOneRange = 512;
+
+TreeShape tree_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
+                     long long seqlen_k) {
+  const long long cus = m ? m->cus : 256, rows = seqlen_q * (h / hk);
+  TreeShape f{};
+  f.rw = rows <= 32 && d < 256 ? 1 : rows <= 64 ? 2 : 4;
+  f.row_blocks = (rows + 32 * f.rw - 1) / (32 * f.rw);
+  f.blocks = b * hk * f.row_blocks;
+  f.splits = 1;
+  if (f.blocks && seqlen_k > kTreeOneRange)
+    f.splits = std::max(1ll, std::min({kTreeTarget * cus / f.blocks, (seqlen_k + kTreeMinKeys - 1) / kTreeMinKeys,
+                                       64ll}));  // the merge holds a row's parts in one wave's lanes
+  return f;
+}
+
 int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
                             void* stream) {
   const char* op = "paged_attention_tree";
@@ -2165,6 +2189,38 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
   a.dtype = (int)dt; a.group = (int)(H / HK); a.seqlen_q = (int)SQ;
   const long long rows = a.B && SQ ? T * H : 0;
   if (rows > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+  // the fast kernels: 16-byte rows (q, K, V), 8-byte pieces of o, 16-key runs within a page, row
+  // offsets of a run within 32 bits
+  auto rows16 = [](const View& w) {
+    return aligned16(w.addr()) && w.stride[0] % 8 == 0 && w.stride[1] % 8 == 0 && w.stride[2] % 8 == 0 && w.stride[0] >= 0 &&
+           w.stride[1] >= 0 && w.stride[1] < (1ll << 26);
+  };
+  const bool fast = is_float16ish(dt) && (D == 64 || D == 128 || D == 256) && (long long)a.max_pages * a.block_size <= 0x7FFF0000 &&
+                    a.scale_log2 > 0.0f && std::isfinite(a.scale_log2) && a.block_size % 16 == 0 && rows16(k) && rows16(v) &&
+                    aligned16(q.addr()) && a.q_st % 8 == 0 && a.q_sh % 8 == 0 && o.addr() % 8 == 0 && a.o_st % 4 == 0 &&
+                    a.o_sh % 4 == 0;
+  if (fast && rows) {
+    const TreeShape f = tree_shape(m, a.B, H, HK, D, std::min(SQ, T), SK);
+    if (f.blocks > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+    if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
+    // as many parts as the workspace holds records for
+    const long long block_rows = 32 * f.rw;
+    a.seqlen_q = (int)std::min(SQ, T);
+    a.row_blocks = (int)f.row_blocks;
+    a.splits = (int)std::max(std::min(f.splits, ws.shape[0] / (f.blocks * block_rows * (D + 2))), 1ll);
+    a.turn = std::max(a.B / a.splits, 1);
+    a.merge_rows = (int)std::min(block_rows, std::min(SQ, T) * (H / HK));
+    a.part = (float*)ws.v->data;
+    a.ml = a.part + f.blocks * block_rows * a.splits * D;
+    const long long grid = f.blocks * a.splits;
+    if (grid > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
+    char name[64];
+    const int n = snprintf(name, sizeof name, "g950_attn_tree_%s_d%lld_r%lld", dt == G950_DTYPE_BFLOAT16 ? "bf16" : "f16", D, f.rw);
+    if (int rc = launch(m, name, (unsigned)grid, 256u, a, stream)) return rc;
+    if (a.splits == 1) return G950_OK;
+    snprintf(name + n, sizeof name - n, "_merge");
+    return launch(m, name, (unsigned)((f.blocks * a.merge_rows + 3) / 4), 256u, a, stream);
+  }
   return launch(m, "g950_attn_tree_general", (unsigned)rows, 64u, a, stream);
 }
 
@@ -2531,8 +2587,14 @@ size_t g950_paged_attention_int4_workspace(g950_module* m, int64_t b, int64_t h,
   return f.splits > 1 ? (size_t)(f.blocks * f.rows * f.splits * (d + 2)) * 4 : 0;
 }
 
-size_t g950_paged_attention_tree_workspace(g950_module*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) {
-  return 0;
+size_t g950_paged_attention_tree_workspace(g950_module* m, int64_t b, int64_t h, int64_t hk, int64_t d, int64_t seqlen_q,
+                                           int64_t seqlen_k) {
+  const int64_t most = 1ll << 31;
+  if (b <= 0 || hk <= 0 || h < hk || h % hk || seqlen_q <= 0 || seqlen_k <= 0 || b > most || h > 65536 ||
+      seqlen_q > kTreeNodes || seqlen_k > most || (d != 64 && d != 128 && d != 256))
+    return 0;
+  const TreeShape f = tree_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
+  return f.splits > 1 ? (size_t)(f.blocks * 32 * f.rw * f.splits * (d + 2)) * 4 : 0;
 }
 
 int g950_sync(void* stream) {
