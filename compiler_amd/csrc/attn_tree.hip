@@ -141,9 +141,10 @@ __device__ __forceinline__ void attn_tree_general_body(const AttnTreeArgs& p) {
 //     each 32-key tile of the tree costs it a word of visible keys.  Tiles that every row
 //     sees whole (all but a few) skip that.
 //   * What a row does not see may hold anything: scores are replaced, and where V of a
-//     masked tile is not finite, 0 V would not be 0; such a tile's V is taken apart into
-//     its finite values and the signs of its infinities (NaN: both), which are joined where
-//     a row sees them.
+//     masked tile is not finite, 0 V would not be 0: such a tile is multiplied without
+//     those values, which are added, key by key, where a row sees them.
+constexpr int TREE_MIN_TILES = 4;  // of a part
+
 struct TreeSpan {
   TreeSeq sq;
   int kend;     // keys past the last that can be seen
@@ -159,28 +160,101 @@ __device__ __forceinline__ TreeSpan tree_span(const AttnTreeArgs& p, int z) {
   return s;
 }
 
+// sums of `v` over the lanes up to the own one
+__device__ __forceinline__ int tree_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
+// How the batch's keys are dealt: every sequence's tiles are cut into parts of c (the last
+// one shorter), c so that all sequences together have at most p.parts parts; no sequence has
+// more than 64.  The lengths live on the device, so each wave works this out, 64
+// sequences at a time: a batch of different lengths becomes parts of one length, and as
+// many as the chip has places for.
+struct TreeDeal {
+  const AttnTreeArgs& p;
+  int n0;  // tiles of sequence `lane`, the first 64 of the batch
+  int c;
+  __device__ __forceinline__ int tiles(int z0) const {
+    const int z = z0 + (int)(threadIdx.x & 63);
+    return z < p.B ? tree_span(p, z).n : 0;
+  }
+  __device__ __forceinline__ int tiles_again(int z0) const { return z0 ? tiles(z0) : n0; }
+  __device__ __forceinline__ explicit TreeDeal(const AttnTreeArgs& args) : p(args) {
+    n0 = tiles(0);
+    long long sum = 0;
+    int most = 0;
+    for (int z0 = 0; z0 < p.B; z0 += 64) {
+      const int n = tiles_again(z0);
+      sum += __builtin_amdgcn_readlane(tree_scan(n), 63);
+      most = max(most, (int)wave_reduce<OpMax>((float)n));  // (rounded: a 64th of it is all that is used)
+    }
+    const int room = p.parts - p.B;
+    c = max(max((int)((sum + room - 1) / room), most / 63 + 1), TREE_MIN_TILES);
+  }
+  // the sequence that part `part` belongs to, and the parts before that sequence; -1: none
+  __device__ __forceinline__ int sequence(int part, int& before) const {
+    int start = 0;
+    for (int z0 = 0; z0 < p.B; z0 += 64) {
+      const int k = (tiles_again(z0) + c - 1) / c, upto = start + tree_scan(k);
+      const uint64_t past = __ballot(upto > part);
+      if (past) {
+        const int at = __ffsll((unsigned long long)past) - 1;
+        before = __builtin_amdgcn_readlane(upto - k, at);
+        return z0 + at;
+      }
+      start = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return -1;
+  }
+  // the parts before sequence z
+  __device__ __forceinline__ int before(int z) const {
+    int start = 0;
+    for (int z0 = 0;; z0 += 64) {
+      const int k = (tiles_again(z0) + c - 1) / c, upto = start + tree_scan(k);
+      if (z < z0 + 64) return __builtin_amdgcn_readlane(upto - k, z - z0);
+      start = __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+};
+
 // What a workgroup does: tiles t0 .. t1 - 1 of a block of rows of a (sequence, KV head); rec:
-// where its partial rows go, -1 if it has all the tiles.  A sequence's tiles are cut into at most
-// `splits` parts of at least 4 by its own length; the sequence moves on with the part, so
-// that workgroups sharing a CU differ in length where the batch does.
+// where its partial rows go, -1 if it has all the tiles.  Blocks and heads of a part are neighbours:
+// the blocks, which read the same keys, are a multiple of 8 apart where there are 8 heads, so that one
+// XCD's L2 has them.
 struct TreePart {
   int z, hk, block, t0, t1, rec;
 };
-__device__ __forceinline__ int tree_part(const AttnTreeArgs& p, int n) {
-  return max((int)((uint32_t)(n + p.splits - 1) / (uint32_t)p.splits), 4);
-}
 __device__ __forceinline__ TreePart tree_deal(const AttnTreeArgs& p, TreeSpan& sp) {
-  const uint32_t heads = p.Hkv, pairs = p.B * heads, units = pairs * p.row_blocks;
-  const uint32_t split = blockIdx.x / units, unit = blockIdx.x % units, pair = unit % pairs;
+  const uint32_t heads = p.Hkv, units = heads * p.row_blocks, unit = blockIdx.x % units;
+  const int part = blockIdx.x / units;
   TreePart w;
-  w.z = (pair / heads + split * (uint32_t)p.turn) % (uint32_t)p.B;
-  w.hk = pair % heads;
-  w.block = unit / pairs;
+  w.hk = unit % heads;
+  w.block = unit / heads;
+  w.t0 = 0;
+  w.rec = -1;
+  if (p.parts == 0) {
+    w.z = part;
+    sp = tree_span(p, w.z);
+    w.t1 = sp.n;
+    return w;
+  }
+  const TreeDeal d(p);
+  int before = 0;
+  w.z = d.sequence(part, before);
+  if (w.z < 0) {
+    sp.n = 0;
+    return w;
+  }
   sp = tree_span(p, w.z);
-  const int c = tree_part(p, sp.n);
-  w.t0 = (int)split * c;
-  w.t1 = min(sp.n, w.t0 + c);
-  w.rec = sp.n <= c ? -1 : ((w.z * p.Hkv + w.hk) * p.row_blocks + w.block) * p.splits + split;
+  w.t0 = (part - before) * d.c;
+  w.t1 = min(sp.n, w.t0 + d.c);
+  if (sp.n > d.c) w.rec = blockIdx.x;
   return w;
 }
 
@@ -195,18 +269,12 @@ __device__ __forceinline__ void tree_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// a V fragment's infinities (+: 1, else 0) and NaN (1) as numbers of the type
+// a value of the type (low half) that is not finite and `sees`, else 0
 template <bool F16>
-__device__ __forceinline__ uint32_t tree_odd(uint32_t w, uint32_t sign) {
-  constexpr uint32_t EXP = F16 ? 0x7C00u : 0x7F80u, ONE = F16 ? 0x3C00u : 0x3F80u;
-  uint32_t r = 0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t x = (w >> (16 * h)) & 0xFFFFu;
-    const bool odd = (x & EXP) == EXP && ((x & 0x7FFFu) != EXP || (x >> 15) == sign);
-    r |= (odd ? ONE : 0u) << (16 * h);
-  }
-  return r;
+__device__ __forceinline__ float tree_odd(uint32_t w, bool sees) {
+  constexpr uint32_t EXP = F16 ? 0x7C00u : 0x7F80u;
+  const float x = F16 ? f16_to_f32((uint16_t)w) : bf16_to_f32((uint16_t)w);
+  return sees && (w & EXP) == EXP ? x : 0.0f;
 }
 template <bool F16>
 __device__ __forceinline__ uint32_t tree_finite(uint32_t w) {
@@ -325,6 +393,10 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     }
   };
 
+  // (the queries are waited for here, not by the compiler's count in the loop, where it
+  // would take the DMA's loads along)
+#pragma unroll
+  for (int ks = 0; ks < DS; ++ks) asm volatile("" : "+v"(qf[ks]));
   __syncthreads();  // parents
   int first = 0;    // first key before the tree that the row sees
   if (p.left >= 0) {
@@ -367,14 +439,16 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
       }
       const uint32_t alive = (uint32_t)(live[(i / SB) & 1] >> (i % SB * RUNS + 2 * SUB * kw)) & ((1u << (2 * SUB)) - 1);
       const bool mask = alive != (1u << (2 * SUB)) - 1 || kv0 + 32 * SUB > min(sq.base, hi) || __any(first > kv0);
-      uint32_t vis[SUB];  // the row's visible keys of each tile, from 4 g on
+      uint32_t vis[SUB];  // the row's visible keys of each tile
       if (mask) {
 #pragma unroll
         for (int t = SUB - 1; t >= 0; --t) {
           const int k0 = kv0 + 32 * t, n0 = k0 - sq.base;  // first key, and as a node
           uint32_t v = n0 <= -32 ? ~0u : n0 < 0 ? (1u << -n0) - 1 : 0u;
           if (first > k0) v &= first - k0 < 32 ? ~0u << (first - k0) : 0u;
-          if (n0 > -32)
+          // (a tile behind the range is walked by the part that it belongs to: here there may
+          // be no parents)
+          if (n0 > -32 && k0 < hi)
             while (cur >= max(n0, 0)) {
               if (cur - n0 < 32 && (p.left < 0 || up <= p.left)) v |= 1u << (cur - n0);
               cur = par[cur];
@@ -383,10 +457,11 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
           if (hi - k0 < 32) v &= hi > k0 ? (1u << (hi - k0)) - 1 : 0u;
           if (!(alive >> (2 * t) & 1)) v &= 0xFFFF0000u;
           if (!(alive >> (2 * t + 1) & 1)) v &= 0xFFFFu;
-          vis[t] = v >> (4 * g);
+          vis[t] = v;
+          v >>= 4 * g;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (!(vis[t] >> (8 * (e >> 2) + (e & 3)) & 1)) s[t][e] = -__builtin_huge_valf();
+            if (!(v >> (8 * (e >> 2) + (e & 3)) & 1)) s[t][e] = -__builtin_huge_valf();
         }
       }
       float mh = s[0][0];
@@ -446,39 +521,34 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
 #pragma unroll
             for (int b = 0; b < DB; ++b) o[b] = mfma16<F16>(vfrag(t, k2, b), pf[t][k2], o[b]);
       } else {
-        constexpr uint32_t ONE = F16 ? 0x3C00u : 0x3F80u;
 #pragma unroll
-        for (int b = 0; b < DB; ++b)
+        for (int t = 0; t < SUB; ++t) {
 #pragma unroll
-          for (int sign = 0; sign < 2; ++sign) {
-            __builtin_amdgcn_sched_barrier(0);
-            f32x16 seen;
+          for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) seen[e] = 0.0f;
+            for (int b = 0; b < DB; ++b) {
+              __builtin_amdgcn_sched_barrier(0);
+              u32x4 f = vfrag(t, k2, b);
 #pragma unroll
-            for (int t = 0; t < SUB; ++t)
+              for (int e = 0; e < 4; ++e) f[e] = tree_finite<F16>(f[e]);
+              o[b] = mfma16<F16>(f, pf[t][k2], o[b]);
+            }
+          // key by key: this lane's dims 32 b + 8 e + 4 g .. + 3
+#pragma unroll 1
+          for (int k = 0; k < 32; ++k) {
+            const bool sees = vis[t] >> k & 1;
 #pragma unroll
-              for (int k2 = 0; k2 < 2; ++k2) {
-                const u32x4 f = vfrag(t, k2, b);
-                u32x4 x, see;
-                uint32_t v = vis[t];
-                asm volatile("" : "+v"(v));  // (kept as a word, not as all its bits)
+            for (int b = 0; b < DB; ++b) {
+              __builtin_amdgcn_sched_barrier(0);  // (a few values at a time)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  x[e] = tree_odd<F16>(f[e], sign);
-                  const int at = 16 * k2 + 8 * (e >> 1) + 2 * (e & 1);
-                  see[e] = (v >> at & 1 ? ONE : 0u) | (v >> (at + 1) & 1 ? ONE << 16 : 0u);
-                }
-                seen = mfma16<F16>(x, see, seen);
-                if (sign) continue;
+              for (int e = 0; e < 4; ++e) {
+                const u32x2 x = *(const u32x2*)(st + KT + (32 * t + k) * ROW + ((b ^ vswz(k)) << 6) + 16 * e + 8 * g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = tree_finite<F16>(f[e]);
-                o[b] = mfma16<F16>(x, pf[t][k2], o[b]);
+                for (int h = 0; h < 4; ++h) o[b][4 * e + h] += tree_odd<F16>(x[h >> 1] >> (16 * (h & 1)), sees);
               }
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (seen[e] > 0.0f) o[b][e] += sign ? -__builtin_huge_valf() : __builtin_huge_valf();
+            }
           }
+        }
       }
     }
     // every wave's LDS reads have returned before the stage's slot is refilled
@@ -541,33 +611,31 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
 }
 
 // Joins the parts of a block of rows: one wave per row, lane s holds part s's maximum and
-// sum (at most 64 parts), D / 64 outputs per lane; the records are read before the lengths
-// say how many of them there are (what lies behind the last one is read and left).
+// sum (at most 64 parts), D / 64 outputs per lane.
 template <int D, bool F16, int ROWS>
 __device__ __forceinline__ void attn_tree_merge_body(const AttnTreeArgs& p) {
   const int lane = threadIdx.x & 63;
   const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t id = item / (uint32_t)p.merge_rows, r = item % (uint32_t)p.merge_rows;
-  if (id >= (uint32_t)(p.B * p.Hkv * p.row_blocks)) return;
-  const uint32_t blocks = p.row_blocks, heads = p.Hkv, pair = id / blocks;
-  const int block = id % blocks, z = pair / heads, hk = pair % heads;
-  const int row = block * ROWS + r;
+  const uint32_t heads = p.Hkv, units = heads * p.row_blocks, unit = id % units;
+  const int z = id / units, hk = unit % heads, block = unit / heads;
+  if (z >= p.B) return;
+  const TreeDeal d(p);
+  const TreeSpan sp = tree_span(p, z);
+  const int row = block * ROWS + r, count = (sp.n + d.c - 1) / d.c;
+  if (row >= sp.sq.nq * p.group || count <= 1) return;  // (one part: its workgroup had all of it)
   constexpr int E = D / 64, U = 32 / E;
   using vec = float __attribute__((ext_vector_type(E)));
-  const long long rec = (long long)id * p.splits * ROWS + r;
+  const long long rec = ((long long)d.before(z) * units + unit) * ROWS + r, step = (long long)units * ROWS;
   const float* part = p.part + rec * D + lane * E;
-  const float* pair_ml = p.ml + 2 * (rec + (long long)min(lane, p.splits - 1) * ROWS);
+  const float* pair_ml = p.ml + 2 * (rec + min(lane, count - 1) * step);
   float m = pair_ml[0], l = pair_ml[1];
   vec v[U];
   auto load = [&](int s0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = *(const vec*)(part + (long long)min(s0 + u, p.splits - 1) * ROWS * D);
+    for (int u = 0; u < U; ++u) v[u] = *(const vec*)(part + min(s0 + u, count - 1) * step * D);
   };
   load(0);
-  const TreeSpan sp = tree_span(p, z);
-  if (row >= sp.sq.nq * p.group) return;
-  const int c = tree_part(p, sp.n), count = (sp.n + c - 1) / c;
-  if (count <= 1) return;  // its workgroup had all of it
   if (lane >= count) {
     m = -__builtin_huge_valf();
     l = 0.0f;

@@ -232,11 +232,10 @@ struct AttnTreeArgs {
   int group;                // query heads per KV head
   int seqlen_q;             // nodes per sequence that take part
   int row_blocks;           // blocks of rows (node x head of the group) per (sequence, KV head)
-  int splits;               // parts that a block's keys are cut into at most
-  int turn;                 // sequences to move on by from one part to the next
+  int parts;                // parts that the batch's keys are cut into at most; 0: one per sequence
   int merge_rows;           // rows of a block that any sequence can have
-  float* part;              // [blocks * splits][rows][D] unnormalised O
-  float* ml;                // [blocks * splits][rows][2] maximum (log2 units), sum
+  float* part;              // [parts][row_blocks][Hkv][rows][D] unnormalised O
+  float* ml;                // [parts][row_blocks][Hkv][rows][2] maximum (log2 units), sum
 };
 
 // Verification of drafted trees (verify_tree.hip).

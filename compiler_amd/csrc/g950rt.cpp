@@ -2103,22 +2103,22 @@ static_assert(kTreeNodes == TREE_NODES, "the header's limit is the kernels'");
 struct TreeShape {
   long long rw;          // 32-row tiles of a block
   long long row_blocks;  // per (sequence, KV head)
-  long long blocks;      // of the call
-  long long splits;      // parts wanted
+  long long units;       // blocks of a sequence
+  long long parts;       // of the batch, wanted; 0: one per sequence
 };
-constexpr long long kTreeTarget = 4, kTreeMinKeys = 256, kTreeOneRange = 512;
+constexpr long long kTreeOneRange = 512;
 
 TreeShape tree_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
                      long long seqlen_k) {
+  static const long long env1 = getenv("TREE_T1") ? atoi(getenv("TREE_T1")) : 4, env2 = getenv("TREE_T2") ? atoi(getenv("TREE_T2")) : 2;
   const long long cus = m ? m->cus : 256, rows = seqlen_q * (h / hk);
   TreeShape f{};
   f.rw = rows <= 32 && d < 256 ? 1 : rows <= 64 ? 2 : 4;
   f.row_blocks = (rows + 32 * f.rw - 1) / (32 * f.rw);
-  f.blocks = b * hk * f.row_blocks;
-  f.splits = 1;
-  if (f.blocks && seqlen_k > kTreeOneRange)
-    f.splits = std::max(1ll, std::min({kTreeTarget * cus / f.blocks, (seqlen_k + kTreeMinKeys - 1) / kTreeMinKeys,
-                                       64ll}));  // the merge holds a row's parts in one wave's lanes
+  f.units = hk * f.row_blocks;
+  const long long places = (f.rw == 1 ? env1 : env2) * cus;
+  if (f.units && seqlen_k > kTreeOneRange && b * f.units < places)
+    f.parts = std::max(places / f.units, 2 * b);
   return f;
 }
 
@@ -2201,25 +2201,24 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
                     a.o_sh % 4 == 0;
   if (fast && rows) {
     const TreeShape f = tree_shape(m, a.B, H, HK, D, std::min(SQ, T), SK);
-    if (f.blocks > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
     if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
-    // as many parts as the workspace holds records for
     const long long block_rows = 32 * f.rw;
+    // as many parts as the workspace holds records for; one more than the sequences, or none
+    a.parts = (int)std::min(f.parts, ws.shape[0] / (f.units * block_rows * (D + 2)));
+    if (a.parts <= a.B) a.parts = 0;
     a.seqlen_q = (int)std::min(SQ, T);
     a.row_blocks = (int)f.row_blocks;
-    a.splits = (int)std::max(std::min(f.splits, ws.shape[0] / (f.blocks * block_rows * (D + 2))), 1ll);
-    a.turn = std::max(a.B / a.splits, 1);
     a.merge_rows = (int)std::min(block_rows, std::min(SQ, T) * (H / HK));
     a.part = (float*)ws.v->data;
-    a.ml = a.part + f.blocks * block_rows * a.splits * D;
-    const long long grid = f.blocks * a.splits;
+    a.ml = a.part + a.parts * f.units * block_rows * D;
+    const long long grid = f.units * (a.parts ? a.parts : a.B);
     if (grid > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
     char name[64];
     const int n = snprintf(name, sizeof name, "g950_attn_tree_%s_d%lld_r%lld", dt == G950_DTYPE_BFLOAT16 ? "bf16" : "f16", D, f.rw);
     if (int rc = launch(m, name, (unsigned)grid, 256u, a, stream)) return rc;
-    if (a.splits == 1) return G950_OK;
+    if (!a.parts) return G950_OK;
     snprintf(name + n, sizeof name - n, "_merge");
-    return launch(m, name, (unsigned)((f.blocks * a.merge_rows + 3) / 4), 256u, a, stream);
+    return launch(m, name, (unsigned)((a.B * f.units * a.merge_rows + 3) / 4), 256u, a, stream);
   }
   return launch(m, "g950_attn_tree_general", (unsigned)rows, 64u, a, stream);
 }
@@ -2594,7 +2593,7 @@ size_t g950_paged_attention_tree_workspace(g950_module* m, int64_t b, int64_t h,
       seqlen_q > kTreeNodes || seqlen_k > most || (d != 64 && d != 128 && d != 256))
     return 0;
   const TreeShape f = tree_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
-  return f.splits > 1 ? (size_t)(f.blocks * 32 * f.rw * f.splits * (d + 2)) * 4 : 0;
+  return (size_t)(f.parts * f.units * 32 * f.rw * (d + 2)) * 4;
 }
 
 int g950_sync(void* stream) {
