@@ -141,8 +141,8 @@ __device__ __forceinline__ void attn_tree_general_body(const AttnTreeArgs& p) {
 //     each 32-key tile of the tree costs it a word of visible keys.  Tiles that every row
 //     sees whole (all but a few) skip that.
 //   * What a row does not see may hold anything: scores are replaced, and where V of a
-//     masked tile is not finite, 0 V would not be 0: such a tile is multiplied without
-//     those values, which are added, key by key, where a row sees them.
+//     stage that some row does not see whole is not finite, 0 V would not be 0: such values
+//     are added, key by key, where a row sees them, and taken out of the stage.
 constexpr int TREE_MIN_TILES = 4;  // of a part
 
 struct TreeSpan {
@@ -283,19 +283,13 @@ __device__ __forceinline__ uint32_t tree_finite(uint32_t w) {
   if ((w >> 16 & EXP) == EXP) w &= 0xFFFFu;
   return w;
 }
-template <bool F16>
-__device__ __forceinline__ bool tree_is_odd(uint32_t w) {
-  constexpr uint32_t EXP = F16 ? 0x7C00u : 0x7F80u;
-  return (w & EXP) == EXP || (w >> 16 & EXP) == EXP;
-}
-
 template <int D, int RW>
 struct TreeCfg {
   static constexpr int KW = 4 / RW;
   static constexpr int SUB = KW == 1 ? 2 : 1;           // 32-key tiles of a wave in a stage
   static constexpr int TKS = 32 * KW * SUB;             // keys of a stage
   static constexpr int ROW = 2 * D, KT = TKS * ROW, STAGE = 2 * KT;
-  static constexpr int NS = STAGE <= 16384 ? 4 : 2;
+  static constexpr int NS = STAGE <= 16384 && RW < 4 ? 4 : 2;
   static constexpr int ROWS = 32 * RW;
   static constexpr int LDS = NS * STAGE;
   static_assert(LDS >= 4 * 32 * D * 4, "the waves' partial O fits the ring");
@@ -314,6 +308,7 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
   __shared__ short par[TREE_NODES];
   __shared__ float ml[4][32][2];
+  __shared__ int odd[4];
   if (blockDim.x != 256) return;  // launch shape must match the kernel
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -357,46 +352,49 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     koff[u] = key * k_r + ((dpos ^ kswz(key)) << 4);
     voff[u] = key * v_r + ((dpos ^ (vswz(key) << 2)) << 4);
   }
-  // pages and rows of the runs of the next SB stages, one per lane; a run without a page (or
-  // past the end) reads page 0 and is masked
+  // pages and rows of the runs of SB stages, one per lane, looked up a stage before they are
+  // needed; a run without a page (or past the end) reads page 0 and is masked
   const int* table = p.table + (long long)w.z * p.table_s;
-  int pages = 0, prow = 0;
+  int next = -1, pages = 0, prow = 0;
   uint64_t live[2] = {0, 0};  // by the parity of the batch of SB stages
-  auto issue = [&](int j) {
+  auto batch_key = [&](int j) { return lo + TKS * (nst - 1 - (j + lane / RUNS)) + 16 * (lane % RUNS); };
+  auto look = [&](int j) {
+    const int key = batch_key(j), e = (uint32_t)max(key, 0) / (uint32_t)p.block_size;
+    next = key >= lo && key < hi && e < p.max_pages ? table[e] : -1;
+  };
+  uint32_t pg[RPW], pr[RPW];  // of the wave's runs of the last stage whose K was issued
+  auto stage_pages = [&](int j) {
     if (j % SB == 0) {
-      const int key = lo + TKS * (nst - 1 - (j + lane / RUNS)) + 16 * (lane % RUNS);
-      int ph = -1;
-      if (key >= lo && key < hi) {
-        const int e = (uint32_t)key / (uint32_t)p.block_size;
-        ph = e < p.max_pages ? table[e] : -1;
-        ph = ph < p.pages ? ph : -1;
-        prow = ph < 0 ? 0 : key - e * p.block_size;
-      } else {
-        prow = 0;
-      }
+      const int key = batch_key(j), ph = next < p.pages ? next : -1;
       const uint64_t m = __ballot(ph >= 0);
       if ((j / SB) & 1) live[1] = m;
       else live[0] = m;
       pages = max(ph, 0);
+      prow = ph < 0 ? 0 : (uint32_t)key % (uint32_t)p.block_size;
     }
-    const uint32_t dst = ring32 + (j % NS) * C::STAGE;
 #pragma unroll
     for (int x = 0; x < RPW; ++x) {
-      const int run = wave + 4 * x, at = j % SB * RUNS + run;
-      const uint32_t pg = __builtin_amdgcn_readlane(pages, at), pr = __builtin_amdgcn_readlane(prow, at);
-      const char* ks = kbase + 2 * (pg * (uint64_t)p.k_p) + (uint64_t)pr * k_r;
-      const char* vs = vbase + 2 * (pg * (uint64_t)p.v_p) + (uint64_t)pr * v_r;
-#pragma unroll
-      for (int u = 0; u < DI; ++u) dma_base16(ks, koff[u], dst + run * 16 * ROW + u * 1024);
-#pragma unroll
-      for (int u = 0; u < DI; ++u) dma_base16(vs, voff[u], dst + KT + run * 16 * ROW + u * 1024);
+      const int at = j % SB * RUNS + wave + 4 * x;
+      pg[x] = __builtin_amdgcn_readlane(pages, at);
+      pr[x] = __builtin_amdgcn_readlane(prow, at);
     }
   };
+  auto dma = [&](const char* base, long long page, uint32_t step, const uint32_t (&off)[DI], uint32_t dst) {
+#pragma unroll
+    for (int x = 0; x < RPW; ++x) {
+      const char* src = base + 2 * (pg[x] * (uint64_t)page) + (uint64_t)pr[x] * step;
+#pragma unroll
+      for (int u = 0; u < DI; ++u) dma_base16(src, off[u], dst + (wave + 4 * x) * 16 * ROW + u * 1024);
+    }
+  };
+  auto dma_k = [&](uint32_t dst) { dma(kbase, p.k_p, k_r, koff, ring32 + dst); };
+  auto dma_v = [&](uint32_t dst) { dma(vbase, p.v_p, v_r, voff, ring32 + dst); };
 
   // (the queries are waited for here, not by the compiler's count in the loop, where it
   // would take the DMA's loads along)
 #pragma unroll
   for (int ks = 0; ks < DS; ++ks) asm volatile("" : "+v"(qf[ks]));
+  look(0);
   __syncthreads();  // parents
   int first = 0;    // first key before the tree that the row sees
   if (p.left >= 0) {
@@ -411,156 +409,287 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
   for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
-  float ms = -__builtin_huge_valf(), l = 0.0f;
+  float ms = -__builtin_huge_valf(), l[4] = {};
   const float c2 = p.scale_log2;
   // operand reads: K of key r32, V of keys 4 g + (lane & 15) / 4 .. of a 16-d half block
   const int kread = r32 * ROW, kx = (g ^ kswz(r32)) << 4;
   const int j16 = lane & 15;
   const int vread = (4 * g + (j16 >> 2)) * ROW + 32 * ((lane >> 4) & 1) + 8 * (j16 & 3), vx = vswz(j16 >> 2) << 6;
-  for (int j = 0; j < NS && j < nst; ++j) issue(j);
-  for (int i = 0; i < nst; ++i) {
-    // stage i has landed once at most the later stages' loads are in flight
-    if (i + NS <= nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * DPT) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    tree_barrier();
-    if (busy) {
-      const char* st = lds + (i % NS) * C::STAGE + kw * 32 * SUB * ROW;
-      const int kv0 = lo + TKS * (nst - 1 - i) + 32 * SUB * kw;
-      f32x16 s[SUB];
+  f32x16 s[SUB];
+  u32x4 pf[SUB][2];
+  uint32_t vis[SUB];  // the row's visible keys of each tile of a masked stage
+  // S^T of a wave's tiles (K at `kp`)
+  auto scores = [&](const char* kp) {
 #pragma unroll
-      for (int t = 0; t < SUB; ++t) {
+    for (int t = 0; t < SUB; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+      for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < DS; ++ks) {
-          const u32x4 kf = *(const u32x4*)(st + t * 32 * ROW + kread + (kx ^ (ks << 5)));
-          s[t] = mfma16<F16>(kf, qf[ks], s[t]);
-        }
-      }
-      const uint32_t alive = (uint32_t)(live[(i / SB) & 1] >> (i % SB * RUNS + 2 * SUB * kw)) & ((1u << (2 * SUB)) - 1);
-      const bool mask = alive != (1u << (2 * SUB)) - 1 || kv0 + 32 * SUB > min(sq.base, hi) || __any(first > kv0);
-      uint32_t vis[SUB];  // the row's visible keys of each tile
-      if (mask) {
-#pragma unroll
-        for (int t = SUB - 1; t >= 0; --t) {
-          const int k0 = kv0 + 32 * t, n0 = k0 - sq.base;  // first key, and as a node
-          uint32_t v = n0 <= -32 ? ~0u : n0 < 0 ? (1u << -n0) - 1 : 0u;
-          if (first > k0) v &= first - k0 < 32 ? ~0u << (first - k0) : 0u;
-          // (a tile behind the range is walked by the part that it belongs to: here there may
-          // be no parents)
-          if (n0 > -32 && k0 < hi)
-            while (cur >= max(n0, 0)) {
-              if (cur - n0 < 32 && (p.left < 0 || up <= p.left)) v |= 1u << (cur - n0);
-              cur = par[cur];
-              ++up;
-            }
-          if (hi - k0 < 32) v &= hi > k0 ? (1u << (hi - k0)) - 1 : 0u;
-          if (!(alive >> (2 * t) & 1)) v &= 0xFFFF0000u;
-          if (!(alive >> (2 * t + 1) & 1)) v &= 0xFFFFu;
-          vis[t] = v;
-          v >>= 4 * g;
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (!(v >> (8 * (e >> 2) + (e & 3)) & 1)) s[t][e] = -__builtin_huge_valf();
-        }
-      }
-      float mh = s[0][0];
+    for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
       for (int t = 0; t < SUB; ++t)
+        s[t] = mfma16<F16>(*(const u32x4*)(kp + t * 32 * ROW + kread + (kx ^ (ks << 5))), qf[ks], s[t]);
+  };
+  // stage i's scores of unseen keys replaced
+  auto mask = [&](int i) {
+    const int kv0 = lo + TKS * (nst - 1 - i) + 32 * SUB * kw;
+    const uint32_t alive = (uint32_t)(live[(i / SB) & 1] >> (i % SB * RUNS + 2 * SUB * kw)) & ((1u << (2 * SUB)) - 1);
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) mh = vmax3(mh, s[t][e], s[t][e + 1]);
-      mh *= c2;
-      if (__any(mh > ms + 8.0f)) {
-        const float mt = tree_row<OpMax>(mh);
-        const bool move = mt > ms + 8.0f;
-        const float alpha = move ? __builtin_amdgcn_exp2f(ms - mt) : 1.0f;
-        l *= alpha;
+    for (int t = 0; t < SUB; ++t) vis[t] = ~0u;
+    if (alive == (1u << (2 * SUB)) - 1 && kv0 + 32 * SUB <= min(sq.base, hi) && !__any(first > kv0)) return;
 #pragma unroll
-        for (int b = 0; b < DB; ++b) o[b] *= alpha;
-        ms = move ? mt : ms;
-      }
-      // rows without a visible key so far: exponent base 0, exp2(-inf) = 0
-      const float mb = ms == -__builtin_huge_valf() ? 0.0f : ms;
-      u32x4 pf[SUB][2];
-#pragma unroll
-      for (int t = 0; t < SUB; ++t) {
-        float pe[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pe[e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c2, -mb));
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) l += (pe[e] + pe[e + 1]) + (pe[e + 2] + pe[e + 3]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pf[t][e >> 2][e & 3] = pack2(pe[2 * e], pe[2 * e + 1], F16);
-      }
-      typedef short s16x4 __attribute__((ext_vector_type(4)));
-      auto vfrag = [&](int t, int k2, int b) {
-        u32x4 f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4*)(st + KT + (32 * t + 16 * k2 + 8 * h) * ROW + vread + ((b << 6) ^ vx))));
-          f[2 * h] = x[0];
-          f[2 * h + 1] = x[1];
+    for (int t = SUB - 1; t >= 0; --t) {
+      const int k0 = kv0 + 32 * t, n0 = k0 - sq.base;  // first key, and as a node
+      uint32_t v = n0 <= -32 ? ~0u : n0 < 0 ? (1u << -n0) - 1 : 0u;
+      if (first > k0) v &= first - k0 < 32 ? ~0u << (first - k0) : 0u;
+      // (a tile behind the range is walked by the part that it belongs to: here there may
+      // be no parents)
+      if (n0 > -32 && k0 < hi)
+        while (cur >= max(n0, 0)) {
+          if (cur - n0 < 32 && (p.left < 0 || up <= p.left)) v |= 1u << (cur - n0);
+          cur = par[cur];
+          ++up;
         }
-        return f;
-      };
-      bool odd = false;  // something in V that is not finite
-      if (mask) {
-        for (int x = 0; x < 32 * SUB * ROW / 1024; ++x) {
-          const u32x4 f = *(const u32x4*)(st + KT + x * 1024 + lane * 16);
+      if (hi - k0 < 32) v &= hi > k0 ? (1u << (hi - k0)) - 1 : 0u;
+      if (!(alive >> (2 * t) & 1)) v &= 0xFFFF0000u;
+      if (!(alive >> (2 * t + 1) & 1)) v &= 0xFFFFu;
+      vis[t] = v;
+      v >>= 4 * g;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= tree_is_odd<F16>(f[e]);
-        }
-        odd = __any(odd);
+      for (int e = 0; e < 16; ++e)
+        if (!(v >> (8 * (e >> 2) + (e & 3)) & 1)) s[t][e] = -__builtin_huge_valf();
+    }
+  };
+  auto softmax = [&]() {
+    float mh = s[0][0];
+#pragma unroll
+    for (int t = 0; t < SUB; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) mh = vmax3(mh, s[t][e], s[t][e + 1]);
+    mh *= c2;
+    if (__any(mh > ms + 8.0f)) {
+      const float mt = tree_row<OpMax>(mh);
+      const bool move = mt > ms + 8.0f;
+      const float alpha = move ? __builtin_amdgcn_exp2f(ms - mt) : 1.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l[e] *= alpha;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] *= alpha;
+      ms = move ? mt : ms;
+    }
+    // rows without a visible key so far: exponent base 0, exp2(-inf) = 0
+    const float mb = ms == -__builtin_huge_valf() ? 0.0f : ms;
+#pragma unroll
+    for (int t = 0; t < SUB; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c2, -mb));
+        l[e & 3] += s[t][e];
       }
-      if (!odd) {
 #pragma unroll
-        for (int t = 0; t < SUB; ++t)
+      for (int e = 0; e < 8; ++e) pf[t][e >> 2][e & 3] = pack2(s[t][2 * e], s[t][2 * e + 1], F16);
+    }
+  };
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  auto vfrag = [&](const char* vp, int t, int k2, int b) {
+    u32x4 f;
 #pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2)
+    for (int h = 0; h < 2; ++h) {
+      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(vp + (32 * t + 16 * k2 + 8 * h) * ROW + vread + ((b << 6) ^ vx))));
+      f[2 * h] = x[0];
+      f[2 * h + 1] = x[1];
+    }
+    return f;
+  };
+  // O^T += V^T.P^T of a wave's tiles (V at `vp`)
+  auto values = [&](const char* vp) {
 #pragma unroll
-            for (int b = 0; b < DB; ++b) o[b] = mfma16<F16>(vfrag(t, k2, b), pf[t][k2], o[b]);
-      } else {
+    for (int t = 0; t < SUB; ++t)
 #pragma unroll
-        for (int t = 0; t < SUB; ++t) {
+      for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2)
+        for (int b = 0; b < DB; ++b) o[b] = mfma16<F16>(vfrag(vp, t, k2, b), pf[t][k2], o[b]);
+  };
+  // Stage i (V at `vp`) where some row does not see all of it: what is not finite in V is
+  // added to the rows that see it and taken out of the tile.  Called by all waves, behind the
+  // softmax.
+  auto clean = [&](int i, char* vp) {
+    const int kv0 = lo + TKS * (nst - 1 - i);
+    const uint32_t alive = (uint32_t)(live[(i / SB) & 1] >> (i % SB * RUNS)) & ((1u << RUNS) - 1);
+    if (alive == (1u << RUNS) - 1 && kv0 + TKS <= min(sq.base, hi) && (p.left < 0 || sq.base + sq.nq - p.left <= kv0)) return;
+    // an exponent of ones carries into the bit above it
+    constexpr uint32_t EXP = F16 ? 0x7C007C00u : 0x7F807F80u, CARRY = F16 ? 0x04000400u : 0x00800080u;
+    uint32_t found = 0;
+#pragma unroll 4
+    for (int x = tid; x < KT / 16; x += 256) {
+      const u32x4 f = *(const u32x4*)(vp + x * 16);
 #pragma unroll
-            for (int b = 0; b < DB; ++b) {
-              __builtin_amdgcn_sched_barrier(0);
-              u32x4 f = vfrag(t, k2, b);
+      for (int e = 0; e < 4; ++e) found |= (f[e] & EXP) + CARRY;
+    }
+    found = __any(found & 0x80008000u);
+    if (lane == 0) odd[wave] = (int)found;
+    __syncthreads();
+    if (!(odd[0] | odd[1] | odd[2] | odd[3])) return;
+    if (busy)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) f[e] = tree_finite<F16>(f[e]);
-              o[b] = mfma16<F16>(f, pf[t][k2], o[b]);
-            }
-          // key by key: this lane's dims 32 b + 8 e + 4 g .. + 3
+      for (int t = 0; t < SUB; ++t)
 #pragma unroll 1
-          for (int k = 0; k < 32; ++k) {
-            const bool sees = vis[t] >> k & 1;
+        for (int k = 0; k < 32; ++k) {  // this lane's dims 32 b + 8 e + 4 g .. + 3 of the key
+          const bool sees = vis[t] >> k & 1;
 #pragma unroll
-            for (int b = 0; b < DB; ++b) {
-              __builtin_amdgcn_sched_barrier(0);  // (a few values at a time)
+          for (int b = 0; b < DB; ++b) {
+            __builtin_amdgcn_sched_barrier(0);  // (a few values at a time)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const u32x2 x = *(const u32x2*)(st + KT + (32 * t + k) * ROW + ((b ^ vswz(k)) << 6) + 16 * e + 8 * g);
+            for (int e = 0; e < 4; ++e) {
+              const u32x2 x = *(const u32x2*)(vp + (32 * (kw * SUB + t) + k) * ROW + ((b ^ vswz(k)) << 6) + 16 * e + 8 * g);
 #pragma unroll
-                for (int h = 0; h < 4; ++h) o[b][4 * e + h] += tree_odd<F16>(x[h >> 1] >> (16 * (h & 1)), sees);
-              }
+              for (int h = 0; h < 4; ++h) o[b][4 * e + h] += tree_odd<F16>(x[h >> 1] >> (16 * (h & 1)), sees);
             }
           }
         }
+    __syncthreads();
+#pragma unroll 1
+    for (int x = tid; x < KT / 16; x += 256) {
+      u32x4 f = *(const u32x4*)(vp + x * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = tree_finite<F16>(f[e]);
+      *(u32x4*)(vp + x * 16) = f;
+    }
+    __syncthreads();
+  };
+
+  if constexpr (RW == 4 && D < 256) {
+    // Bound by the matrix cores and the vector ALU beside the bytes.  Iteration i: V of
+    // stage i and K of i + 1 have landed; softmax of stage i, then its V and the next
+    // stage's scores in one run of MFMAs at raised priority, whose operand reads are issued ahead
+    // of them (two groups of V, eight fragments of K): the softmax of one of the two
+    // waves of a SIMD runs beside the MFMAs of the other.  K is issued two stages ahead, V one.
+    auto kat = [&](int i) { return (uint32_t)(i & 1) * KT; };
+    auto vat = [&](int i) { return (uint32_t)(2 + (i & 1)) * KT; };
+    constexpr int R = 2 * DB, NV = 2 * SUB, NK = SUB * DS;
+    u32x2 vt[2][R];
+    u32x4 kf[8];
+    auto vread_ = [&](auto ic, uint32_t slot) {  // group I: V of keys 16 I .. + 15
+      constexpr int I = decltype(ic)::value;
+      static_for<R>([&](auto qc) {
+        constexpr int Q = decltype(qc)::value;
+        lds_rdtr<(16 * I + 8 * (Q & 1)) * ROW>(vt[I & 1][Q], ring32 + slot + vread + (((Q >> 1) << 6) ^ vx));
+      });
+    };
+    auto vmma = [&](auto ic) {
+      constexpr int I = decltype(ic)::value;
+      static_for<DB>([&](auto bc) {
+        constexpr int B = decltype(bc)::value;
+        const u32x4 vf = {vt[I & 1][2 * B][0], vt[I & 1][2 * B][1], vt[I & 1][2 * B + 1][0], vt[I & 1][2 * B + 1][1]};
+        o[B] = mfma16<F16>(vf, pf[I >> 1][I & 1], o[B]);
+      });
+    };
+    auto kread_ = [&](auto jc, uint32_t slot) {  // fragment J: tile J % SUB, k-step J / SUB
+      constexpr int J = decltype(jc)::value;
+      if constexpr (J < NK)
+        lds_rd128<(J % SUB) * 32 * ROW>(kf[J & 7], ring32 + slot + kread + (kx ^ ((J / SUB) << 5)));
+    };
+    auto kahead = [&](uint32_t slot) { static_for<4>([&](auto jc) { kread_(jc, slot); }); };
+    // O^T += V^T.P^T, with the first four fragments of the next K on the way (each wait
+    // names how many reads were issued after the group it completes).  What is read ahead is
+    // waited for in the same run of code: no branch or copy meets a register in flight.
+    auto run_v = [&](uint32_t vslot, uint32_t kslot) {
+      vread_(std::integral_constant<int, 0>{}, vslot);
+      vread_(std::integral_constant<int, 1>{}, vslot);
+      static_for<NV>([&](auto ic) {
+        constexpr int I = decltype(ic)::value;
+        if constexpr (I + 1 == NV) kahead(kslot);
+        constexpr int after = I + 1 < NV ? R : 4;
+        lds_wait<after>(vt[I & 1]);
+        vmma(ic);
+        if constexpr (I + 2 < NV) vread_(std::integral_constant<int, I + 2>{}, vslot);
+      });
+    };
+    auto run_k = [&](uint32_t slot) {
+      static_for<4>([&](auto jc) { kread_(std::integral_constant<int, decltype(jc)::value + 4>{}, slot); });
+      static_for<NK>([&](auto jc) {
+        constexpr int J = decltype(jc)::value;
+        constexpr int after = NK - J - 1 < 7 ? NK - J - 1 : 7;
+        lds_wait<after>(kf[J & 7]);
+        s[J % SUB] = mfma16<F16>(kf[J & 7], qf[J / SUB], J < SUB ? (f32x16){} : s[J % SUB]);
+        kread_(std::integral_constant<int, J + 8>{}, slot);
+      });
+    };
+    if (nst > 0) {
+      stage_pages(0);
+      dma_k(kat(0));
+      dma_v(vat(0));
+    }
+    if (nst > 1) {
+      stage_pages(1);
+      dma_k(kat(1));
+    }
+    // K of stage 0 has landed (V of stage 0 and K of stage 1 may be in flight)
+    if (nst > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * DI * RPW) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(DI * RPW) : "memory");
+    tree_barrier();
+    if (busy && nst > 0) {
+      kahead(kat(0));
+      run_k(kat(0));
+    }
+    for (int i = 0; i < nst; ++i) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      tree_barrier();
+      // (into the slots of K of stage i, whose scores are formed, and of V of stage i - 1)
+      if (i + 1 < nst) dma_v(vat(i + 1));
+      if (i + 2 < nst) {
+        stage_pages(i + 2);
+        dma_k(kat(i + 2));
+        if ((i + 3) % SB == 0) look(i + 3);
+      }
+      if (busy) {
+        mask(i);
+        softmax();
+      }
+      clean(i, lds + vat(i));
+      if (busy) {
+        __builtin_amdgcn_s_setprio(2);
+        // (behind the last stage the scores are those of what the slot holds, and nobody's)
+        run_v(vat(i), kat(i + 1));
+        run_k(kat(i + 1));
+        __builtin_amdgcn_s_setprio(0);
       }
     }
-    // every wave's LDS reads have returned before the stage's slot is refilled
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     tree_barrier();
-    if (i + NS < nst) issue(i + NS);
+  } else {
+    // Bound by the bytes: whole stages in a ring of NS.
+    auto issue = [&](int j) {
+      stage_pages(j);
+      dma_k(j % NS * C::STAGE);
+      dma_v(j % NS * C::STAGE + KT);
+      if ((j + 1) % SB == 0) look(j + 1);
+    };
+    for (int j = 0; j < NS && j < nst; ++j) issue(j);
+    for (int i = 0; i < nst; ++i) {
+      // stage i has landed once at most the later stages' loads are in flight
+      if (i + NS <= nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * DPT) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      tree_barrier();
+      const char* st = lds + (i % NS) * C::STAGE + kw * 32 * SUB * ROW;
+      if (busy) {
+        scores(st);
+        mask(i);
+        softmax();
+      }
+      clean(i, lds + (i % NS) * C::STAGE + KT);
+      if (busy) values(st + KT);
+      // every wave's LDS reads have returned before the stage's slot is refilled
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      tree_barrier();
+      if (i + NS < nst) issue(i + NS);
+    }
   }
 
   // ---- the waves' partial rows through the ring (16-byte pieces XOR-swizzled by the row),
   // maxima and sums beside it
   char* mine = lds + wave * 32 * D * 4;
-  const float ls = tree_row<OpSum>(l);
+  const float ls = tree_row<OpSum>((l[0] + l[1]) + (l[2] + l[3]));
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
