@@ -253,7 +253,12 @@ struct VerifyArgs {
   long long t_row, d_row, path_z, count_z, next_z;
   int T, B, V, L;
   int token64, distinct;
+  int parts;                // workgroups of a sequence, at most 64
+  double* px;               // parts: [T][2] each node's probabilities after its parent
+  uint64_t* told;           // parts: [B][VERIFY_TELL][parts] sums
 };
+// rounds of a sequence whose sums the workgroups tell each other
+constexpr int VERIFY_TELL = 32;
 
 // Attention over a paged cache of 4-bit rows (attn_int4.hip).
 struct AttnInt4Args {

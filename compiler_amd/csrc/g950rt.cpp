@@ -2223,18 +2223,28 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
   return launch(m, "g950_attn_tree_general", (unsigned)rows, 64u, a, stream);
 }
 
+// Workgroups of a sequence: as many as there are CUs for, with some thousand columns each.
+long long verify_parts(const g950_module* m, long long b, long long v) {
+  static const long long env1 = getenv("VER_C") ? atoi(getenv("VER_C")) : 2048, env2 = getenv("VER_M") ? atoi(getenv("VER_M")) : 1;
+  const long long cus = env2 * (m ? m->cus : 256);
+  return b < 1 ? 1 : std::max(1ll, std::min({cus / b, v / env1, 64ll}));
+}
+size_t verify_bytes(long long b, long long t, long long parts) {
+  return parts > 1 ? (size_t)(t * 16 + b * VERIFY_TELL * parts * 8) : 0;
+}
+
 int op_verify_tree(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
                    void* stream) {
   const char* op = "verify_tree";
-  if (nviews != 10 || nsc != 1)
-    return fail(G950_USAGE, "%s: needs 10 views (count_ptr .. uniform_ptr) and the scalar distinct", op);
-  View count, cu, draft, next, parent, path, target, tokens, last, u;
-  const struct { View* w; const char* name; int nd; bool out; } vw[10] = {
+  if (nviews != 11 || nsc != 1)
+    return fail(G950_USAGE, "%s: needs 11 views (count_ptr .. workspace_ptr) and the scalar distinct", op);
+  View count, cu, draft, next, parent, path, target, tokens, last, u, ws;
+  const struct { View* w; const char* name; int nd; bool out; } vw[11] = {
       {&count, "count_ptr", 1, true}, {&cu, "cu_seqlens_q_ptr", 1, false}, {&draft, "draft_probs_ptr", 2, false},
       {&next, "next_ptr", 1, true}, {&parent, "parent_ptr", 1, false}, {&path, "path_ptr", 2, true},
       {&target, "target_probs_ptr", 2, false}, {&tokens, "tokens_ptr", 1, false},
-      {&last, "uniform_next_ptr", 1, false}, {&u, "uniform_ptr", 1, false}};
-  for (uint32_t i = 0; i < 10; ++i)
+      {&last, "uniform_next_ptr", 1, false}, {&u, "uniform_ptr", 1, false}, {&ws, "workspace_ptr", 1, true}};
+  for (uint32_t i = 0; i < 11; ++i)
     if (int rc = check_view(views, i, vw[i].name, vw[i].nd, *vw[i].w, vw[i].out)) return rc;
   long long distinct_;
   if (int rc = scalar_int(&sc[0], "distinct", distinct_)) return rc;
@@ -2258,11 +2268,13 @@ int op_verify_tree(g950_module* m, const g950_view* views, uint32_t nviews, cons
       last.v->dtype != G950_DTYPE_FLOAT32)
     return fail(G950_USAGE, "%s: count_ptr int32 [b], cu_seqlens_q_ptr int32 [b + 1], path_ptr int32 [b, most], next_ptr [b] "
                             "and uniform_next_ptr float32 [b] disagree", op);
-  for (const View* w : {&target, &draft, &tokens, &u, &last, &cu, &path})
+  if (ws.v->dtype != G950_DTYPE_FLOAT32) return fail(G950_USAGE, "%s: workspace_ptr must be float32", op);
+  if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
+  for (const View* w : {&target, &draft, &tokens, &u, &last, &cu, &path, &ws})
     if (int rc = last_contiguous(*w, op)) return rc;
-  for (const View* out : {&count, &next, &path}) {
+  for (const View* out : {&count, &next, &path, &ws}) {
     if (int rc = distinct(*out, op)) return rc;
-    for (const View* w : {&cu, &draft, &parent, &target, &tokens, &last, &u, &count, &next, &path})
+    for (const View* w : {&cu, &draft, &parent, &target, &tokens, &last, &u, &count, &next, &path, &ws})
       if (out != w)
         if (int rc = keep_apart(*out, *w, op)) return rc;
   }
@@ -2274,7 +2286,19 @@ int op_verify_tree(g950_module* m, const g950_view* views, uint32_t nviews, cons
   a.count_z = count.stride[0]; a.next_z = next.stride[0];
   a.T = (int)T; a.B = (int)B; a.V = (int)V; a.L = (int)L;
   a.token64 = tk == G950_DTYPE_INT64; a.distinct = distinct_ ? 1 : 0;
-  return launch(m, std::string("g950_verify_tree_") + rr_dtype(dt), (unsigned)B, 1024u, a, stream);
+  const std::string name = std::string("g950_verify_tree_") + rr_dtype(dt);
+  // as many parts as the workspace has places for
+  const long long room = (long long)ws.shape[0] * 4 - T * 16, want = verify_parts(m, B, V);
+  a.parts = (int)(B && room > 0 ? std::min(want, room / (B * VERIFY_TELL * 8)) : 1);
+  if (a.parts < 2) {
+    a.parts = 1;
+    if (B > (long long)max_grid(256)) return fail(G950_USAGE, "%s: grid too large", op);
+    return launch(m, name, (unsigned)B, 256u, a, stream);
+  }
+  a.px = (double*)ws.v->data;
+  a.told = (uint64_t*)(a.px + 2 * T);
+  if (int rc = launch(m, name + "_gather", (unsigned)B, 256u, a, stream)) return rc;
+  return launch(m, name + "_parts", (unsigned)(B * a.parts), 256u, a, stream);
 }
 
 int op_paged_keep_path(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar*, uint32_t nsc,
@@ -2594,6 +2618,11 @@ size_t g950_paged_attention_tree_workspace(g950_module* m, int64_t b, int64_t h,
     return 0;
   const TreeShape f = tree_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
   return (size_t)(f.parts * f.units * 32 * f.rw * (d + 2)) * 4;
+}
+
+size_t g950_verify_tree_workspace(g950_module* m, int64_t b, int64_t tokens, int64_t v) {
+  if (b <= 0 || tokens < 0 || v <= 0 || b > 0x7FFFFFF || tokens > 0x7FFFFFFF || v > 0x7FFFFFFF) return 0;
+  return verify_bytes(b, tokens, verify_parts(m, b, v));
 }
 
 int g950_sync(void* stream) {

@@ -17,162 +17,379 @@
 // sum_{w <= v} R(w) > r sum R; where nothing is left (S = 0), p's row itself is taken.  All sums are held in
 // 64 bits: a comparison falls otherwise than the formula's only where both sides agree
 // to 2^-45 or so.
+//
+// A test needs four numbers; a refusal needs its node's two rows, and the next test waits
+// for their sum: a chain of passes over one pair of rows after the other (a megabyte each at
+// 128000 tokens in fp32), which one CU streams at some 100 GB/s.  So a sequence's columns are cut into
+// `parts`, one workgroup each, all of which follow the path on their own and tell each other
+// their sums.
+//   * A sum is told in one 64-bit word, by a relaxed atomic, in a place of its own for every
+//     (sequence, round, part); the launch before empties the places (a pattern that no sum
+//     has).  So nothing else needs to be ordered, and a place is never written twice with
+//     different values.
+//   * A workgroup waits for a sum for a bounded time only, then adds up that part itself,
+//     in the same order, to the same bits: no workgroup depends on another one's being on
+//     the chip.  (After TELL rounds it adds up all of them.)
+//   * The part in which the random number's share falls belongs to one workgroup, which
+//     finds the token.
 namespace g950 {
 
-constexpr int VERIFY_THREADS = 1024, VERIFY_WAVES = VERIFY_THREADS / 64;
+constexpr int VERIFY_THREADS = 256, VERIFY_WAVES = VERIFY_THREADS / 64;
+constexpr int VERIFY_SPINS = 64;  // looks at what others tell, about a microsecond each
+constexpr uint64_t VERIFY_EMPTY = ~0ull;
 
+// 16 bytes of a row, which may begin at any element
+typedef u32x4 __attribute__((aligned(4))) verify_word4;
+typedef u32x4 __attribute__((aligned(2))) verify_word2;
 // a probability: below zero and NaN count as none
+__device__ __forceinline__ double verify_value(float x) { return (double)fmaxf(x, 0.0f); }
+__device__ __forceinline__ double verify_value(bf16_t x) { return verify_value(bf16_to_f32(x.bits)); }
+__device__ __forceinline__ double verify_value(f16_t x) { return verify_value(f16_to_f32(x.bits)); }
 template <typename T>
-__device__ __forceinline__ double verify_value(T x) {
-  if constexpr (std::is_same_v<T, float>) return fmax((double)x, 0.0);
-  else if constexpr (std::is_same_v<T, bf16_t>) return fmax((double)bf16_to_f32(x.bits), 0.0);
-  else return fmax((double)f16_to_f32(x.bits), 0.0);
+__device__ __forceinline__ double verify_element(const u32x4& w, int e) {
+  if constexpr (sizeof(T) == 4) return verify_value(__uint_as_float(w[e]));
+  else return verify_value(T{(uint16_t)(w[e / 2] >> (16 * (e & 1)))});
 }
 
-__device__ __forceinline__ double verify_shfl_up(double v, int by) { return __shfl_up(v, by); }
+// sums of `v` over the lanes up to the own one
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double verify_dpp(double v) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)w, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(w >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double verify_scan(double v) {
+  v += verify_dpp<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += verify_dpp<0x112, 0xF>(v);
+  v += verify_dpp<0x114, 0xF>(v);
+  v += verify_dpp<0x118, 0xF>(v);
+  v += verify_dpp<0x142, 0xA>(v);  // row_bcast 15, 31
+  v += verify_dpp<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ double verify_lane(double v, int lane) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)w, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(w >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 
-// One workgroup per sequence.
+// A node's token and its probabilities after its parent.
 template <typename T>
+__device__ __forceinline__ void verify_node(const VerifyArgs& a, int b0, int i, int& p, int& x, double& px, double& qx) {
+  p = a.parent[b0 + i];
+  p = i > 0 && p >= 0 && p < i ? p : -1;
+  const long long t = a.token64 ? ((const long long*)a.tokens)[b0 + i] : ((const int*)a.tokens)[b0 + i];
+  const bool in = p >= 0 && t >= 0 && t < a.V;
+  x = in ? (int)t : -1;
+  px = in ? verify_value(((const T*)a.target)[(b0 + p) * a.t_row + t]) : 0.0;
+  qx = !a.draft ? 1.0 : in ? verify_value(((const T*)a.draft)[(b0 + p) * a.d_row + t]) : 0.0;
+}
+__device__ __forceinline__ int verify_nodes(const VerifyArgs& a, int z, int& b0) {
+  b0 = a.cu[z];
+  const int b1 = a.cu[z + 1];
+  return b0 >= 0 && b1 >= b0 && b1 <= a.T ? min(b1 - b0, TREE_NODES) : 0;
+}
+
+// The launch before the parts': every node's probabilities side by side, and the places of the sums
+// empty.
+template <typename T>
+__device__ __forceinline__ void verify_gather_body(const VerifyArgs& a) {
+  const int z = blockIdx.x;
+  uint64_t* told = a.told + (long long)z * VERIFY_TELL * a.parts;
+  for (int i = threadIdx.x; i < VERIFY_TELL * a.parts; i += 256) told[i] = VERIFY_EMPTY;
+  int b0;
+  const int n = verify_nodes(a, z, b0);
+  for (int i = threadIdx.x; i < n; i += 256) {
+    int p, x;
+    verify_node<T>(a, b0, i, p, x, a.px[2 * (long long)(b0 + i)], a.px[2 * (long long)(b0 + i) + 1]);
+  }
+}
+
+// PARTS: a.parts workgroups per sequence, behind verify_gather; else one.
+template <typename T, bool PARTS>
 __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
+  using W = std::conditional_t<sizeof(T) == 4, verify_word4, verify_word2>;
+  constexpr int N = 16 / (int)sizeof(T);
   __shared__ double px[TREE_NODES], qx[TREE_NODES];
   __shared__ float us[TREE_NODES];
   __shared__ int tok[TREE_NODES], gone[TREE_NODES];
   __shared__ short par[TREE_NODES];
-  __shared__ double seg[VERIFY_WAVES + 1];
-  __shared__ int found;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int z = blockIdx.x;
-  const int b0 = a.cu[z], b1 = a.cu[z + 1];
-  const int n = b0 >= 0 && b1 >= b0 && b1 <= a.T ? min(b1 - b0, TREE_NODES) : 0;
+  __shared__ double seg[VERIFY_WAVES], other[VERIFY_WAVES], scan[VERIFY_WAVES];
+  __shared__ double upto[64];  // sum of the parts up to and with the one
+  __shared__ unsigned long long missing;
+  __shared__ int found, some;
+  if (blockDim.x != VERIFY_THREADS) return;  // launch shape must match the kernel
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int parts = PARTS ? a.parts : 1;
+  const int z = blockIdx.x / (unsigned)parts, part = blockIdx.x % (unsigned)parts;
+  int b0;
+  const int n = verify_nodes(a, z, b0);
   int* path = a.path + z * a.path_z;
+  auto answer = [&](int token) {
+    if (a.token64) ((long long*)a.next)[z * a.next_z] = token;
+    else ((int*)a.next)[z * a.next_z] = token;
+  };
   if (n == 0) {
+    if (part) return;
     for (int i = tid; i < a.L; i += VERIFY_THREADS) path[i] = -1;
     if (tid == 0) {
       a.count[z * a.count_z] = 0;
-      if (a.token64) ((long long*)a.next)[z * a.next_z] = -1;
-      else ((int*)a.next)[z * a.next_z] = -1;
+      answer(-1);
     }
     return;
   }
   const T* P = (const T*)a.target;
   const T* Q = (const T*)a.draft;
-  // every node's token, its probability after its parent and there in the draft
   for (int i = tid; i < n; i += VERIFY_THREADS) {
-    int p = a.parent[b0 + i];
-    p = i > 0 && p >= 0 && p < i ? p : -1;
-    const long long x = a.token64 ? ((const long long*)a.tokens)[b0 + i] : ((const int*)a.tokens)[b0 + i];
-    const bool in = p >= 0 && x >= 0 && x < a.V;
+    int p, x;
+    if constexpr (PARTS) {
+      p = a.parent[b0 + i];
+      p = i > 0 && p >= 0 && p < i ? p : -1;
+      const long long t = a.token64 ? ((const long long*)a.tokens)[b0 + i] : ((const int*)a.tokens)[b0 + i];
+      x = p >= 0 && t >= 0 && t < a.V ? (int)t : -1;
+      px[i] = a.px[2 * (long long)(b0 + i)];
+      qx[i] = a.px[2 * (long long)(b0 + i) + 1];
+    } else {
+      verify_node<T>(a, b0, i, p, x, px[i], qx[i]);
+    }
     par[i] = (short)p;
-    tok[i] = in ? (int)x : -1;
+    tok[i] = x;
     us[i] = a.u[b0 + i];
-    px[i] = in ? verify_value(P[(b0 + p) * a.t_row + x]) : 0.0;
-    qx[i] = !Q ? 1.0 : in ? verify_value(Q[(b0 + p) * a.d_row + x]) : 0.0;
   }
   __syncthreads();
-  int cur = 0, count = 1, refused = 0;
+
+  int cur = 0, count = 1, refused = 0, round = 0;
   double A = 0.0, S = 1.0, rest = 1.0;
-  // what is left of column v
-  auto left = [&](const T* pr, const T* qr, int v) {
-    double r = verify_value(pr[v]);
-    if (qr) return fmax(r - A * verify_value(qr[v]), 0.0);
-    for (int k = 0; k < refused; ++k) r = gone[k] == v ? 0.0 : r;
-    return r;
+  // N columns of a row from v on: near its end the last N, of which cover() says which are
+  // columns v .. end - 1 (a row of fewer: element by element)
+  auto place = [&](long long v) { return max(min(v, (long long)a.V - N), 0ll); };
+  auto read = [&](const T* row, long long v) {
+    if (a.V >= N) return u32x4(*(const W*)(row + place(v)));
+    u32x4 w = {0, 0, 0, 0};
+    for (int e = 0; e < a.V; ++e) {
+      if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(row[e]);
+      else w[e / 2] |= (uint32_t)row[e].bits << (16 * (e & 1));
+    }
+    return w;
   };
-  const int per = (a.V + VERIFY_WAVES - 1) / VERIFY_WAVES;  // columns of a wave
-  // seg[w]: what is left in the columns of the waves before w
+  auto cover = [&](long long v, long long end) {
+    const int n = (int)max(min(end - v, (long long)N), 0ll);
+    return n ? ((1u << n) - 1) << (int)(v - place(v)) : 0u;
+  };
+  // what is left of them
+  auto left = [&](const u32x4& wp, const u32x4& wq, long long v, long long end, double (&r)[N]) {
+    const uint32_t in = cover(v, end);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      r[e] = verify_element<T>(wp, e);
+      if (Q) r[e] = fmax(fma(-A, verify_element<T>(wq, e), r[e]), 0.0);
+    }
+    if (!Q)
+      for (int k = 0; k < refused; ++k) {
+        const long long at = gone[k] - place(v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) r[e] = at == e ? 0.0 : r[e];
+      }
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = in >> e & 1 ? r[e] : 0.0;
+  };
+  // columns of a part, and of a wave of it: whole vectors
+  const long long len = ((a.V + parts - 1) / parts + N - 1) / N * N;
+  const long long share = ((len + VERIFY_WAVES - 1) / VERIFY_WAVES + N - 1) / N * N;
+  auto bounds = [&](int of, int w, long long& from, long long& to) {
+    const long long end = min((of + 1) * len, (long long)a.V);
+    from = min(of * len + w * share, end);
+    to = min(from + share, end);
+  };
+  // what is left of the node's row: S, and upto[] and seg[] as well.  (One place in the code
+  // for all of it: code that runs a few times is bound by being fetched.)
   auto sum = [&]() {
     const T* pr = P + (long long)(b0 + cur) * a.t_row;
-    const T* qr = Q && A > 0.0 ? Q + (long long)(b0 + cur) * a.d_row : nullptr;
-    const long long end = min((long long)(wave + 1) * per, (long long)a.V);
-    double s = 0.0;
-    for (long long v = (long long)wave * per + lane; v < end; v += 64) s += left(pr, qr, (int)v);
-    for (int k = 32; k; k >>= 1) s += __shfl_xor(s, k);
-    __syncthreads();
-    if (lane == 0) seg[wave + 1] = s;
-    __syncthreads();
-    if (tid == 0) {
-      seg[0] = 0.0;
-      for (int w = 0; w < VERIFY_WAVES; ++w) seg[w + 1] += seg[w];
-    }
-    __syncthreads();
-    return seg[VERIFY_WAVES];
-  };
-  bool known = false;  // seg holds the sums of this node with this A
-  for (int i = 1; i < n && count < a.L; ++i) {
-    if (par[i] != cur) continue;
-    double r = Q ? fmax(px[i] - A * qx[i], 0.0) : px[i];
-    if (!Q)
-      for (int k = 0; k < refused; ++k) r = gone[k] == tok[i] ? 0.0 : r;
-    if ((double)us[i] * qx[i] * S < r * rest) {
-      if (tid == 0) path[count] = i;
-      ++count;
-      cur = i;
-      refused = 0;
-      A = 0.0;
-      S = rest = 1.0;
-      known = false;
-    } else if (Q) {
-      A += S / rest;
-      S = sum();
-      known = true;
-      if (a.distinct) rest = fmax(rest - qx[i], 0x1p-24);
-    } else {
-      S -= r;
-      __syncthreads();
-      if (tid == 0) gone[refused] = tok[i];
-      ++refused;
-      __syncthreads();
-    }
-  }
-  double total = known ? S : sum();
-  if (!(total > 0.0)) {
-    A = 0.0;
-    refused = 0;
-    total = sum();
-  }
-  // the first column whose sum passes the random number's share
-  const double want = (double)a.last[z] * total;
-  int w = 0;
-  while (w + 1 < VERIFY_WAVES && !(seg[w + 1] > want)) ++w;
-  while (w > 0 && !(seg[w + 1] > seg[w])) --w;  // (a share past the end)
-  const T* pr = P + (long long)(b0 + cur) * a.t_row;
-  const T* qr = Q && A > 0.0 ? Q + (long long)(b0 + cur) * a.d_row : nullptr;
-  if (tid == 0) found = -1;
-  __syncthreads();
-  if (wave == 0) {
-    double before = seg[w];
-    const long long end = min((long long)(w + 1) * per, (long long)a.V);
-    int some = -1, hit = -1;  // last column with something left; the one wanted
-    for (long long v0 = (long long)w * per; v0 < end && hit < 0; v0 += 64) {
-      const long long v = v0 + lane;
-      const double r = v < end ? left(pr, qr, (int)v) : 0.0;
-      double s = r;
-      for (int k = 1; k < 64; k <<= 1) {
-        const double t = __shfl_up(s, k);
-        s += lane >= k ? t : 0.0;
+    const T* qr = Q + (long long)(b0 + cur) * a.d_row;
+    const bool both = Q && A > 0.0;
+    uint64_t todo = 1ull << part;
+    for (bool own = true; todo; own = false) {
+      const int of = __ffsll((unsigned long long)todo) - 1;
+      todo &= todo - 1;
+      // the waves' sums of the part
+      long long from, end;
+      bounds(of, wave, from, end);
+      double t = 0.0;
+      constexpr int U = 4;  // vectors of each row in flight
+#pragma unroll 1
+      for (long long v0 = from + lane * N; v0 - lane * N < end; v0 += 64 * N * U) {
+        u32x4 wp[U], wq[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          wp[u] = read(pr, v0 + 64 * N * u);
+          wq[u] = both ? read(qr, v0 + 64 * N * u) : (u32x4){0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          double r[N];
+          left(wp[u], wq[u], v0 + 64 * N * u, end, r);
+#pragma unroll
+          for (int e = 0; e < N; ++e) t += r[e];
+        }
       }
-      const uint64_t over = __ballot(r > 0.0 && before + s > want), any = __ballot(r > 0.0);
-      if (over) hit = (int)v0 + __ffsll((unsigned long long)over) - 1;
-      if (any) some = (int)v0 + 63 - __clzll((long long)any);
-      before += __shfl(s, 63);
+      t = verify_lane(verify_scan(t), 63);
+      __syncthreads();  // (whoever read the sums before is done)
+      if (lane == 0) (own ? seg : other)[wave] = t;
+      __syncthreads();
+      if (wave == 0) {
+        double t = 0.0;
+#pragma unroll
+        for (int w = 0; w < VERIFY_WAVES; ++w) t += (own ? seg : other)[w];
+        if (lane == 0) upto[of] = t;
+        if (PARTS && own) {
+          // told, and the others' taken
+          uint64_t* told = a.told + ((long long)z * VERIFY_TELL + round) * parts;
+          const bool tell = round < VERIFY_TELL;
+          if (tell && lane == 0)
+            __hip_atomic_store(told + part, __builtin_bit_cast(uint64_t, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          bool have = lane == part || lane >= parts;
+          for (int spin = 0; tell && spin < VERIFY_SPINS && !__all(have); ++spin) {
+            if (!have) {
+              const uint64_t w = __hip_atomic_load(told + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              have = w != VERIFY_EMPTY;
+              if (have) upto[lane] = __builtin_bit_cast(double, w);
+            }
+            __builtin_amdgcn_s_sleep(1);
+          }
+          const uint64_t none = __ballot(!have);
+          if (lane == 0) missing = none;
+        }
+      }
+      if (PARTS && own) {
+        __syncthreads();
+        todo = missing;
+      }
     }
-    if (lane == 0) found = hit >= 0 ? hit : some >= 0 ? some : 0;
+    ++round;
+    __syncthreads();
+    if (wave == 0) {
+      const double t = verify_scan(lane < parts ? upto[lane] : 0.0);
+      if (lane < parts) upto[lane] = t;
+    }
+    __syncthreads();
+    S = upto[parts - 1];
+  };
+
+  int at = 1;         // nodes before it are done with
+  bool walk = true;   // the path goes on
+  bool known = false; // S, seg and upto are those of this node with this A
+  for (;;) {
+    while (walk) {
+      // the next child of the node, 64 nodes at a time
+      int i = n;
+      for (int k = at & ~63; k < n && i == n && count < a.L; k += 64) {
+        const uint64_t kids = __ballot(k + lane < n && k + lane >= at && par[k + lane] == cur);
+        if (kids) i = k + __ffsll((unsigned long long)kids) - 1;
+      }
+      if (i == n) {
+        walk = false;
+        break;
+      }
+      at = i + 1;
+      double r = Q ? fmax(fma(-A, qx[i], px[i]), 0.0) : px[i];
+      for (int k = 0; k < refused; ++k) r = gone[k] == tok[i] ? 0.0 : r;
+      if ((double)us[i] * qx[i] * S < r * rest) {
+        if (tid == 0 && part == 0) path[count] = i;
+        ++count;
+        cur = i;
+        refused = 0;
+        A = 0.0;
+        S = rest = 1.0;
+        known = false;
+      } else if (Q) {
+        A += S / rest;
+        if (a.distinct) rest = fmax(rest - qx[i], 0x1p-24);
+        known = false;
+        break;
+      } else {
+        S -= r;
+        __syncthreads();
+        if (tid == 0) gone[refused] = tok[i];
+        ++refused;
+        __syncthreads();
+      }
+    }
+    if (!walk && known) {
+      if (S > 0.0 || (A == 0.0 && refused == 0)) break;
+      A = 0.0;  // nothing left: p itself
+      refused = 0;
+    }
+    sum();
+    known = true;
   }
+  if (part == 0) {
+    for (int i = count + tid; i < a.L; i += VERIFY_THREADS) path[i] = -1;
+    if (tid == 0) {
+      path[0] = 0;
+      a.count[z * a.count_z] = count;
+    }
+  }
+  // the first column whose sum passes the random number's share: its part (where none
+  // does, the last with something left; part 0 of nothing), its wave, its column
+  const double want = (double)a.last[z] * S;
+  const double mine = upto[min(lane, parts - 1)], below = lane ? upto[min(lane, parts) - 1] : 0.0;
+  const uint64_t over = __ballot(lane < parts && mine > want), some_left = __ballot(lane < parts && mine > below);
+  const int of = over ? __ffsll((unsigned long long)over) - 1 : some_left ? 63 - __clzll((long long)some_left) : 0;
+  if (of != part) return;
+  double before = verify_lane(below, of);
+  int w = 0;
+  while (w + 1 < VERIFY_WAVES && !(before + seg[w] > want)) before += seg[w++];
+  while (w > 0 && !(seg[w] > 0.0)) before -= seg[--w];  // (a share past the end)
+  long long from, end;
+  bounds(part, w, from, end);
+  const T* pr = P + (long long)(b0 + cur) * a.t_row;
+  const T* qr = Q + (long long)(b0 + cur) * a.d_row;
+  if (tid == 0) found = 0x7FFFFFFF, some = -1;
   __syncthreads();
-  for (int i = count + tid; i < a.L; i += VERIFY_THREADS) path[i] = -1;
-  if (tid == 0) {
-    path[0] = 0;
-    a.count[z * a.count_z] = count;
-    if (a.token64) ((long long*)a.next)[z * a.next_z] = found;
-    else ((int*)a.next)[z * a.next_z] = found;
+  for (long long v0 = from; v0 < end; v0 += VERIFY_THREADS * N) {
+    const long long v = v0 + tid * N;
+    double r[N], s = 0.0;
+    const u32x4 none = {0, 0, 0, 0};
+    left(read(pr, v), Q && A > 0.0 ? read(qr, v) : none, v, end, r);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += r[e];
+    const double t = verify_scan(s);
+    if (lane == 63) scan[wave] = t;
+    __syncthreads();
+    double mine = before + (t - s);
+#pragma unroll
+    for (int k = 0; k < VERIFY_WAVES; ++k) mine += k < wave ? scan[k] : 0.0;
+    int hit = -1, any = -1;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      mine += r[e];
+      if (r[e] > 0.0) {
+        any = (int)(place(v) + e);
+        if (hit < 0 && mine > want) hit = any;
+      }
+    }
+    if (hit >= 0) atomicMin(&found, hit);
+    if (any >= 0) atomicMax(&some, any);
+#pragma unroll
+    for (int k = 0; k < VERIFY_WAVES; ++k) before += scan[k];
+    __syncthreads();
+    if (found != 0x7FFFFFFF) break;
   }
+  if (tid == 0) answer(found != 0x7FFFFFFF ? found : some >= 0 ? some : 0);
 }
 
 }  // namespace g950
 
-#define G950_VERIFY(TNAME, T)                                                                                 \
-  extern "C" __global__ __launch_bounds__(1024) void g950_verify_tree_##TNAME(const g950::VerifyArgs a) {    \
-    g950::verify_tree_body<T>(a);                                                                             \
+#define G950_VERIFY(TNAME, T)                                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void g950_verify_tree_##TNAME(const g950::VerifyArgs a) {        \
+    g950::verify_tree_body<T, false>(a);                                                                          \
+  }                                                                                                               \
+  extern "C" __global__ __launch_bounds__(256) void g950_verify_tree_##TNAME##_parts(const g950::VerifyArgs a) { \
+    g950::verify_tree_body<T, true>(a);                                                                           \
+  }                                                                                                               \
+  extern "C" __global__ __launch_bounds__(256) void g950_verify_tree_##TNAME##_gather(const g950::VerifyArgs a) { \
+    g950::verify_gather_body<T>(a);                                                                               \
   }
 G950_VERIFY(f32, float)
 G950_VERIFY(bf16, g950::bf16_t)

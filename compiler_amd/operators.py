@@ -336,8 +336,8 @@ def paged_attention_tree_kernel(q_ptr, k_cache_ptr, v_cache_ptr, page_table_ptr,
 
 
 def verify_tree_kernel(target_probs_ptr, draft_probs_ptr, tokens_ptr, parent_ptr, uniform_ptr, uniform_next_ptr,
-                       cu_seqlens_q_ptr, path_ptr, count_ptr, next_ptr, distinct, *, stream=None, sync=False,
-                       prepare=False):
+                       cu_seqlens_q_ptr, path_ptr, count_ptr, next_ptr, workspace_ptr, distinct, *, stream=None,
+                       sync=False, prepare=False):
     """Drafted trees verified against the target's probabilities
     (G950_OP_VERIFY_TREE; no reference counterpart): probabilities [tokens, v]
     after each node (draft: those that its children were drawn from, or empty), tokens and
@@ -345,9 +345,9 @@ def verify_tree_kernel(target_probs_ptr, draft_probs_ptr, tokens_ptr, parent_ptr
     [b] and the next token [b] come out."""
     return _launch_sorted(rt.OP_VERIFY_TREE,
                           (count_ptr, cu_seqlens_q_ptr, draft_probs_ptr, next_ptr, parent_ptr, path_ptr, target_probs_ptr,
-                           tokens_ptr, uniform_next_ptr, uniform_ptr),
-                          (True, False, False, True, False, True, False, False, False, False), (distinct,), stream, sync,
-                          prepare)
+                           tokens_ptr, uniform_next_ptr, uniform_ptr, workspace_ptr),
+                          (True, False, False, True, False, True, False, False, False, False, True), (distinct,), stream,
+                          sync, prepare)
 
 
 def paged_keep_path_kernel(k_cache_ptr, v_cache_ptr, page_table_ptr, cu_seqlens_q_ptr, seqused_k_ptr, path_ptr, count_ptr,
@@ -612,11 +612,12 @@ def paged_attention_tree(q, k_cache, v_cache, page_table, cu_seqlens_q, seqused_
 
 
 def verify_tree(target_probs, draft_probs, tokens, parent, uniform, uniform_next, cu_seqlens_q, most, distinct=False,
-                path=None, count=None, next_token=None, **kw):
+                path=None, count=None, next_token=None, workspace=None, **kw):
     """Drafted trees verified (verify_tree_kernel); draft_probs None: the drafts were
     chosen, not drawn; ``distinct``: siblings were drawn without replacement.  Returns
     path [b, most] (the accepted nodes, root first, then -1), count [b] and the
-    next token [b]."""
+    next token [b].  The workspace (float32) comes from torch's allocator, on the call's
+    stream, unless given."""
     import torch
     b, stream = cu_seqlens_q.shape[0] - 1, kw.get("stream")
     empty = torch.empty if stream is None else _on_stream(stream, torch.empty)
@@ -624,8 +625,10 @@ def verify_tree(target_probs, draft_probs, tokens, parent, uniform, uniform_next
     count = empty((b,), dtype=torch.int32, device=tokens.device) if count is None else count
     next_token = empty((b,), dtype=tokens.dtype, device=tokens.device) if next_token is None else next_token
     draft = _none(target_probs.dtype, target_probs.device, 2) if draft_probs is None else draft_probs
+    if workspace is None:
+        workspace = _workspace(rt.module().verify_tree_workspace(b, tokens.shape[0], target_probs.shape[1]), tokens, stream)
     verify_tree_kernel(target_probs, draft, tokens, parent, uniform, uniform_next, cu_seqlens_q, path, count, next_token,
-                       bool(distinct), **kw)
+                       workspace, bool(distinct), **kw)
     return path, count, next_token
 
 

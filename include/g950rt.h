@@ -292,8 +292,9 @@ typedef struct g950_scalar {
  *           draft_probs_ptr[T,V] or empty, next_ptr[B], parent_ptr i32[T], path_ptr
  *           i32[B,most] (the path's nodes, root first, then -1), target_probs_ptr[T,V]
  *           f32 | bf16 | f16 (draft the same), tokens_ptr[T] i32 | i64 (next the same),
- *           uniform_next_ptr f32[B], uniform_ptr f32[T].  A sequence without nodes: count 0,
- *           path and next -1
+ *           uniform_next_ptr f32[B], uniform_ptr f32[T], workspace_ptr f32 (1-D, 16-byte
+ *           aligned, any length: g950_verify_tree_workspace gives the one that serves all; calls
+ *           that may overlap need one each).  A sequence without nodes: count 0, path and next -1
  *   scalars distinct
  * G950_OP_PAGED_KEEP_PATH  the path's rows moved to where its tokens belong: cache row base
  *                      + i gets what row base + path[b,i] held, for i < count[b] and i <=
@@ -395,6 +396,10 @@ size_t g950_paged_attention_int4_workspace(g950_module *module, int64_t b, int64
  * seqlen_k keys. */
 size_t g950_paged_attention_tree_workspace(g950_module *module, int64_t b, int64_t h, int64_t hk, int64_t d,
                                            int64_t seqlen_q, int64_t seqlen_k);
+
+/* Bytes of workspace_ptr with which G950_OP_VERIFY_TREE has a sequence's columns
+ * added up by as many workgroups as pays: b trees of `tokens` nodes in all, v columns. */
+size_t g950_verify_tree_workspace(g950_module *module, int64_t b, int64_t tokens, int64_t v);
 
 /* Run every contract check and the kernel choice of g950_launch without
  * touching a device (no module, no HIP call).  On success

@@ -41,13 +41,14 @@ def attend(t=7, h=8, hk=2, d=128, pages=9, bs=16, b=3, dt=BF, scale=0.1, sk=64, 
     return call(rt.OP_PAGED_ATTENTION_TREE, v, [scale, sk, sq, left], change, {"o_ptr", "softmax_lse_ptr", "workspace_ptr"})
 
 
-def verify(t=9, vocab=100, b=3, most=5, dt=F32, tk=I64, drawn=True, **change):
+def verify(t=9, vocab=100, b=3, most=5, dt=F32, tk=I64, drawn=True, ws=0, **change):
     v = {"count_ptr": dict(shape=[b], dtype=I32), "cu_seqlens_q_ptr": dict(shape=[b + 1], dtype=I32),
          "draft_probs_ptr": dict(shape=[t, vocab] if drawn else [0, 0], dtype=dt), "next_ptr": dict(shape=[b], dtype=tk),
          "parent_ptr": dict(shape=[t], dtype=I32), "path_ptr": dict(shape=[b, most], dtype=I32),
          "target_probs_ptr": dict(shape=[t, vocab], dtype=dt), "tokens_ptr": dict(shape=[t], dtype=tk),
-         "uniform_next_ptr": dict(shape=[b], dtype=F32), "uniform_ptr": dict(shape=[t], dtype=F32)}
-    return call(rt.OP_VERIFY_TREE, v, [False], change, {"count_ptr", "next_ptr", "path_ptr"})
+         "uniform_next_ptr": dict(shape=[b], dtype=F32), "uniform_ptr": dict(shape=[t], dtype=F32),
+         "workspace_ptr": dict(shape=[ws], dtype=F32)}
+    return call(rt.OP_VERIFY_TREE, v, [False], change, {"count_ptr", "next_ptr", "path_ptr", "workspace_ptr"})
 
 
 def keep(b=3, pages=9, bs=16, hk=2, d=128, most=5, dt=BF, layers=None, **change):
@@ -128,6 +129,14 @@ def test_verify():
     refused(verify(path_ptr=dict(output=False)), rt.REJECTED, "output flag")
     refused(verify(path_ptr=dict(over="count_ptr")), rt.USAGE, "overlaps")
     refused(verify(parent_ptr=dict(over="next_ptr")), rt.USAGE, "overlaps")
+    refused(verify(ws=64, workspace_ptr=dict(over="uniform_ptr")), rt.USAGE, "overlaps")
+    refused(verify(workspace_ptr=dict(dtype=BF)), rt.USAGE, "float32")
+    refused(verify(ws=64, workspace_ptr=dict(offset=1)), rt.USAGE, "16-byte")
+    # as many workgroups as the workspace has places for
+    assert verify(vocab=50000)[1] == "g950_verify_tree_f32"
+    assert verify(vocab=50000, ws=9 * 4 + 3 * 64 * 2 - 1)[1] == "g950_verify_tree_f32"
+    assert verify(vocab=50000, ws=9 * 4 + 3 * 64 * 2)[1] == "g950_verify_tree_f32_parts"
+    assert verify(vocab=1000, ws=1 << 20)[1] == "g950_verify_tree_f32"
 
 
 def test_keep():
@@ -154,7 +163,7 @@ def test_keep():
 
 
 @pytest.mark.parametrize("op,nv,ns", [(rt.OP_PAGED_APPEND_TREE, 12, 1), (rt.OP_PAGED_ATTENTION_TREE, 10, 4),
-                                      (rt.OP_VERIFY_TREE, 10, 1), (rt.OP_PAGED_KEEP_PATH, 8, 0)])
+                                      (rt.OP_VERIFY_TREE, 11, 1), (rt.OP_PAGED_KEEP_PATH, 8, 0)])
 def test_arity(op, nv, ns):
     for v, s in ((nv - 1, ns), (nv, ns + 1)):
         a = Args()

@@ -431,6 +431,31 @@ def test_verify_seeds(drafts):
     assert lengths >= {0, 1, 2, 3}
 
 
+@pytest.mark.parametrize("drafts", ["drawn", "distinct", "chosen"])
+def test_verify_any_workspace(drafts):
+    """One workgroup a sequence, several and as many as are wanted: the same answers."""
+    for case in ("large", "odd_large"):
+        c = verify_case(case, drafts, "bfloat16", seed=1)
+        t, b = c["target"].shape[0], len(c["ql"])
+        for parts in (0, 1, 2, 7, 64):
+            ws = torch.full((t * 4 + b * 64 * parts,), float("nan"), device="cuda")
+            verify_check(c, verify_run(c, "bfloat16", workspace=ws))
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_verify_many_refusals(dt):
+    """A root with 90 children, nearly all of them refused: more sums than the workgroups tell each
+    other, the rest each adds up by itself."""
+    VERIFY["refused"] = dict(ql=[91, 60], v=9000, kinds=["star"])
+    c = verify_case("refused", "drawn", dt, seed=2)
+    c["u"][:] = 1 - 2.0 ** -24
+    for ws in (None, torch.empty(0, device="cuda")):
+        got = verify_run(c, dt, workspace=ws)
+        verify_check(c, got)
+    c["tokens"][1:80] = int(c["target"][0].argmin())
+    verify_check(c, verify_run(c, dt))
+
+
 @pytest.mark.parametrize("most", [1, 2, 3])
 def test_verify_full_paths(most):
     for drafts in ("drawn", "chosen"):
