@@ -143,7 +143,6 @@ __device__ __forceinline__ void attn_tree_general_body(const AttnTreeArgs& p) {
 //   * What a row does not see may hold anything: scores are replaced, and where V of a
 //     stage that some row does not see whole is not finite, 0 V would not be 0: such values
 //     are added, key by key, where a row sees them, and taken out of the stage.
-constexpr int TREE_MIN_TILES = 4;  // of a part
 
 struct TreeSpan {
   TreeSeq sq;
@@ -172,9 +171,8 @@ __device__ __forceinline__ int tree_scan(int v) {
 }
 
 // How the batch's keys are dealt: every sequence's tiles are cut into parts of c (the last
-// one shorter), c so that all sequences together have at most p.parts parts; no sequence has
-// more than 64.  The lengths live on the device, so each wave works this out, 64
-// sequences at a time: a batch of different lengths becomes parts of one length, and as
+// one shorter), c so that all sequences together have at most p.parts parts.  The lengths
+// live on the device, so each wave works this out, 64 sequences at a time: a batch of different lengths becomes parts of one length, and as
 // many as the chip has places for.
 struct TreeDeal {
   const AttnTreeArgs& p;
@@ -188,14 +186,12 @@ struct TreeDeal {
   __device__ __forceinline__ explicit TreeDeal(const AttnTreeArgs& args) : p(args) {
     n0 = tiles(0);
     long long sum = 0;
-    int most = 0;
     for (int z0 = 0; z0 < p.B; z0 += 64) {
       const int n = tiles_again(z0);
       sum += __builtin_amdgcn_readlane(tree_scan(n), 63);
-      most = max(most, (int)wave_reduce<OpMax>((float)n));  // (rounded: a 64th of it is all that is used)
     }
     const int room = p.parts - p.B;
-    c = max(max((int)((sum + room - 1) / room), most / 63 + 1), TREE_MIN_TILES);
+    c = max((int)((sum + room - 1) / room), p.min_tiles);
   }
   // the sequence that part `part` belongs to, and the parts before that sequence; -1: none
   __device__ __forceinline__ int sequence(int part, int& before) const {
@@ -289,7 +285,7 @@ struct TreeCfg {
   static constexpr int SUB = KW == 1 ? 2 : 1;           // 32-key tiles of a wave in a stage
   static constexpr int TKS = 32 * KW * SUB;             // keys of a stage
   static constexpr int ROW = 2 * D, KT = TKS * ROW, STAGE = 2 * KT;
-  static constexpr int NS = STAGE <= 16384 && RW < 4 ? 4 : 2;
+  static constexpr int NS = 2;
   static constexpr int ROWS = 32 * RW;
   static constexpr int LDS = NS * STAGE;
   static_assert(LDS >= 4 * 32 * D * 4, "the waves' partial O fits the ring");
@@ -559,7 +555,7 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     __syncthreads();
   };
 
-  if constexpr (RW == 4 && D < 256) {
+  if constexpr (D < 256) {
     // Bound by the matrix cores and the vector ALU beside the bytes.  Iteration i: V of
     // stage i and K of i + 1 have landed; softmax of stage i, then its V and the next
     // stage's scores in one run of MFMAs at raised priority, whose operand reads are issued ahead
@@ -568,13 +564,14 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     auto kat = [&](int i) { return (uint32_t)(i & 1) * KT; };
     auto vat = [&](int i) { return (uint32_t)(2 + (i & 1)) * KT; };
     constexpr int R = 2 * DB, NV = 2 * SUB, NK = SUB * DS;
+    const uint32_t own = kw * 32 * SUB * ROW;  // this wave's keys of a stage
     u32x2 vt[2][R];
     u32x4 kf[8];
     auto vread_ = [&](auto ic, uint32_t slot) {  // group I: V of keys 16 I .. + 15
       constexpr int I = decltype(ic)::value;
       static_for<R>([&](auto qc) {
         constexpr int Q = decltype(qc)::value;
-        lds_rdtr<(16 * I + 8 * (Q & 1)) * ROW>(vt[I & 1][Q], ring32 + slot + vread + (((Q >> 1) << 6) ^ vx));
+        lds_rdtr<(16 * I + 8 * (Q & 1)) * ROW>(vt[I & 1][Q], ring32 + slot + own + vread + (((Q >> 1) << 6) ^ vx));
       });
     };
     auto vmma = [&](auto ic) {
@@ -588,7 +585,7 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     auto kread_ = [&](auto jc, uint32_t slot) {  // fragment J: tile J % SUB, k-step J / SUB
       constexpr int J = decltype(jc)::value;
       if constexpr (J < NK)
-        lds_rd128<(J % SUB) * 32 * ROW>(kf[J & 7], ring32 + slot + kread + (kx ^ ((J / SUB) << 5)));
+        lds_rd128<(J % SUB) * 32 * ROW>(kf[J & 7], ring32 + slot + own + kread + (kx ^ ((J / SUB) << 5)));
     };
     auto kahead = [&](uint32_t slot) { static_for<4>([&](auto jc) { kread_(jc, slot); }); };
     // O^T += V^T.P^T, with the first four fragments of the next K on the way (each wait
@@ -739,61 +736,91 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
   }
 }
 
-// Joins the parts of a block of rows: one wave per row, lane s holds part s's maximum and
-// sum (at most 64 parts), D / 64 outputs per lane.
-template <int D, bool F16, int ROWS>
+// Joins the parts of a block of rows, 16 bytes of a row per lane, U parts at a time: NW
+// waves per 256 / D rows, which take the parts in turn.
+template <int D, bool F16, int ROWS, int NW>
 __device__ __forceinline__ void attn_tree_merge_body(const AttnTreeArgs& p) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t id = item / (uint32_t)p.merge_rows, r = item % (uint32_t)p.merge_rows;
+  constexpr int LPR = D / 4, AT = 64 / LPR, U = 8;  // lanes of a row, rows of a wave
+  __shared__ float js[NW][64][6];
+  if (blockDim.x != (NW == 1 ? 256 : 64 * NW)) return;  // launch shape must match the kernel
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int nw = NW;
+  const int share = NW == 1 ? 0 : wave;
+  const uint32_t item = NW == 1 ? blockIdx.x * 4 + wave : blockIdx.x, groups = (p.merge_rows + AT - 1) / AT;
+  const uint32_t id = item / groups, r0 = item % groups * AT;
   const uint32_t heads = p.Hkv, units = heads * p.row_blocks, unit = id % units;
   const int z = id / units, hk = unit % heads, block = unit / heads;
   if (z >= p.B) return;
   const TreeDeal d(p);
   const TreeSpan sp = tree_span(p, z);
-  const int row = block * ROWS + r, count = (sp.n + d.c - 1) / d.c;
-  if (row >= sp.sq.nq * p.group || count <= 1) return;  // (one part: its workgroup had all of it)
-  constexpr int E = D / 64, U = 32 / E;
-  using vec = float __attribute__((ext_vector_type(E)));
+  const int rows = min(sp.sq.nq * p.group - block * ROWS, ROWS), count = (sp.n + d.c - 1) / d.c;
+  if ((int)r0 >= rows || count <= 1) return;  // (one part: its workgroup had all of it)
+  const int r = min((int)r0 + lane / LPR, rows - 1);
   const long long rec = ((long long)d.before(z) * units + unit) * ROWS + r, step = (long long)units * ROWS;
-  const float* part = p.part + rec * D + lane * E;
-  const float* pair_ml = p.ml + 2 * (rec + min(lane, count - 1) * step);
-  float m = pair_ml[0], l = pair_ml[1];
-  vec v[U];
-  auto load = [&](int s0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = *(const vec*)(part + min(s0 + u, count - 1) * step * D);
-  };
-  load(0);
-  if (lane >= count) {
-    m = -__builtin_huge_valf();
-    l = 0.0f;
-  }
-  const float mt = wave_reduce<OpMax>(m);
-  // no finite score in a part: nothing seen (O = l = 0), or only NaN, which stays
-  const float f = m == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(m - mt);
-  const float lt = wave_reduce<OpSum>(f * l);
-  vec acc = {};
-  for (int s0 = 0;;) {
+  const float* part = p.part + rec * D + lane % LPR * 4;
+  const float* pair = p.ml + 2 * rec;
+  float m = -__builtin_huge_valf(), l = 0.0f;
+  f32x4 acc = {};
+  for (int s0 = share; s0 < count; s0 += U * nw) {
+    f32x4 v[U];
+    f32x2 ml[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s0 + u, 63)));
-      if (s0 + u < count)
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(x, v[u][e], acc[e]);
+      const long long s = min(s0 + u * nw, count - 1) * step;
+      v[u] = *(const f32x4*)(part + s * D);
+      ml[u] = *(const f32x2*)(pair + s * 2);
     }
-    if ((s0 += U) >= count) break;
-    load(s0);
-  }
-  const int i = (uint32_t)row / (uint32_t)p.group, h = hk * p.group + (uint32_t)row % (uint32_t)p.group;
-  const bool empty = !(lt > 0.0f);  // zero or NaN
-  const float inv = empty ? 1.0f : 1.0f / lt;
-  uint16_t* dst = (uint16_t*)p.o + (long long)(sp.sq.q0 + i) * p.o_st + (long long)h * p.o_sh + lane * E;
+    float to = m;
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = F16 ? f32_to_f16(acc[e] * inv) : f32_to_bf16(acc[e] * inv);
-  if (lane == 0)
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * nw < count) to = fmaxf(to, ml[u][0]);
+    // no finite score so far, or in a part: nothing seen (O = l = 0), or only NaN, which stays
+    const float was = m == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    acc *= was;
+    l *= was;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * nw < count) {
+        const float f = ml[u][0] == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(ml[u][0] - to);
+        l = fmaf(f, ml[u][1], l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, v[u][e], acc[e]);
+      }
+    m = to;
+  }
+  if constexpr (NW > 1) {
+    float* mine = js[wave][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mine[e] = acc[e];
+    mine[4] = m;
+    mine[5] = l;
+    __syncthreads();
+    if (wave) return;
+    float to = m;
+#pragma unroll
+    for (int w = 1; w < NW; ++w) to = fmaxf(to, js[w][lane][4]);
+    acc = (f32x4){};
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float* x = js[w][lane];
+      const float f = x[4] == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(x[4] - to);
+      l = fmaf(f, x[5], l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+    }
+    m = to;
+  }
+  if ((int)r0 + lane / LPR >= rows) return;
+  const uint32_t row = block * ROWS + r, G = p.group;
+  const int i = row / G, h = hk * G + row % G;
+  const bool empty = !(l > 0.0f);  // zero or NaN
+  const float inv = empty ? 1.0f : 1.0f / l;
+  char* dst = (char*)p.o + 2 * ((long long)(sp.sq.q0 + i) * p.o_st + (long long)h * p.o_sh + lane % LPR * 4);
+  *(u32x2*)dst = (u32x2){pack2(acc[0] * inv, acc[1] * inv, F16), pack2(acc[2] * inv, acc[3] * inv, F16)};
+  if (lane % LPR == 0)
     p.lse[(long long)h * p.lse_h + (long long)(sp.sq.q0 + i) * p.lse_t] =
-        empty ? __builtin_huge_valf() : (mt + __log2f(lt)) * 0.69314718055994530942f;
+        empty ? __builtin_huge_valf() : (m + __log2f(l)) * 0.69314718055994530942f;
 }
 
 }  // namespace g950
@@ -801,13 +828,17 @@ __device__ __forceinline__ void attn_tree_merge_body(const AttnTreeArgs& p) {
 extern "C" __global__ __launch_bounds__(64) void g950_attn_tree_general(const g950::AttnTreeArgs p) {
   g950::attn_tree_general_body(p);
 }
+#define G950_TREE_MERGE(NAME, D, F16, RW, NW)                                                               \
+  extern "C" __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void NAME(const g950::AttnTreeArgs p) { \
+    g950::attn_tree_merge_body<D, F16, 32 * RW, NW>(p);                                                     \
+  }
 #define G950_TREE(NAME, D, F16, RW, PER_CU)                                                                 \
   extern "C" __global__ __launch_bounds__(256, PER_CU) void NAME##_r##RW(const g950::AttnTreeArgs p) {      \
     g950::attn_tree_body<D, F16, RW>(p);                                                                    \
   }                                                                                                         \
-  extern "C" __global__ __launch_bounds__(256) void NAME##_r##RW##_merge(const g950::AttnTreeArgs p) {      \
-    g950::attn_tree_merge_body<D, F16, 32 * RW>(p);                                                         \
-  }
+  G950_TREE_MERGE(NAME##_r##RW##_merge1, D, F16, RW, 1)                                                      \
+  G950_TREE_MERGE(NAME##_r##RW##_merge4, D, F16, RW, 4)                                                      \
+  G950_TREE_MERGE(NAME##_r##RW##_merge16, D, F16, RW, 16)
 #define G950_TREE_SET(TNAME, F16)                          \
   G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 1, 2)   \
   G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 2, 2)   \

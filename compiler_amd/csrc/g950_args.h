@@ -234,6 +234,7 @@ struct AttnTreeArgs {
   int row_blocks;           // blocks of rows (node x head of the group) per (sequence, KV head)
   int parts;                // parts that the batch's keys are cut into at most; 0: one per sequence
   int merge_rows;           // rows of a block that any sequence can have
+  int min_tiles;            // of 64 keys, of a part
   float* part;              // [parts][row_blocks][Hkv][rows][D] unnormalised O
   float* ml;                // [parts][row_blocks][Hkv][rows][2] maximum (log2 units), sum
 };

@@ -2110,15 +2110,16 @@ constexpr long long kTreeOneRange = 512;
 
 TreeShape tree_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
                      long long seqlen_k) {
-  static const long long env1 = getenv("TREE_T1") ? atoi(getenv("TREE_T1")) : 4, env2 = getenv("TREE_T2") ? atoi(getenv("TREE_T2")) : 2;
+  static const long long env1 = getenv("TREE_T1") ? atoi(getenv("TREE_T1")) : 6, env2 = getenv("TREE_T2") ? atoi(getenv("TREE_T2")) : 2;
   const long long cus = m ? m->cus : 256, rows = seqlen_q * (h / hk);
   TreeShape f{};
-  f.rw = rows <= 32 && d < 256 ? 1 : rows <= 64 ? 2 : 4;
+  static const long long env4 = getenv("TREE_R1") ? atoi(getenv("TREE_R1")) : 0;
+  f.rw = env4 && rows <= 32 && d < 256 ? 1 : rows <= 64 ? 2 : 4;
   f.row_blocks = (rows + 32 * f.rw - 1) / (32 * f.rw);
   f.units = hk * f.row_blocks;
-  const long long places = (f.rw == 1 ? env1 : env2) * cus;
+  const long long places = (rows <= 32 ? env1 : env2) * cus;
   if (f.units && seqlen_k > kTreeOneRange && b * f.units < places)
-    f.parts = std::max(places / f.units, 2 * b);
+    f.parts = std::min(std::max(places / f.units, 2 * b), 128 * b);
   return f;
 }
 
@@ -2206,6 +2207,8 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
     // as many parts as the workspace holds records for; one more than the sequences, or none
     a.parts = (int)std::min(f.parts, ws.shape[0] / (f.units * block_rows * (D + 2)));
     if (a.parts <= a.B) a.parts = 0;
+    static const int env6 = getenv("TREE_MIN") ? atoi(getenv("TREE_MIN")) : 2;
+    a.min_tiles = env6;
     a.seqlen_q = (int)std::min(SQ, T);
     a.row_blocks = (int)f.row_blocks;
     a.merge_rows = (int)std::min(block_rows, std::min(SQ, T) * (H / HK));
@@ -2217,15 +2220,19 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
     const int n = snprintf(name, sizeof name, "g950_attn_tree_%s_d%lld_r%lld", dt == G950_DTYPE_BFLOAT16 ? "bf16" : "f16", D, f.rw);
     if (int rc = launch(m, name, (unsigned)grid, 256u, a, stream)) return rc;
     if (!a.parts) return G950_OK;
-    snprintf(name + n, sizeof name - n, "_merge");
-    return launch(m, name, (unsigned)((a.B * f.units * a.merge_rows + 3) / 4), 256u, a, stream);
+    const long long groups = a.B * f.units * ((a.merge_rows + 256 / D - 1) / (256 / D));
+    static const long long env3 = getenv("TREE_MW") ? atoi(getenv("TREE_MW")) : 2048;
+    static const long long env5 = getenv("TREE_MX") ? atoi(getenv("TREE_MX")) : 128;
+    const int nw = groups <= env5 ? 16 : groups <= env3 ? 4 : 1;
+    snprintf(name + n, sizeof name - n, "_merge%d", nw);
+    return launch(m, name, (unsigned)(nw == 1 ? (groups + 3) / 4 : groups), nw == 1 ? 256u : 64u * nw, a, stream);
   }
   return launch(m, "g950_attn_tree_general", (unsigned)rows, 64u, a, stream);
 }
 
 // Workgroups of a sequence: as many as there are CUs for, with some thousand columns each.
 long long verify_parts(const g950_module* m, long long b, long long v) {
-  static const long long env1 = getenv("VER_C") ? atoi(getenv("VER_C")) : 2048, env2 = getenv("VER_M") ? atoi(getenv("VER_M")) : 1;
+  static const long long env1 = getenv("VER_C") ? atoi(getenv("VER_C")) : 2048, env2 = getenv("VER_M") ? atoi(getenv("VER_M")) : 2;
   const long long cus = env2 * (m ? m->cus : 256);
   return b < 1 ? 1 : std::max(1ll, std::min({cus / b, v / env1, 64ll}));
 }

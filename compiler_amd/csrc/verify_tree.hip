@@ -215,6 +215,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
       // the waves' sums of the part
       long long from, end;
       bounds(of, wave, from, end);
+      if (!Q) __syncthreads();  // gone[]
       double t = 0.0;
       constexpr int U = 4;  // vectors of each row in flight
 #pragma unroll 1
@@ -279,40 +280,69 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
   int at = 1;         // nodes before it are done with
   bool walk = true;   // the path goes on
   bool known = false; // S, seg and upto are those of this node with this A
+  // the nodes of the window, one per lane
+  int window = 0, up, mine_x, before = 0;  // before: refused children in earlier windows
+  float mine_u;
+  double mine_p, mine_q;
+  uint64_t out = 0;  // the window's refused children
+  auto load = [&]() {
+    const int i = min(window + lane, n - 1);
+    up = window + lane < n ? par[i] : -1;
+    mine_x = tok[i];
+    mine_u = us[i];
+    mine_p = px[i];
+    mine_q = qx[i];
+    out = 0;
+  };
+  load();
   for (;;) {
     while (walk) {
-      // the next child of the node, 64 nodes at a time
-      int i = n;
-      for (int k = at & ~63; k < n && i == n && count < a.L; k += 64) {
-        const uint64_t kids = __ballot(k + lane < n && k + lane >= at && par[k + lane] == cur);
-        if (kids) i = k + __ffsll((unsigned long long)kids) - 1;
+      // the next child of the node: lane i holds node `window` + i, a test reads its lane
+      uint64_t kids = 0;
+      while (at < n && count < a.L) {
+        if (at >= window + 64) {
+          window = at & ~63;
+          load();
+          before = refused;
+          __syncthreads();  // gone[]
+        }
+        kids = __ballot(up == cur) & (~0ull << (at - window));
+        if (kids) break;
+        at = window + 64;
       }
-      if (i == n) {
+      if (!kids) {
         walk = false;
         break;
       }
-      at = i + 1;
-      double r = Q ? fmax(fma(-A, qx[i], px[i]), 0.0) : px[i];
-      for (int k = 0; k < refused; ++k) r = gone[k] == tok[i] ? 0.0 : r;
-      if ((double)us[i] * qx[i] * S < r * rest) {
-        if (tid == 0 && part == 0) path[count] = i;
+      const int l = __ffsll((unsigned long long)kids) - 1;
+      at = window + l + 1;
+      const int x = __builtin_amdgcn_readlane(mine_x, l);
+      const double p = verify_lane(mine_p, l), q = verify_lane(mine_q, l), u = (double)__builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine_u), l));
+      double r = Q ? fmax(fma(-A, q, p), 0.0) : p;
+      if (refused) {  // (without q: a token that was refused already is out)
+        if (__ballot(mine_x == x) & out) r = 0.0;
+        for (int k = 0; k < before; ++k) r = gone[k] == x ? 0.0 : r;
+      }
+      if (u * q * S < r * rest) {
+        if (tid == 0 && part == 0) path[count] = window + l;
         ++count;
-        cur = i;
-        refused = 0;
+        cur = window + l;
+        refused = before = 0;
+        out = 0;
         A = 0.0;
         S = rest = 1.0;
         known = false;
       } else if (Q) {
         A += S / rest;
-        if (a.distinct) rest = fmax(rest - qx[i], 0x1p-24);
+        if (a.distinct) rest = fmax(rest - q, 0x1p-24);
         known = false;
         break;
       } else {
         S -= r;
-        __syncthreads();
-        if (tid == 0) gone[refused] = tok[i];
+        if (tid == 0) gone[refused] = x;
         ++refused;
-        __syncthreads();
+        out |= 1ull << l;
       }
     }
     if (!walk && known) {
@@ -337,10 +367,10 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
   const uint64_t over = __ballot(lane < parts && mine > want), some_left = __ballot(lane < parts && mine > below);
   const int of = over ? __ffsll((unsigned long long)over) - 1 : some_left ? 63 - __clzll((long long)some_left) : 0;
   if (of != part) return;
-  double before = verify_lane(below, of);
+  double start = verify_lane(below, of);
   int w = 0;
-  while (w + 1 < VERIFY_WAVES && !(before + seg[w] > want)) before += seg[w++];
-  while (w > 0 && !(seg[w] > 0.0)) before -= seg[--w];  // (a share past the end)
+  while (w + 1 < VERIFY_WAVES && !(start + seg[w] > want)) start += seg[w++];
+  while (w > 0 && !(seg[w] > 0.0)) start -= seg[--w];  // (a share past the end)
   long long from, end;
   bounds(part, w, from, end);
   const T* pr = P + (long long)(b0 + cur) * a.t_row;
@@ -357,7 +387,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
     const double t = verify_scan(s);
     if (lane == 63) scan[wave] = t;
     __syncthreads();
-    double mine = before + (t - s);
+    double mine = start + (t - s);
 #pragma unroll
     for (int k = 0; k < VERIFY_WAVES; ++k) mine += k < wave ? scan[k] : 0.0;
     int hit = -1, any = -1;
@@ -372,7 +402,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
     if (hit >= 0) atomicMin(&found, hit);
     if (any >= 0) atomicMax(&some, any);
 #pragma unroll
-    for (int k = 0; k < VERIFY_WAVES; ++k) before += scan[k];
+    for (int k = 0; k < VERIFY_WAVES; ++k) start += scan[k];
     __syncthreads();
     if (found != 0x7FFFFFFF) break;
   }
