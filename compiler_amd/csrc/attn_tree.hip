@@ -283,28 +283,28 @@ template <int D, int RW>
 struct TreeCfg {
   static constexpr int KW = 4 / RW;
   static constexpr int SUB = KW == 1 ? 2 : 1;           // 32-key tiles of a wave in a stage
-  static constexpr int TKS = 32 * KW * SUB;             // keys of a stage
+  static constexpr int TKS = 32 * KW * SUB;             // keys of a stage: 64
   static constexpr int ROW = 2 * D, KT = TKS * ROW, STAGE = 2 * KT;
-  static constexpr int NS = 2;
   static constexpr int ROWS = 32 * RW;
-  static constexpr int LDS = NS * STAGE;
+  static constexpr int LDS = 2 * STAGE;
   static_assert(LDS >= 4 * 32 * D * 4, "the waves' partial O fits the ring");
 };
 
 template <int D, bool F16, int RW>
 __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
   using C = TreeCfg<D, RW>;
-  constexpr int KW = C::KW, SUB = C::SUB, TKS = C::TKS, ROW = C::ROW, KT = C::KT, NS = C::NS, ROWS = C::ROWS;
+  constexpr int KW = C::KW, SUB = C::SUB, TKS = C::TKS, ROW = C::ROW, KT = C::KT, ROWS = C::ROWS;
   constexpr int KPI = 1024 / ROW, CH = ROW / 16;  // keys of a DMA instruction, 16-byte pieces of a row
   constexpr int DI = 16 / KPI;                    // DMA instructions of 16 keys' K
   constexpr int RUNS = TKS / 16, RPW = RUNS / 4;  // 16-key runs of a stage, of a wave's loads
   constexpr int SB = 64 / RUNS;                   // stages of which the lanes hold the runs' pages
-  constexpr int DPT = RPW * 2 * DI;               // DMA instructions of a wave and stage
   constexpr int DS = D / 16, DB = D / 32;
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
   __shared__ short par[TREE_NODES];
   __shared__ float ml[4][32][2];
   __shared__ int odd[4];
+  __shared__ float share[ROWS][KW];
+  __shared__ long long place[ROWS];
   if (blockDim.x != 256) return;  // launch shape must match the kernel
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -411,6 +411,7 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
   const int kread = r32 * ROW, kx = (g ^ kswz(r32)) << 4;
   const int j16 = lane & 15;
   const int vread = (4 * g + (j16 >> 2)) * ROW + 32 * ((lane >> 4) & 1) + 8 * (j16 & 3), vx = vswz(j16 >> 2) << 6;
+  const uint32_t own = kw * 32 * SUB * ROW;  // this wave's keys of a stage
   f32x16 s[SUB];
   u32x4 pf[SUB][2];
   uint32_t vis[SUB];  // the row's visible keys of each tile of a masked stage
@@ -564,7 +565,6 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     auto kat = [&](int i) { return (uint32_t)(i & 1) * KT; };
     auto vat = [&](int i) { return (uint32_t)(2 + (i & 1)) * KT; };
     constexpr int R = 2 * DB, NV = 2 * SUB, NK = SUB * DS;
-    const uint32_t own = kw * 32 * SUB * ROW;  // this wave's keys of a stage
     u32x2 vt[2][R];
     u32x4 kf[8];
     auto vread_ = [&](auto ic, uint32_t slot) {  // group I: V of keys 16 I .. + 15
@@ -655,31 +655,32 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     }
     tree_barrier();
   } else {
-    // Bound by the bytes: whole stages in a ring of NS.
+    // (no registers for reads ahead: whole stages, products as the compiler orders them)
     auto issue = [&](int j) {
       stage_pages(j);
-      dma_k(j % NS * C::STAGE);
-      dma_v(j % NS * C::STAGE + KT);
+      dma_k((j & 1) * C::STAGE);
+      dma_v((j & 1) * C::STAGE + KT);
       if ((j + 1) % SB == 0) look(j + 1);
     };
-    for (int j = 0; j < NS && j < nst; ++j) issue(j);
+    if (nst > 0) issue(0);
+    if (nst > 1) issue(1);
     for (int i = 0; i < nst; ++i) {
-      // stage i has landed once at most the later stages' loads are in flight
-      if (i + NS <= nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * DPT) : "memory");
+      // stage i has landed once at most the next one's loads are in flight
+      if (i + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * RPW * DI) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       tree_barrier();
-      const char* st = lds + (i % NS) * C::STAGE + kw * 32 * SUB * ROW;
+      char* st = lds + (i & 1) * C::STAGE;
       if (busy) {
-        scores(st);
+        scores(st + own);
         mask(i);
         softmax();
       }
-      clean(i, lds + (i % NS) * C::STAGE + KT);
-      if (busy) values(st + KT);
+      clean(i, st + KT);
+      if (busy) values(st + KT + own);
       // every wave's LDS reads have returned before the stage's slot is refilled
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       tree_barrier();
-      if (i + NS < nst) issue(i + NS);
+      if (i + 2 < nst) issue(i + 2);
     }
   }
 
@@ -698,41 +699,47 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     ml[wave][r32][1] = ls;
   }
   __syncthreads();
-  constexpr int CPR = D / 4;  // 16-byte pieces (4 d) of a row
-  for (int it = tid; it < nrows * CPR; it += 256) {
-    const int r = it / CPR, c = it % CPR, w0 = r / 32 * KW, rr = r % 32;
-    float m = ml[w0][rr][0];
+  // a row's weights of its waves' shares and its place: worked out once for all of its pieces
+  if (tid < nrows) {
+    const int w0 = tid / 32 * KW, rr = tid % 32;
+    float m = ml[w0][rr][0], lt = 0.0f, f[KW];
 #pragma unroll
     for (int x = 1; x < KW; ++x) m = fmaxf(m, ml[w0 + x][rr][0]);
-    f32x4 sum = {};
-    float lt = 0.0f;
 #pragma unroll
     for (int x = 0; x < KW; ++x) {
-      const float mw = ml[w0 + x][rr][0], lw = ml[w0 + x][rr][1];
       // no finite score: no key of this row (l = 0), or only NaN ones
-      const float f = mw == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      lt = fmaf(f, lw, lt);
-      const f32x4 ow = *(const f32x4*)(lds + (w0 + x) * 32 * D * 4 + rr * D * 4 + ((c ^ (rr & 15)) << 4));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, ow[e], sum[e]);
+      f[x] = ml[w0 + x][rr][0] == -__builtin_huge_valf() ? 1.0f : __builtin_amdgcn_exp2f(ml[w0 + x][rr][0] - m);
+      lt = fmaf(f[x], ml[w0 + x][rr][1], lt);
     }
-    if (w.rec >= 0) {
-      const long long rec = (long long)w.rec * ROWS + r;
-      *(f32x4*)(p.part + rec * D + c * 4) = sum;
-      if (c == 0) {
-        p.ml[2 * rec] = m;
-        p.ml[2 * rec + 1] = lt;
-      }
-      continue;
-    }
-    const int i = (uint32_t)(row0 + r) / G, h = w.hk * G + (uint32_t)(row0 + r) % G;
     const bool empty = !(lt > 0.0f);  // zero or NaN
-    const float inv = empty ? 1.0f : 1.0f / lt;
-    char* dst = (char*)p.o + 2 * ((long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh + c * 4);
-    *(u32x2*)dst = (u32x2){pack2(sum[0] * inv, sum[1] * inv, F16), pack2(sum[2] * inv, sum[3] * inv, F16)};
-    if (c == 0)
+    const uint32_t at = row0 + tid, i = at / G, h = w.hk * G + at % G;
+    if (w.rec >= 0) {
+      const long long rec = (long long)w.rec * ROWS + tid;
+      *(f32x2*)(p.ml + 2 * rec) = (f32x2){m, lt};
+      place[tid] = rec * D;
+    } else {
       p.lse[(long long)h * p.lse_h + (long long)(sq.q0 + i) * p.lse_t] =
           empty ? __builtin_huge_valf() : (m + __log2f(lt)) * 0.69314718055994530942f;
+      place[tid] = (long long)(sq.q0 + i) * p.o_st + (long long)h * p.o_sh;
+    }
+#pragma unroll
+    for (int x = 0; x < KW; ++x) share[tid][x] = w.rec >= 0 || empty ? f[x] : f[x] / lt;
+  }
+  __syncthreads();
+  constexpr int CPR = D / 4;  // 16-byte pieces (4 d) of a row
+#pragma unroll 4
+  for (int k = 0; k < ROWS * CPR / 256; ++k) {
+    const int r = (tid + 256 * k) / CPR, c = tid % CPR, w0 = r / 32 * KW, rr = r % 32;
+    if (r >= nrows) break;
+    f32x4 sum = {};
+#pragma unroll
+    for (int x = 0; x < KW; ++x) {
+      const f32x4 ow = *(const f32x4*)(lds + (w0 + x) * 32 * D * 4 + rr * D * 4 + ((c ^ (rr & 15)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(share[r][x], ow[e], sum[e]);
+    }
+    if (w.rec >= 0) *(f32x4*)(p.part + place[r] + c * 4) = sum;
+    else *(u32x2*)((uint16_t*)p.o + place[r] + c * 4) = (u32x2){pack2(sum[0], sum[1], F16), pack2(sum[2], sum[3], F16)};
   }
 }
 
@@ -840,10 +847,8 @@ extern "C" __global__ __launch_bounds__(64) void g950_attn_tree_general(const g9
   G950_TREE_MERGE(NAME##_r##RW##_merge4, D, F16, RW, 4)                                                      \
   G950_TREE_MERGE(NAME##_r##RW##_merge16, D, F16, RW, 16)
 #define G950_TREE_SET(TNAME, F16)                          \
-  G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 1, 2)   \
   G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 2, 2)   \
   G950_TREE(g950_attn_tree_##TNAME##_d64, 64, F16, 4, 2)   \
-  G950_TREE(g950_attn_tree_##TNAME##_d128, 128, F16, 1, 1) \
   G950_TREE(g950_attn_tree_##TNAME##_d128, 128, F16, 2, 2) \
   G950_TREE(g950_attn_tree_##TNAME##_d128, 128, F16, 4, 2) \
   G950_TREE(g950_attn_tree_##TNAME##_d256, 256, F16, 2, 1) \

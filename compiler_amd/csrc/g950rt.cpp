@@ -2098,28 +2098,38 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
 constexpr long long kTreeNodes = G950_TREE_NODES;
 static_assert(kTreeNodes == TREE_NODES, "the header's limit is the kernels'");
 
-// How attention of trees cuts a call: blocks of rows (node x head of the group) per
-// (sequence, KV head), and parts of their keys, whose records need a workspace.
+// How attention of trees cuts a call: blocks of 64 or 128 rows (node x head of the group) per
+// (sequence, KV head), and parts of the batch's keys, whose records need a workspace.  The lengths are the
+// device's: parts are dealt there, all of about one length.
+// Measured at d 128 in bfloat16, 32 query heads on 8 KV heads, us for the parts + for joining them:
+//   * Parts for two workgroups per CU, as many as are resident; for up to 32 rows, whose
+//     records are small, six, which end together more evenly.  16 trees of 9 to 32 nodes over 300
+//     to 4096 keys 43 + 9 with two, 49 + 11 with three, 52 + 14 with four, 58 + 7 with one; 8 of
+//     50 to 64 over 2049 to 8192 63 + 10, 76 + 12, 71 + 14, 117 + 7; 32 single tokens over 300 to
+//     4096 74 + 5 with two, 64 + 5 with four, 62 + 5 with six, 63 + 6 with eight.
+//   * Parts of 128 keys or more: one tree of 26 nodes behind 974 keys 12.4 + 4.8, 14.3 + 4.6 with
+//     256, 18.8 + 4.6 with 512.  At most 128 a sequence: two of 50001 and 65537 keys (d 64, one
+//     KV head) 17.1 + 6.4, with 256 15.9 + 8.5.
+//   * Up to 512 keys one part.
 struct TreeShape {
   long long rw;          // 32-row tiles of a block
   long long row_blocks;  // per (sequence, KV head)
   long long units;       // blocks of a sequence
   long long parts;       // of the batch, wanted; 0: one per sequence
 };
-constexpr long long kTreeOneRange = 512;
+constexpr long long kTreePlaces = 2, kTreeFewRows = 32, kTreeFewPlaces = 6, kTreeMost = 128, kTreeOneRange = 512;
+constexpr int kTreeMinTiles = 2;
 
 TreeShape tree_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
                      long long seqlen_k) {
-  static const long long env1 = getenv("TREE_T1") ? atoi(getenv("TREE_T1")) : 6, env2 = getenv("TREE_T2") ? atoi(getenv("TREE_T2")) : 2;
   const long long cus = m ? m->cus : 256, rows = seqlen_q * (h / hk);
   TreeShape f{};
-  static const long long env4 = getenv("TREE_R1") ? atoi(getenv("TREE_R1")) : 0;
-  f.rw = env4 && rows <= 32 && d < 256 ? 1 : rows <= 64 ? 2 : 4;
+  f.rw = rows <= 64 ? 2 : 4;
   f.row_blocks = (rows + 32 * f.rw - 1) / (32 * f.rw);
   f.units = hk * f.row_blocks;
-  const long long places = (rows <= 32 ? env1 : env2) * cus;
+  const long long places = (rows <= kTreeFewRows ? kTreeFewPlaces : kTreePlaces) * cus;
   if (f.units && seqlen_k > kTreeOneRange && b * f.units < places)
-    f.parts = std::min(std::max(places / f.units, 2 * b), 128 * b);
+    f.parts = std::min(std::max(places / f.units, 2 * b), kTreeMost * b);
   return f;
 }
 
@@ -2207,8 +2217,7 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
     // as many parts as the workspace holds records for; one more than the sequences, or none
     a.parts = (int)std::min(f.parts, ws.shape[0] / (f.units * block_rows * (D + 2)));
     if (a.parts <= a.B) a.parts = 0;
-    static const int env6 = getenv("TREE_MIN") ? atoi(getenv("TREE_MIN")) : 2;
-    a.min_tiles = env6;
+    a.min_tiles = kTreeMinTiles;
     a.seqlen_q = (int)std::min(SQ, T);
     a.row_blocks = (int)f.row_blocks;
     a.merge_rows = (int)std::min(block_rows, std::min(SQ, T) * (H / HK));
@@ -2221,20 +2230,21 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
     if (int rc = launch(m, name, (unsigned)grid, 256u, a, stream)) return rc;
     if (!a.parts) return G950_OK;
     const long long groups = a.B * f.units * ((a.merge_rows + 256 / D - 1) / (256 / D));
-    static const long long env3 = getenv("TREE_MW") ? atoi(getenv("TREE_MW")) : 2048;
-    static const long long env5 = getenv("TREE_MX") ? atoi(getenv("TREE_MX")) : 128;
-    const int nw = groups <= env5 ? 16 : groups <= env3 ? 4 : 1;
+    // waves that share a row's parts, where there are few rows: 52 groups of rows of 128 parts 6.4 us
+    // with 16, 8.3 with 4; 416 of 8 parts 6.7 with 16, 4.8 with 4; 8192 of 4 9.1 with 1, 20.6 with 4
+    const int nw = groups <= 128 ? 16 : groups <= 2048 ? 4 : 1;
     snprintf(name + n, sizeof name - n, "_merge%d", nw);
     return launch(m, name, (unsigned)(nw == 1 ? (groups + 3) / 4 : groups), nw == 1 ? 256u : 64u * nw, a, stream);
   }
   return launch(m, "g950_attn_tree_general", (unsigned)rows, 64u, a, stream);
 }
 
-// Workgroups of a sequence: as many as there are CUs for, with some thousand columns each.
+// Workgroups of a sequence: two for every CU, with 2048 columns each at least (16 trees over
+// 128000 tokens: 32.7 us with two, 35.4 with one, 38 with four; one over 32000 tokens: 13.7 with 1024,
+// 2048 or 4096 columns).
 long long verify_parts(const g950_module* m, long long b, long long v) {
-  static const long long env1 = getenv("VER_C") ? atoi(getenv("VER_C")) : 2048, env2 = getenv("VER_M") ? atoi(getenv("VER_M")) : 2;
-  const long long cus = env2 * (m ? m->cus : 256);
-  return b < 1 ? 1 : std::max(1ll, std::min({cus / b, v / env1, 64ll}));
+  const long long places = 2 * (m ? m->cus : 256);
+  return b < 1 ? 1 : std::max(1ll, std::min({places / b, v / 2048, 64ll}));
 }
 size_t verify_bytes(long long b, long long t, long long parts) {
   return parts > 1 ? (size_t)(t * 16 + b * VERIFY_TELL * parts * 8) : 0;
