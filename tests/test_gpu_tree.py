@@ -181,6 +181,13 @@ ATTEND = {
     "page10": dict(ql=[7, 2], kl=[170, 9], h=4, hk=2, d=128, page=10),
     "odd_d": dict(ql=[12, 1], kl=[70, 300], h=4, hk=2, d=80, page=16),
     "d1": dict(ql=[6], kl=[70], h=2, hk=1, d=1, page=16),
+    "many_parts": dict(ql=[1 + i % 5 for i in range(70)], kl=[540 + 97 * i % 1500 for i in range(70)], h=4, hk=1, d=64,
+                       page=16),
+    "part_edges": dict(ql=[2] * 24, kl=[514 + 61 * i for i in range(24)], h=4, hk=1, d=128, page=64),
+    "part_edges_window": dict(ql=[3, 1] * 12, kl=[514 + 61 * i for i in range(24)], h=4, hk=1, d=64, page=64, left=700),
+    "wide_parts": dict(ql=[60, 51, 64, 33], kl=[700, 900, 64, 1300], h=32, hk=8, d=128, page=64),
+    "wide_parts_d64": dict(ql=[60, 51, 64, 33, 41], kl=[700, 900, 64, 1300, 41], h=32, hk=8, d=64, page=16),
+    "d256_parts": dict(ql=[5, 2], kl=[2600, 1077], h=8, hk=2, d=256, page=32),
     "batch": dict(ql=[26 - i % 20 for i in range(40)], kl=[1100 - 25 * i for i in range(40)], h=8, hk=2, d=128, page=64),
 }
 
@@ -237,6 +244,20 @@ def attend_check(c, dt, o, lse):
 def test_attend(case, dt):
     c = attend_case(case, dt)
     attend_check(c, dt, *attend_run(c, dt))
+
+
+# the last kernel of some of them (behind g950_attn_tree_<type>_): every form by name
+FORMS = {"one_key": "d128_r2", "rows64": "d64_r2", "rows33": "d128_r2", "rows65": "d64_r4", "rows128": "d128_r4_merge4",
+         "chain": "d128_r4", "large": "d64_r4_merge4", "d256": "d256_r2_merge16", "d256_blocks": "d256_r4_merge4",
+         "longest_parts": "d128_r2_merge16", "parts_d64": "d64_r4_merge16", "wide_parts": "d128_r4_merge1",
+         "wide_parts_d64": "d64_r4_merge1", "part_edges": "d128_r2_merge16", "many_parts": "d64_r2_merge4", "page48": "d128_r2",
+         "page1": "general", "page10": "general", "odd_d": "general", "d1": "general"}
+
+
+@pytest.mark.parametrize("case", sorted(FORMS))
+def test_attend_forms(case):
+    attend_run(attend_case(case, "float16"), "float16")
+    assert rt.module().last_kernel == "g950_attn_tree_" + ("" if FORMS[case] == "general" else "f16_") + FORMS[case]
 
 
 @pytest.mark.parametrize("floats", [0, 5000, 1 << 22])
