@@ -202,6 +202,13 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
     from = min(of * len + w * share, end);
     to = min(from + share, end);
   };
+  // A wave's share of up to U vectors of each row stays in registers: the next sum of the
+  // same node and the search for the token need no loads.
+  constexpr int U = 4;
+  const bool fits = share <= 64 * N * U;
+  u32x4 wp[U], wq[U];
+  int held = -1;        // the node whose vectors they are
+  bool held_q = false;  // q's as well
   // what is left of the node's row: S, and upto[] and seg[] as well.  (One place in the code
   // for all of it: code that runs a few times is bound by being fetched.)
   auto sum = [&]() {
@@ -217,15 +224,15 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
       bounds(of, wave, from, end);
       if (!Q) __syncthreads();  // gone[]
       double t = 0.0;
-      constexpr int U = 4;  // vectors of each row in flight
+      const bool here = own && held == cur && (held_q || !both);
 #pragma unroll 1
       for (long long v0 = from + lane * N; v0 - lane * N < end; v0 += 64 * N * U) {
-        u32x4 wp[U], wq[U];
+        if (!here)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          wp[u] = read(pr, v0 + 64 * N * u);
-          wq[u] = both ? read(qr, v0 + 64 * N * u) : (u32x4){0, 0, 0, 0};
-        }
+          for (int u = 0; u < U; ++u) {
+            wp[u] = read(pr, v0 + 64 * N * u);
+            wq[u] = both ? read(qr, v0 + 64 * N * u) : (u32x4){0, 0, 0, 0};
+          }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           double r[N];
@@ -234,6 +241,8 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
           for (int e = 0; e < N; ++e) t += r[e];
         }
       }
+      held = own && fits ? cur : -1;
+      held_q = here ? held_q : both;
       t = verify_lane(verify_scan(t), 63);
       __syncthreads();  // (whoever read the sums before is done)
       if (lane == 0) (own ? seg : other)[wave] = t;
@@ -373,6 +382,38 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
   while (w > 0 && !(seg[w] > 0.0)) start -= seg[--w];  // (a share past the end)
   long long from, end;
   bounds(part, w, from, end);
+  if (held == cur) {  // the wave that has them
+    if (wave != w) return;
+    int some = -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long v = from + lane * N + 64 * N * u;
+      double r[N], s = 0.0;
+      left(wp[u], wq[u], v, end, r);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += r[e];
+      const double t = verify_scan(s);
+      double mine = start + (t - s);
+      int hit = -1, any = -1;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        mine += r[e];
+        if (r[e] > 0.0) {
+          any = (int)(place(v) + e);
+          if (hit < 0 && mine > want) hit = any;
+        }
+      }
+      const uint64_t hits = __ballot(hit >= 0), anys = __ballot(any >= 0);
+      if (hits) {
+        if (lane == __ffsll((unsigned long long)hits) - 1) answer(hit);
+        return;
+      }
+      if (anys) some = __builtin_amdgcn_readlane(any, 63 - __clzll((long long)anys));
+      start += verify_lane(t, 63);
+    }
+    if (lane == 0) answer(max(some, 0));
+    return;
+  }
   const T* pr = P + (long long)(b0 + cur) * a.t_row;
   const T* qr = Q + (long long)(b0 + cur) * a.d_row;
   if (tid == 0) found = 0x7FFFFFFF, some = -1;
