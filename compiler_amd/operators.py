@@ -567,15 +567,31 @@ def paged_attention_int4(q, k_cache, k_scale, v_cache, v_scale, page_table, cu_s
     return o, lse
 
 
+def _new(like, code, shape, stream):
+    """torch.empty of ``shape`` on like's device, its dtype by code (0: like's), for an output
+    of a call on ``stream``."""
+    if stream is None:
+        t = (rt._packer or rt._load_packer()).empty(like, code, *shape)
+        if t is not None:
+            return t
+    import torch
+    dtype = {0: like.dtype, rt.DT_F32: torch.float32, rt.DT_INT32: torch.int32}[code]
+    return (torch.empty if stream is None else _on_stream(stream, torch.empty))(shape, dtype=dtype, device=like.device)
+
+
+def _room(floats, like, stream):
+    """_workspace, from native code on the current stream."""
+    if stream is None and rt._raw_stream(rt.module().device) != 2:
+        return _new(like, rt.DT_F32, (floats,), None)
+    return _workspace(floats, like, stream)
+
+
 def paged_append_tree(q, k, v, cos, sin, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, parent,
                       interleaved=False, out=None, **kw):
     """paged_append for drafted trees: ``parent`` holds each token's parent within its
     sequence.  See paged_append_tree_kernel."""
-    import torch
-    stream = kw.get("stream")
-    empty_like = torch.empty_like if stream is None else _on_stream(stream, torch.empty_like)
     q = k.new_empty((k.shape[0], 0, k.shape[2])) if q is None else q
-    out = empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    out = _new(q, 0, q.shape, kw.get("stream")) if out is None else out
     paged_append_tree_kernel(q, k, v, cos, sin, out, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, parent,
                              bool(interleaved), **kw)
     return out
@@ -587,24 +603,17 @@ def paged_attention_tree(q, k_cache, v_cache, page_table, cu_seqlens_q, seqused_
     to 1024), seqlen_k the most keys of a sequence.  Returns o and lse [h,
     tokens].  The workspace (float32) comes from torch's allocator, on the
     call's stream, unless given."""
-    import torch
     t, h, d = q.shape
     seqlen_q, seqlen_k = int(seqlen_q), int(seqlen_k)
     stream = kw.get("stream")
-    if out is None:
-        o = (torch.empty_like if stream is None else _on_stream(stream, torch.empty_like))(
-            q, memory_format=torch.contiguous_format)
-    else:
-        o = out
-    if lse is None:
-        lse = (torch.empty if stream is None else _on_stream(stream, torch.empty))(
-            (h, t), dtype=torch.float32, device=q.device)
+    o = _new(q, 0, (t, h, d), stream) if out is None else out
+    lse = _new(q, rt.DT_F32, (h, t), stream) if lse is None else lse
     if workspace is None:
         floats = 0
-        if q.dtype != torch.float32:
+        if q.element_size() == 2:
             floats = rt.module().attention_tree_workspace(cu_seqlens_q.shape[0] - 1, h, k_cache.shape[2], d,
                                                           min(seqlen_q, t), seqlen_k)
-        workspace = _workspace(floats, q, stream)
+        workspace = _room(floats, q, stream)
     paged_attention_tree_kernel(q, k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, parent, o, lse, workspace,
                                 seqlen_q, seqlen_k, 1.0 / math.sqrt(d) if scale is None else float(scale),
                                 int(window_left), **kw)
@@ -618,15 +627,13 @@ def verify_tree(target_probs, draft_probs, tokens, parent, uniform, uniform_next
     path [b, most] (the accepted nodes, root first, then -1), count [b] and the
     next token [b].  The workspace (float32) comes from torch's allocator, on the call's
     stream, unless given."""
-    import torch
     b, stream = cu_seqlens_q.shape[0] - 1, kw.get("stream")
-    empty = torch.empty if stream is None else _on_stream(stream, torch.empty)
-    path = empty((b, int(most)), dtype=torch.int32, device=tokens.device) if path is None else path
-    count = empty((b,), dtype=torch.int32, device=tokens.device) if count is None else count
-    next_token = empty((b,), dtype=tokens.dtype, device=tokens.device) if next_token is None else next_token
+    path = _new(tokens, rt.DT_INT32, (b, int(most)), stream) if path is None else path
+    count = _new(tokens, rt.DT_INT32, (b,), stream) if count is None else count
+    next_token = _new(tokens, 0, (b,), stream) if next_token is None else next_token
     draft = _none(target_probs.dtype, target_probs.device, 2) if draft_probs is None else draft_probs
     if workspace is None:
-        workspace = _workspace(rt.module().verify_tree_workspace(b, tokens.shape[0], target_probs.shape[1]), tokens, stream)
+        workspace = _room(rt.module().verify_tree_workspace(b, tokens.shape[0], target_probs.shape[1]), tokens, stream)
     verify_tree_kernel(target_probs, draft, tokens, parent, uniform, uniform_next, cu_seqlens_q, path, count, next_token,
                        workspace, bool(distinct), **kw)
     return path, count, next_token
@@ -635,10 +642,7 @@ def verify_tree(target_probs, draft_probs, tokens, parent, uniform, uniform_next
 def paged_keep_path(k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, path, count, out=None, **kw):
     """Moves the accepted paths' cache rows (paged_keep_path_kernel) and returns the
     keys that each sequence has now [b]."""
-    import torch
-    stream = kw.get("stream")
-    empty_like = torch.empty_like if stream is None else _on_stream(stream, torch.empty_like)
-    out = empty_like(seqused_k) if out is None else out
+    out = _new(seqused_k, 0, seqused_k.shape, kw.get("stream")) if out is None else out
     paged_keep_path_kernel(k_cache, v_cache, page_table, cu_seqlens_q, seqused_k, path, count, out, **kw)
     return out
 
