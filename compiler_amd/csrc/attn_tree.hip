@@ -190,14 +190,24 @@ struct TreeDeal {
       const int n = tiles_again(z0);
       sum += __builtin_amdgcn_readlane(tree_scan(n), 63);
     }
-    const int room = p.parts - p.B;
-    c = max((int)((sum + room - 1) / room), p.min_tiles);
+    // the least c that gives no more than p.parts: between those of parts without remainders and
+    // with one for every sequence
+    int lo = max((int)((sum + p.parts - 1) / p.parts), p.min_tiles);
+    c = max((int)((sum + p.parts - p.B - 1) / (p.parts - p.B)), p.min_tiles);
+    while (lo < c) {
+      const int mid = (uint32_t)(lo + c) / 2;
+      int n = 0;
+      for (int z0 = 0; z0 < p.B; z0 += 64) n += __builtin_amdgcn_readlane(tree_scan(cut(tiles_again(z0), mid)), 63);
+      if (n <= p.parts) c = mid;
+      else lo = mid + 1;
+    }
   }
+  static __device__ __forceinline__ int cut(int n, int c) { return (uint32_t)(n + c - 1) / (uint32_t)c; }
   // the sequence that part `part` belongs to, and the parts before that sequence; -1: none
   __device__ __forceinline__ int sequence(int part, int& before) const {
     int start = 0;
     for (int z0 = 0; z0 < p.B; z0 += 64) {
-      const int k = (tiles_again(z0) + c - 1) / c, upto = start + tree_scan(k);
+      const int k = cut(tiles_again(z0), c), upto = start + tree_scan(k);
       const uint64_t past = __ballot(upto > part);
       if (past) {
         const int at = __ffsll((unsigned long long)past) - 1;
@@ -212,7 +222,7 @@ struct TreeDeal {
   __device__ __forceinline__ int before(int z) const {
     int start = 0;
     for (int z0 = 0;; z0 += 64) {
-      const int k = (tiles_again(z0) + c - 1) / c, upto = start + tree_scan(k);
+      const int k = cut(tiles_again(z0), c), upto = start + tree_scan(k);
       if (z < z0 + 64) return __builtin_amdgcn_readlane(upto - k, z - z0);
       start = __builtin_amdgcn_readlane(upto, 63);
     }
