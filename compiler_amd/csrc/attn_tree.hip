@@ -192,8 +192,9 @@ struct TreeDeal {
     }
     // the least c that gives no more than p.parts: between those of parts without remainders and
     // with one for every sequence
-    int lo = max((int)((sum + p.parts - 1) / p.parts), p.min_tiles);
-    c = max((int)((sum + p.parts - p.B - 1) / (p.parts - p.B)), p.min_tiles);
+    // (no sequence has more than 2^25 tiles)
+    int lo = max((int)min((sum + p.parts - 1) / p.parts, 1ll << 25), p.min_tiles);
+    c = max((int)min((sum + p.parts - p.B - 1) / (p.parts - p.B), 1ll << 25), p.min_tiles);
     while (lo < c) {
       const int mid = (uint32_t)(lo + c) / 2;
       int n = 0;
@@ -449,9 +450,9 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
       const int k0 = kv0 + 32 * t, n0 = k0 - sq.base;  // first key, and as a node
       uint32_t v = n0 <= -32 ? ~0u : n0 < 0 ? (1u << -n0) - 1 : 0u;
       if (first > k0) v &= first - k0 < 32 ? ~0u << (first - k0) : 0u;
-      // (a tile behind the range is walked by the part that it belongs to: here there may
-      // be no parents)
-      if (n0 > -32 && k0 < hi)
+      // (nodes behind the range are walked by the part that they belong to, or have no cache
+      // row: here there may be no parents)
+      if (n0 > -32 && k0 < hi && hi > sq.base)
         while (cur >= max(n0, 0)) {
           if (cur - n0 < 32 && (p.left < 0 || up <= p.left)) v |= 1u << (cur - n0);
           cur = par[cur];
@@ -524,7 +525,7 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
   auto clean = [&](int i, char* vp) {
     const int kv0 = lo + TKS * (nst - 1 - i);
     const uint32_t alive = (uint32_t)(live[(i / SB) & 1] >> (i % SB * RUNS)) & ((1u << RUNS) - 1);
-    if (alive == (1u << RUNS) - 1 && kv0 + TKS <= min(sq.base, hi) && (p.left < 0 || sq.base + sq.nq - p.left <= kv0)) return;
+    if (alive == (1u << RUNS) - 1 && kv0 + TKS <= min(sq.base, hi) && (p.left < 0 || (long long)sq.base + sq.nq - p.left <= kv0)) return;
     // an exponent of ones carries into the bit above it
     constexpr uint32_t EXP = F16 ? 0x7C007C00u : 0x7F807F80u, CARRY = F16 ? 0x04000400u : 0x00800080u;
     uint32_t found = 0;

@@ -281,6 +281,21 @@ def test_attend_bad_lists(dt):
     attend_check(c, dt, *attend_run(c, dt))
 
 
+@pytest.mark.parametrize("left", [-1, 40, 2 ** 31 - 1])
+def test_attend_tables_that_end_before_the_tree(left):
+    """The last key that the table holds and the tree's first in one tile: no node of the tree has a row."""
+    for ql, kl, pages in (([5, 3], [59, 57], 3), ([5, 9], [1305, 1309], 81), ([26, 40], [80, 101], 4)):
+        c = attend_case(dict(ql=ql, kl=kl, h=8, hk=2, d=128, page=16, left=left), "bfloat16")
+        c["table"] = np.ascontiguousarray(c["table"][:, :pages])
+        attend_check(c, "bfloat16", *attend_run(c, "bfloat16"))
+
+
+def test_attend_the_widest_window():
+    for case in ("fewer_keys_than_nodes", "parts_d64", "rows129"):
+        c = dict(attend_case(case, "bfloat16"), left=2 ** 31 - 1)
+        attend_check(c, "bfloat16", *attend_run(c, "bfloat16"))
+
+
 @pytest.mark.parametrize("most", [0, 1, 20])
 def test_attend_covers_seqlen_q_nodes(most):
     for case in ("parts", "rows129"):
