@@ -181,10 +181,11 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
   auto left = [&](const u32x4& wp, const u32x4& wq, long long v, long long end, double (&r)[N]) {
     const uint32_t in = cover(v, end);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      r[e] = verify_element<T>(wp, e);
-      if (Q) r[e] = fmax(fma(-A, verify_element<T>(wq, e), r[e]), 0.0);
-    }
+    for (int e = 0; e < N; ++e) r[e] = verify_element<T>(wp, e);
+    // (A = 0 leaves p as it is, whatever q held: infinities too)
+    if (Q && A > 0.0)
+#pragma unroll
+      for (int e = 0; e < N; ++e) r[e] = fmax(fma(-A, verify_element<T>(wq, e), r[e]), 0.0);
     if (!Q)
       for (int k = 0; k < refused; ++k) {
         const long long at = gone[k] - place(v);
@@ -337,6 +338,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
         if (tid == 0 && part == 0) path[count] = window + l;
         ++count;
         cur = window + l;
+        if (before) __syncthreads();  // gone[] has been read
         refused = before = 0;
         out = 0;
         A = 0.0;

@@ -492,6 +492,38 @@ def test_verify_many_refusals(dt):
     verify_check(c, verify_run(c, dt))
 
 
+@pytest.mark.parametrize("drafts", ["drawn", "chosen"])
+def test_verify_wide_levels(drafts):
+    """Each level's children spread over several 64-node windows, all refused but the last one."""
+    VERIFY["wide"] = dict(ql=[600, 1], v=3001)
+    for seed in range(3):
+        c = verify_case("wide", drafts, "float32", seed=seed)
+        c["parent"][1:600] = [-1 if i < 1 else 199 * ((i - 1) // 199) for i in range(1, 600)]
+        c["tokens"][:600] = np.random.default_rng(seed).permutation(3001)[:600]
+        c["u"][:] = 1 - 2.0 ** -24
+        c["u"][[199, 398, 597]] = 0.0
+        for ws in (None, torch.empty(0, device="cuda")):
+            got = verify_run(c, "float32", workspace=ws)
+            verify_check(c, got)
+            if drafts == "chosen":
+                assert got[0][0, :4].tolist() == [0, 199, 398, 597]
+
+
+def test_verify_unbounded_drafts():
+    """A draft's value that is infinite takes its column from what is left, but not from p, which is
+    taken where nothing is left."""
+    VERIFY["two"] = dict(ql=[2], v=9000)
+    c = verify_case("two", "drawn", "float32")
+    c["parent"][:2], c["tokens"][1], c["u"][1], c["last"][0] = [-1, 0], 3, 1 - 2.0 ** -24, 0.5
+    c["target"][0] = 0.125 / 8999
+    c["target"][0, 5000] = 0.875
+    c["draft"][0] = c["target"][0] * 2
+    c["draft"][0, 5000] = np.inf
+    for ws in (None, torch.empty(0, device="cuda")):
+        path, count, nxt = verify_run(c, "float32", workspace=ws)
+        assert count.tolist() == [1] and nxt.tolist() == [5000] and path[0, 0] == 0
+
+
 @pytest.mark.parametrize("most", [1, 2, 3])
 def test_verify_full_paths(most):
     for drafts in ("drawn", "chosen"):
