@@ -2093,7 +2093,6 @@ int op_paged_attention_int4(g950_module* m, const g950_view* views, uint32_t nvi
   return launch(m, "g950_attn_int4_general", (unsigned)rows, 64u, a, stream);
 }
 
-// --------------------------------------------------- norms around a block
 // ------------------------------------------------------------ drafted trees
 constexpr long long kTreeNodes = G950_TREE_NODES;
 static_assert(kTreeNodes == TREE_NODES, "the header's limit is the kernels'");
@@ -2346,7 +2345,8 @@ int op_paged_keep_path(g950_module* m, const g950_view* views, uint32_t nviews, 
     if (k.shape[d] != v.shape[d]) return fail(G950_USAGE, "%s: the caches differ in shape", op);
     if (k.shape[d] > (d < at ? 65536 : 0x7FFFFFFF)) return fail(G950_USAGE, "%s: extent too large", op);
   }
-  const long long layers = at ? k.shape[0] : 1, HK = k.shape[at + 2], D = k.shape[at + 3];
+  // (without layers there are no pages: seqused_out_ptr is written all the same)
+  const long long layers = at ? std::max((long long)k.shape[0], 1ll) : 1, HK = k.shape[at + 2], D = k.shape[at + 3];
   if (HK < 1 || D < 1 || HK > 65536 || D > 65536) return fail(G950_USAGE, "%s: extent empty or too large", op);
   if (k.shape[at + 1] < 1) return fail(G950_USAGE, "%s: pages of no keys", op);
   for (const View* w : {&k, &v}) {
@@ -2369,7 +2369,7 @@ int op_paged_keep_path(g950_module* m, const g950_view* views, uint32_t nviews, 
   a.v_l = at ? step(v, 0) : 0; a.v_p = step(v, at); a.v_r = step(v, at + 1); a.v_h = step(v, at + 2);
   a.table_s = table.stride[0]; a.path_z = path.stride[0]; a.count_z = count.stride[0]; a.out_z = out.stride[0];
   a.T = 0x7FFFFFFF; a.B = (int)B; a.L = (int)L; a.Hkv = (int)HK;
-  a.pages = (int)k.shape[at]; a.block_size = (int)k.shape[at + 1]; a.max_pages = (int)table.shape[1];
+  a.pages = at && !k.shape[0] ? 0 : (int)k.shape[at]; a.block_size = (int)k.shape[at + 1]; a.max_pages = (int)table.shape[1];
   // the widest word that every head's row is made of
   int word = k.isz;
   for (int w : {4, 16}) {
@@ -2385,6 +2385,7 @@ int op_paged_keep_path(g950_module* m, const g950_view* views, uint32_t nviews, 
   return launch(m, "g950_kv_keep_w" + std::to_string(word), (unsigned)(B * blocks * layers), 256u, a, stream);
 }
 
+// --------------------------------------------------- norms around a block
 int op_block_norm(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
                   void* stream) {
   if (nviews != 7 || nsc != 3)

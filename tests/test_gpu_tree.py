@@ -646,6 +646,16 @@ def test_keep_any_path():
         keep_check(c, "bfloat16")
 
 
+def test_keep_without_layers():
+    """Caches of no layers, and of no pages: the lengths are written."""
+    c = keep_case("trees", "bfloat16")
+    for shape in ((0, 4, 64, 2, 128), (0, 64, 2, 128)):
+        k = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+        used = ops.paged_keep_path(k, k.clone(), dev(c["table"]), dev(c["cu"]), dev(c["used"]), dev(c["path"]),
+                                   dev(c["count"]), sync=True)
+        assert used.cpu().tolist() == (c["used"] - np.diff(c["cu"]) + c["count"]).tolist()
+
+
 def test_keep_strides():
     for case, dt in (("trees", "bfloat16"), ("layers", "float32"), ("odd_d", "float16")):
         c = keep_case(case, dt)
