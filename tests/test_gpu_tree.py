@@ -813,3 +813,45 @@ def test_outputs_keep_to_their_streams():
         with pytest.raises(rt.G950Error):
             ops.paged_attention_tree(*bad, out=torch.empty_like(args[0]), lse=torch.empty((8, args[0].shape[0]), device="cuda"),
                                      workspace=torch.empty(0, device="cuda"))
+
+
+def test_offsets_past_32_bits():
+    """Pages and rows more than 2^31 elements in: the bits of the same calls on small tensors."""
+    dt, page, hk, d, far = "bfloat16", 64, 8, 128, 40000
+    c = attend_case(dict(ql=[26, 9], kl=[1500, 700], h=32, hk=hk, d=d, page=page), dt)
+    x = dev(np.random.default_rng(1).standard_normal((c["q"].shape[0], 32 + 2 * hk, d)).astype(np.float32), dt)
+    cos, sin = (dev(y) for y in rope(1500, d, np.random.default_rng(2)))
+    k = keep_case("trees", dt)
+    path, count = dev(k["path"][:2]), dev(k["count"][:2])
+    path[0, :3], count[0] = torch.tensor([0, 5, 9], dtype=torch.int32, device="cuda"), 3
+    path[1, :2], count[1] = torch.tensor([0, 8], dtype=torch.int32, device="cuda"), 2
+
+    def run(kc, vc, table):
+        q = ops.paged_append_tree(x[:, :32], x[:, 32:32 + hk], x[:, 32 + hk:], cos, sin, kc, vc, table, dev(c["cu"]),
+                                  dev(c["used"]), dev(c["parent"]))
+        o, lse = ops.paged_attention_tree(q, kc, vc, table, dev(c["cu"]), dev(c["used"]), dev(c["parent"]), 26, 1500)
+        left = ops.paged_keep_path(kc, vc, table, dev(c["cu"]), dev(c["used"]), path, count)
+        return q[:35], o[:35], lse[:, :35], left
+    small = [dev(c[n], dt) for n in ("k", "v")]
+    large = [torch.zeros((far + c["pool"], page, hk, d), dtype=T[dt], device="cuda") for _ in range(2)]
+    for a, b in zip(large, small):
+        a[far:] = b
+    table = dev(c["table"])
+    want, got = run(*small, table), run(*large, table + far)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for a, b in zip(large, small):
+        assert torch.equal(a[far:], b) and not a[:far].any()
+    del large
+    v, rows = 128000, 20000
+    w = dict(verify_case("large", "drawn", dt))
+    n = w["target"].shape[0]
+    want = verify_run(w, dt)
+    p, q = (torch.zeros((rows + n, v), dtype=T[dt], device="cuda") for _ in range(2))
+    p[rows:], q[rows:] = dev(w["target"], dt), dev(w["draft"], dt)
+    pad = lambda y: torch.cat([torch.zeros(rows, dtype=y.dtype, device="cuda"), y])  # noqa: E731
+    for ws in (None, torch.empty(0, device="cuda")):
+        got = ops.verify_tree(p, q, pad(dev(w["tokens"])), pad(dev(w["parent"])), pad(dev(w["u"])), dev(w["last"]),
+                              dev(w["cu"]) + rows, w["most"], workspace=ws, sync=True)
+        for a, b in zip(got, want):
+            assert np.array_equal(a.cpu().numpy(), b)
