@@ -236,6 +236,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
           }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          if (v0 - lane * N + 64 * N * u >= end) break;
           double r[N];
           left(wp[u], wq[u], v0 + 64 * N * u, end, r);
 #pragma unroll
@@ -394,6 +395,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long v = from + lane * N + 64 * N * u;
+      if (v - lane * N >= end) break;
       double r[N], s = 0.0;
       left(wp[u], wq[u], v, end, r);
 #pragma unroll
