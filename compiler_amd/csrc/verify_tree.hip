@@ -22,7 +22,11 @@
 // for their sum: a chain of passes over one pair of rows after the other (a megabyte each at
 // 128000 tokens in fp32), which one CU streams at some 100 GB/s.  So a sequence's columns are cut into
 // `parts`, one workgroup each, all of which follow the path on their own and tell each other
-// their sums.
+// their sums.  Bound by that chain: 2.9 us a refusal, 3.5 where 16 trees share the chip (waves'
+// sums, barriers, a store and a load past the L2); one workgroup takes 11 over 32000 columns in
+// fp32, 42 over 128000.  One tree of 26 nodes over 32000 columns 2.0 + 10.4 us (gather and parts), 16 of
+// 9 to 26 over 128000, siblings distinct, 4.0 + 25.5; 32 chosen ones over 50257 in bfloat16
+// 2.7 + 12.9.
 //   * A sum is told in one 64-bit word, by a relaxed atomic, in a place of its own for every
 //     (sequence, round, part); the launch before empties the places (a pattern that no sum
 //     has).  So nothing else needs to be ordered, and a place is never written twice with

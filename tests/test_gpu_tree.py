@@ -855,3 +855,27 @@ def test_offsets_past_32_bits():
                               dev(w["cu"]) + rows, w["most"], workspace=ws, sync=True)
         for a, b in zip(got, want):
             assert np.array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_empty_batches(dt):
+    """No sequences, no tokens, neither: nothing is written, and lengths and lists come out as they should."""
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    kc = torch.full((4, 16, 2, 64), 9.0, dtype=T[dt], device="cuda")
+    vc = kc.clone()
+    cos = sin = torch.ones((40, 32), device="cuda")
+    for b, t in ((0, 3), (2, 0), (0, 0), (2, 3)):
+        cu, used, parent = ints(*[0] * (b + 1)), ints(*[20] * b), ints(*[-1] * t)
+        table = torch.zeros((b, 4), dtype=torch.int32, device="cuda")
+        q, k, v = (torch.ones((t, n, 64), dtype=T[dt], device="cuda") for n in (4, 2, 2))
+        out = torch.full_like(q, 9.0)
+        ops.paged_append_tree(q, k, v, cos, sin, kc, vc, table, cu, used, parent, out=out)
+        o, lse = torch.full_like(q, 9.0), torch.full((4, t), 9.0, device="cuda")
+        ops.paged_attention_tree(q, kc, vc, table, cu, used, parent, 3, 800, out=o, lse=lse)
+        p = torch.full((t, 7), 1 / 7, dtype=T[dt], device="cuda")
+        path, count, nxt = ops.verify_tree(p, p, torch.zeros(t, dtype=torch.int64, device="cuda"), parent,
+                                           torch.zeros(t, device="cuda"), torch.zeros(b, device="cuda"), cu, 5)
+        left = ops.paged_keep_path(kc, vc, table, cu, used, path, count, sync=True)
+        assert all((x == 9.0).all() for x in (kc, vc, out, o, lse))
+        assert path.tolist() == [[-1] * 5] * b and count.tolist() == [0] * b and nxt.tolist() == [-1] * b
+        assert left.tolist() == [20] * b
