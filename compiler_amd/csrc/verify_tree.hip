@@ -22,11 +22,11 @@
 // for their sum: a chain of passes over one pair of rows after the other (a megabyte each at
 // 128000 tokens in fp32), which one CU streams at some 100 GB/s.  So a sequence's columns are cut into
 // `parts`, one workgroup each, all of which follow the path on their own and tell each other
-// their sums.  Bound by that chain: 2.9 us a refusal, 3.5 where 16 trees share the chip (waves'
+// their sums.  Bound by that chain: 2.8 us a refusal, 3.5 where 16 trees share the chip (waves'
 // sums, barriers, a store and a load past the L2); one workgroup takes 11 over 32000 columns in
-// fp32, 42 over 128000.  One tree of 26 nodes over 32000 columns 2.0 + 10.4 us (gather and parts), 16 of
-// 9 to 26 over 128000, siblings distinct, 4.0 + 25.5; 32 chosen ones over 50257 in bfloat16
-// 2.7 + 12.9.
+// fp32, 42 over 128000.  One tree of 26 nodes over 32000 columns 2.0 + 10.2 us (gather and parts), 16 of
+// 9 to 26 over 128000, siblings distinct, 4.1 + 24.9; 32 chosen ones over 50257 in bfloat16
+// 2.7 + 12.8.
 //   * A sum is told in one 64-bit word, by a relaxed atomic, in a place of its own for every
 //     (sequence, round, part); the launch before empties the places (a pattern that no sum
 //     has).  So nothing else needs to be ordered, and a place is never written twice with
@@ -119,7 +119,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
   __shared__ float us[TREE_NODES];
   __shared__ int tok[TREE_NODES], gone[TREE_NODES];
   __shared__ short par[TREE_NODES];
-  __shared__ double seg[VERIFY_WAVES], other[VERIFY_WAVES], scan[VERIFY_WAVES];
+  __shared__ double seg[2][VERIFY_WAVES], other[VERIFY_WAVES], scan[VERIFY_WAVES];
   __shared__ double upto[64];  // sum of the parts up to and with the one
   __shared__ unsigned long long missing;
   __shared__ int found, some;
@@ -221,6 +221,7 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
     const T* qr = Q + (long long)(b0 + cur) * a.d_row;
     const bool both = Q && A > 0.0;
     uint64_t todo = 1ull << part;
+    bool alone = false;  // some sums were not told
     for (bool own = true; todo; own = false) {
       const int of = __ffsll((unsigned long long)todo) - 1;
       todo &= todo - 1;
@@ -250,49 +251,57 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
       held = own && fits ? cur : -1;
       held_q = here ? held_q : both;
       t = verify_lane(verify_scan(t), 63);
-      __syncthreads();  // (whoever read the sums before is done)
-      if (lane == 0) (own ? seg : other)[wave] = t;
+      if (!own) __syncthreads();  // (whoever read the sums before is done)
+      if (lane == 0) (own ? seg[round & 1] : other)[wave] = t;
       __syncthreads();
       if (wave == 0) {
-        double t = 0.0;
+        t = 0.0;
 #pragma unroll
-        for (int w = 0; w < VERIFY_WAVES; ++w) t += (own ? seg : other)[w];
-        if (lane == 0) upto[of] = t;
-        if (PARTS && own) {
+        for (int w = 0; w < VERIFY_WAVES; ++w) t += (own ? seg[round & 1] : other)[w];
+        if (!PARTS || !own) {
+          if (lane == 0) upto[of] = t;
+        } else {
           // told, and the others' taken
           uint64_t* told = a.told + ((long long)z * VERIFY_TELL + round) * parts;
           const bool tell = round < VERIFY_TELL;
           if (tell && lane == 0)
             __hip_atomic_store(told + part, __builtin_bit_cast(uint64_t, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           bool have = lane == part || lane >= parts;
+          t = lane < parts ? t : 0.0;
           // (the first look about when the others' sums can be there: looks before that are in their
-          // way.  16 refusals in a row, one tree over 128000 columns: 56 us, 76 without this wait, 61 with
-          // twice as long a one; several looks on the way at a time 85)
+          // way.  16 refusals in a row, one tree over 128000 columns, took 76 us without this wait, 56 with
+          // it, 61 with one twice as long; with several looks on the way at a time 85)
           if (tell) __builtin_amdgcn_s_sleep(15);
           for (int spin = 0; tell && spin < VERIFY_SPINS && !__all(have); ++spin) {
             if (!have) {
               const uint64_t w = __hip_atomic_load(told + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
               have = w != VERIFY_EMPTY;
-              if (have) upto[lane] = __builtin_bit_cast(double, w);
+              if (have) t = __builtin_bit_cast(double, w);
             }
             __builtin_amdgcn_s_sleep(1);
           }
           const uint64_t none = __ballot(!have);
+          if (none == 0) t = verify_scan(t);
+          if (have && lane < parts) upto[lane] = t;
           if (lane == 0) missing = none;
         }
       }
       if (PARTS && own) {
         __syncthreads();
         todo = missing;
+        alone = todo != 0;
       }
     }
     ++round;
-    __syncthreads();
-    if (wave == 0) {
-      const double t = verify_scan(lane < parts ? upto[lane] : 0.0);
-      if (lane < parts) upto[lane] = t;
+    // (seg has two sides, so that a sum takes two barriers)
+    if (!PARTS || alone) __syncthreads();
+    if (PARTS && alone) {
+      if (wave == 0) {
+        const double t = verify_scan(lane < parts ? upto[lane] : 0.0);
+        if (lane < parts) upto[lane] = t;
+      }
+      __syncthreads();
     }
-    __syncthreads();
     S = upto[parts - 1];
   };
 
@@ -389,8 +398,9 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
   if (of != part) return;
   double start = verify_lane(below, of);
   int w = 0;
-  while (w + 1 < VERIFY_WAVES && !(start + seg[w] > want)) start += seg[w++];
-  while (w > 0 && !(seg[w] > 0.0)) start -= seg[--w];  // (a share past the end)
+  const double* waves = seg[(round - 1) & 1];
+  while (w + 1 < VERIFY_WAVES && !(start + waves[w] > want)) start += waves[w++];
+  while (w > 0 && !(waves[w] > 0.0)) start -= waves[--w];  // (a share past the end)
   long long from, end;
   bounds(part, w, from, end);
   if (held == cur) {  // the wave that has them
