@@ -53,9 +53,9 @@ DT_UINT32, DT_INT64, DT_UINT64, DT_F16, DT_BF16, DT_F32, DT_F64 = 7, 8, 9, 10, 1
 
 EXPORTS = ("g950_open", "g950_launch", "g950_launch_noalloc", "g950_workspace_bytes", "g950_validate",
            "g950_paged_attention_int4_workspace", "g950_paged_attention_tree_workspace",
-           "g950_verify_tree_workspace", "g950_last_kernel", "g950_last_form", "g950_sync", "g950_strerror", "g950_last_error", "g950_close", "g950_bundle_open", "g950_bundle_check", "g950_bundle_reason",
-           "g950_bundle_count", "g950_bundle_view", "g950_bundle_scalar", "g950_bundle_exec",
-           "g950_bundle_close")
+           "g950_verify_tree_workspace", "g950_last_kernel", "g950_last_form", "g950_sync", "g950_strerror",
+           "g950_last_error", "g950_close", "g950_bundle_open", "g950_bundle_check", "g950_bundle_reason",
+           "g950_bundle_count", "g950_bundle_view", "g950_bundle_scalar", "g950_bundle_exec", "g950_bundle_close")
 
 
 class G950Error(RuntimeError):

@@ -879,3 +879,50 @@ def test_empty_batches(dt):
         assert all((x == 9.0).all() for x in (kc, vc, out, o, lse))
         assert path.tolist() == [[-1] * 5] * b and count.tolist() == [0] * b and nxt.tolist() == [-1] * b
         assert left.tolist() == [20] * b
+
+
+@pytest.mark.parametrize("drafts", ["drawn", "chosen"])
+def test_verification_by_several_workgroups_at_once(drafts):
+    """Calls of many parts on streams of their own from several threads, beside two captured graphs
+    replayed in turn on new numbers: each the answers of its own inputs."""
+    cases = [verify_case("large", drafts, "float32", seed=s) for s in range(3)]
+    wants = [verify_run(c, "float32") for c in cases]
+    for c, w in zip(cases, wants):
+        verify_check(c, w)
+    names = ("target", "draft", "tokens", "parent", "u", "last", "cu")
+    inputs = [[None if c[n] is None else dev(c[n]) for n in names] for c in cases]
+    most = cases[0]["most"]
+    same = lambda got, want: all(np.array_equal(x.cpu().numpy(), y) for x, y in zip(got, want))  # noqa: E731
+    slots = [[None if x is None else x.clone() for x in inputs[0]] for _ in range(2)]
+    graphs = []
+    for slot in slots:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = ops.verify_tree(*slot, most)
+        graphs.append((g, got, slot))
+    assert rt.module().last_kernel == "g950_verify_tree_f32_parts"
+    errors = []
+
+    def work(i):
+        try:
+            s = own_stream(i)
+            for k in range(6):
+                got = ops.verify_tree(*inputs[(i + k) % 3], most, stream=s)
+                s.synchronize()
+                assert same(got, wants[(i + k) % 3])
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [t.start() for t in threads]
+    for k in range(6):
+        for n, (g, got, slot) in enumerate(graphs):
+            for x, y in zip(slot, inputs[(k + n) % 3]):
+                if x is not None:
+                    x.copy_(y)
+            g.replay()
+        torch.cuda.current_stream().synchronize()
+        for n, (g, got, slot) in enumerate(graphs):
+            assert same(got, wants[(k + n) % 3])
+    [t.join() for t in threads]
+    assert not errors, errors
