@@ -256,10 +256,8 @@ struct VerifyArgs {
   int token64, distinct;
   int parts;                // workgroups of a sequence, at most 64
   double* px;               // parts: [T][2] each node's probabilities after its parent
-  uint64_t* told;           // parts: [B][VERIFY_TELL][parts] sums
+  uint64_t* told;           // parts: [T][parts] sums, row by row of the sequences' nodes
 };
-// rounds of a sequence whose sums the workgroups tell each other
-constexpr int VERIFY_TELL = 32;
 
 // Attention over a paged cache of 4-bit rows (attn_int4.hip).
 struct AttnInt4Args {

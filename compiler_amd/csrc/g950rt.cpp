@@ -2245,8 +2245,10 @@ long long verify_parts(const g950_module* m, long long b, long long v) {
   const long long places = 2 * (m ? m->cus : 256);
   return b < 1 ? 1 : std::max(1ll, std::min({places / b, v / 2048, 64ll}));
 }
+// Places for a part's sums: one a node (and never below 32 a sequence).
+long long verify_places(long long b, long long t) { return std::max(t, 32 * b); }
 size_t verify_bytes(long long b, long long t, long long parts) {
-  return parts > 1 ? (size_t)(t * 16 + b * VERIFY_TELL * parts * 8) : 0;
+  return parts > 1 ? (size_t)(t * 16 + verify_places(b, t) * parts * 8) : 0;
 }
 
 int op_verify_tree(g950_module* m, const g950_view* views, uint32_t nviews, const g950_scalar* sc, uint32_t nsc,
@@ -2305,7 +2307,7 @@ int op_verify_tree(g950_module* m, const g950_view* views, uint32_t nviews, cons
   const std::string name = std::string("g950_verify_tree_") + rr_dtype(dt);
   // as many parts as the workspace has places for
   const long long room = (long long)ws.shape[0] * 4 - T * 16, want = verify_parts(m, B, V);
-  a.parts = (int)(B && room > 0 ? std::min(want, room / (B * VERIFY_TELL * 8)) : 1);
+  a.parts = (int)(B && room > 0 ? std::min(want, room / (verify_places(B, T) * 8)) : 1);
   if (a.parts < 2) {
     a.parts = 1;
     if (B > (long long)max_grid(256)) return fail(G950_USAGE, "%s: grid too large", op);

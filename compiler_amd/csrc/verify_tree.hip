@@ -26,14 +26,17 @@
 // sums, barriers, a store and a load past the L2); one workgroup takes 11 over 32000 columns in
 // fp32, 42 over 128000.  One tree of 26 nodes over 32000 columns 2.0 + 10.2 us (gather and parts), 16 of
 // 9 to 26 over 128000, siblings distinct, 4.1 + 24.9; 32 chosen ones over 50257 in bfloat16
-// 2.7 + 12.8.
+// 2.7 + 12.8.  60 refusals of one root in a row 171 us over 32000 columns as over 128000 (one workgroup
+// 714 and 2620), 120 of them 335.
 //   * A sum is told in one 64-bit word, by a relaxed atomic, in a place of its own for every
 //     (sequence, round, part); the launch before empties the places (a pattern that no sum
 //     has).  So nothing else needs to be ordered, and a place is never written twice with
-//     different values.
+//     different values.  A sequence of n nodes has n rounds at most: one
+//     for each node refused (never the root, and none twice) and one more where the path ends (where
+//     children are chosen: up to two there, and no others).
 //   * A workgroup waits for a sum for a bounded time only, then adds up that part itself,
 //     in the same order, to the same bits: no workgroup depends on another one's being on
-//     the chip.  (After TELL rounds it adds up all of them.)
+//     the chip.
 //   * The part in which the random number's share falls belongs to one workgroup, which
 //     finds the token.
 namespace g950 {
@@ -100,10 +103,10 @@ __device__ __forceinline__ int verify_nodes(const VerifyArgs& a, int z, int& b0)
 template <typename T>
 __device__ __forceinline__ void verify_gather_body(const VerifyArgs& a) {
   const int z = blockIdx.x;
-  uint64_t* told = a.told + (long long)z * VERIFY_TELL * a.parts;
-  for (int i = threadIdx.x; i < VERIFY_TELL * a.parts; i += 256) told[i] = VERIFY_EMPTY;
   int b0;
   const int n = verify_nodes(a, z, b0);
+  uint64_t* told = a.told + (long long)b0 * a.parts;
+  for (int i = threadIdx.x; i < n * a.parts; i += 256) told[i] = VERIFY_EMPTY;
   for (int i = threadIdx.x; i < n; i += 256) {
     int p, x;
     verify_node<T>(a, b0, i, p, x, a.px[2 * (long long)(b0 + i)], a.px[2 * (long long)(b0 + i) + 1]);
@@ -262,17 +265,16 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
           if (lane == 0) upto[of] = t;
         } else {
           // told, and the others' taken
-          uint64_t* told = a.told + ((long long)z * VERIFY_TELL + round) * parts;
-          const bool tell = round < VERIFY_TELL;
-          if (tell && lane == 0)
+          uint64_t* told = a.told + (long long)(b0 + round) * parts;
+          if (lane == 0)
             __hip_atomic_store(told + part, __builtin_bit_cast(uint64_t, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           bool have = lane == part || lane >= parts;
           t = lane < parts ? t : 0.0;
           // (the first look about when the others' sums can be there: looks before that are in their
           // way.  16 refusals in a row, one tree over 128000 columns, took 76 us without this wait, 56 with
           // it, 61 with one twice as long; with several looks on the way at a time 85)
-          if (tell) __builtin_amdgcn_s_sleep(15);
-          for (int spin = 0; tell && spin < VERIFY_SPINS && !__all(have); ++spin) {
+          __builtin_amdgcn_s_sleep(15);
+          for (int spin = 0; spin < VERIFY_SPINS && !__all(have); ++spin) {
             if (!have) {
               const uint64_t w = __hip_atomic_load(told + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
               have = w != VERIFY_EMPTY;
