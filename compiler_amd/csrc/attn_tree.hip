@@ -733,7 +733,7 @@ __device__ __forceinline__ void attn_tree_body(const AttnTreeArgs& p) {
     const bool empty = !(lt > 0.0f);  // zero or NaN
     const uint32_t at = row0 + tid, i = at / G, h = w.hk * G + at % G;
     if (w.rec >= 0) {
-      const long long rec = (long long)w.rec * ROWS + tid;
+      const long long rec = (long long)w.rec * p.merge_rows + tid;
       *(f32x2*)(p.ml + 2 * rec) = (f32x2){m, lt};
       place[tid] = rec * D;
     } else {
@@ -782,7 +782,7 @@ __device__ __forceinline__ void attn_tree_merge_body(const AttnTreeArgs& p) {
   const int rows = min(sp.sq.nq * p.group - block * ROWS, ROWS), count = (sp.n + d.c - 1) / d.c;
   if ((int)r0 >= rows || count <= 1) return;  // (one part: its workgroup had all of it)
   const int r = min((int)r0 + lane / LPR, rows - 1);
-  const long long rec = ((long long)d.before(z) * units + unit) * ROWS + r, step = (long long)units * ROWS;
+  const long long rec = ((long long)d.before(z) * units + unit) * p.merge_rows + r, step = (long long)units * p.merge_rows;
   const float* part = p.part + rec * D + lane % LPR * 4;
   const float* pair = p.ml + 2 * rec;
   float m = -__builtin_huge_valf(), l = 0.0f;

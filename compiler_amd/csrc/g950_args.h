@@ -233,10 +233,10 @@ struct AttnTreeArgs {
   int seqlen_q;             // nodes per sequence that take part
   int row_blocks;           // blocks of rows (node x head of the group) per (sequence, KV head)
   int parts;                // parts that the batch's keys are cut into at most; 0: one per sequence
-  int merge_rows;           // rows of a block that any sequence can have
+  int merge_rows;           // rows of a block that any sequence can have: those of a record
   int min_tiles;            // of 64 keys, of a part
-  float* part;              // [parts][row_blocks][Hkv][rows][D] unnormalised O
-  float* ml;                // [parts][row_blocks][Hkv][rows][2] maximum (log2 units), sum
+  float* part;              // [parts][row_blocks][Hkv][merge_rows][D] unnormalised O
+  float* ml;                // [parts][row_blocks][Hkv][merge_rows][2] maximum (log2 units), sum
 };
 
 // Verification of drafted trees (verify_tree.hip).

@@ -2114,6 +2114,7 @@ struct TreeShape {
   long long rw;          // 32-row tiles of a block
   long long row_blocks;  // per (sequence, KV head)
   long long units;       // blocks of a sequence
+  long long rows;        // of a block that any sequence can have
   long long parts;       // of the batch, wanted; 0: one per sequence
 };
 constexpr long long kTreePlaces = 2, kTreeFewRows = 32, kTreeFewPlaces = 6, kTreeMost = 128, kTreeOneRange = 512;
@@ -2126,6 +2127,7 @@ TreeShape tree_shape(const g950_module* m, long long b, long long h, long long h
   f.rw = rows <= 64 ? 2 : 4;
   f.row_blocks = (rows + 32 * f.rw - 1) / (32 * f.rw);
   f.units = hk * f.row_blocks;
+  f.rows = std::min(32 * f.rw, rows);
   const long long places = (rows <= kTreeFewRows ? kTreeFewPlaces : kTreePlaces) * cus;
   if (f.units && seqlen_k > kTreeOneRange && b * f.units < places)
     f.parts = std::min(std::max(places / f.units, 2 * b), kTreeMost * b);
@@ -2212,16 +2214,15 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
   if (fast && rows) {
     const TreeShape f = tree_shape(m, a.B, H, HK, D, std::min(SQ, T), SK);
     if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
-    const long long block_rows = 32 * f.rw;
     // as many parts as the workspace holds records for; one more than the sequences, or none
-    a.parts = (int)std::min(f.parts, ws.shape[0] / (f.units * block_rows * (D + 2)));
+    a.parts = (int)std::min(f.parts, ws.shape[0] / (f.units * f.rows * (D + 2)));
     if (a.parts <= a.B) a.parts = 0;
     a.min_tiles = kTreeMinTiles;
     a.seqlen_q = (int)std::min(SQ, T);
     a.row_blocks = (int)f.row_blocks;
-    a.merge_rows = (int)std::min(block_rows, std::min(SQ, T) * (H / HK));
+    a.merge_rows = (int)f.rows;
     a.part = (float*)ws.v->data;
-    a.ml = a.part + a.parts * f.units * block_rows * D;
+    a.ml = a.part + a.parts * f.units * f.rows * D;
     const long long grid = f.units * (a.parts ? a.parts : a.B);
     if (grid > 0x7FFFFFFF) return fail(G950_USAGE, "%s: grid too large", op);
     char name[64];
@@ -2637,7 +2638,7 @@ size_t g950_paged_attention_tree_workspace(g950_module* m, int64_t b, int64_t h,
       seqlen_q > kTreeNodes || seqlen_k > most || (d != 64 && d != 128 && d != 256))
     return 0;
   const TreeShape f = tree_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
-  return (size_t)(f.parts * f.units * 32 * f.rw * (d + 2)) * 4;
+  return (size_t)(f.parts * f.units * f.rows * (d + 2)) * 4;
 }
 
 size_t g950_verify_tree_workspace(g950_module* m, int64_t b, int64_t tokens, int64_t v) {
