@@ -42,7 +42,14 @@ __device__ __forceinline__ int tree_sequence(const int* cu, int B, int T, int t)
 
 // One wave per (node, head): any D, type, page size, stride and alignment.  Lanes take
 // keys for the scores, dims for O; keys are taken from the last to the first, so that the
-// way from the node to its root meets them in order.
+// way from the node to its root meets them in order.  Not tuned: every (node, head) reads its keys
+// by itself, each lane its own key's row value by value.  It is slower than the same formula in elementary torch
+// calls but for one tree.  In ms, 32 heads on 8, this kernel / torch: 26 nodes over 1000 keys, 16 trees of 9 to 32 over 300
+// to 4096, 32 single tokens over as many, 8 trees of 50 to 64 over 2049 to 8192
+//   bfloat16, d 96             0.64 / 0.79    8.2 / 1.9   4.1 / 2.0   22.9 / 2.8
+//   bfloat16, d 192            1.07 / 0.79   16.7 / 2.8   8.5 / 3.5   47.9 / 3.8
+//   bfloat16, d 128, pages of 10 0.72 / 0.79 10.5 / 2.2   5.7 / 2.5   29.3 / 3.1
+//   fp32, d 128                0.61 / 0.77    8.7 / 2.1   5.1 / 2.4   26.3 / 3.0
 __device__ __forceinline__ void attn_tree_general_body(const AttnTreeArgs& p) {
   __shared__ float qs[256];
   __shared__ float pr[64];
@@ -132,8 +139,8 @@ __device__ __forceinline__ void attn_tree_general_body(const AttnTreeArgs& p) {
 //     the softmax's running maximum and sum are per lane (two lanes a row).  Its keys 4 g .. + 3
 //     and 8 + 4 g .. + 3 of every 16 are the contraction slots that its own probabilities
 //     feed in O^T = V^T.P^T; V^T's fragments of the same keys come from transposing LDS reads.
-//   * K and V come by direct global->LDS DMA into a ring of stages, TKS keys each, issued NS
-//     stages ahead.  16-byte pieces are swizzled on the way (the source address is the
+//   * K and V come by direct global->LDS DMA into a ring of stages, TKS keys each, K two
+//     stages ahead and V one (d 256: both one).  16-byte pieces are swizzled on the way (the source address is the
 //     lane's): K's by the key, so that the 16 keys of a read lie in all 64 banks, V's
 //     by 64 bytes, so that the four keys of a transposing read do.
 //   * Stages are taken from the last to the first: the tree's keys come first, and a lane
@@ -143,13 +150,19 @@ __device__ __forceinline__ void attn_tree_general_body(const AttnTreeArgs& p) {
 //   * What a row does not see may hold anything: scores are replaced, and where V of a
 //     stage that some row does not see whole is not finite, 0 V would not be 0: such values
 //     are added, key by key, where a row sees them, and taken out of the stage.
+//   * A probability is rounded to the operands' type, once, for P.V (half a step of itself; the sum l and O
+//     stay in fp32): exact products would take a second 16-bit term and P.V's MFMAs twice.  O's
+//     distance from the formula's is 0.0023 of it in bfloat16 (root mean squares; 0.0017 of that
+//     is the rounding of O), 0.00028 in float16 (0.0002).
 // Bound by K and V for few rows, by the matrix cores and the softmax's vector ALU from 64 rows
 // on, and for short batches by a start of some 8 us (dealing the keys 1.6, queries, parents and
 // page table 1.8, the first K 1.9, its scores and the way up the tree 2.3) with 3 behind the last
-// stage.  bfloat16, d 128, 32 heads on 8, parts + joining: 32 single tokens over 300 to 4096 keys
-// 65 + 5.5 us (4.4 TB/s), 16 trees of 9 to 32 nodes over as many 43 + 10, 8 of 50 to 64 over 2049 to 8192
-// 63 + 11 (39 GFLOP); 64 trees of 32 over 8192 380 in all (5.7 TB/s), of 64 540 to 730 (0.8
-// to 1.0 PFLOP/s).  512 threads a workgroup, halves taking turns on the matrix cores: 52 to 58 in
+// stage.  32 heads on 8 in bfloat16, parts + joining: 32 single tokens over 300 to 4096 keys
+// 64 + 5.3 us at d 128 (4.5 TB/s), 38 + 5 at 64, 140 + 6.4 at 256; 16 trees of 9 to 32 nodes over as many 42 + 10, 23 + 6,
+// 95 + 17; 8 of 50 to 64 over 2049 to 8192 61 + 11 (39 GFLOP) at d 128, 178 + 18 at 256; 64 trees of 32 over
+// 8192 390 in all (5.5 TB/s), of 64 565 to 640 (0.86 to 0.97 PFLOP/s).  The way up is walked node by node: one
+// chain of 64 nodes over 4096 keys 32 where as many children of one root take 29, of 1024 149 and 100; 16 chains
+// of 1024 1320 and 1100.  512 threads a workgroup, halves taking turns on the matrix cores: 52 to 58 in
 // place of 43, 780 to 880 in place of 540 to 730.
 
 struct TreeSpan {

@@ -2101,11 +2101,13 @@ static_assert(kTreeNodes == TREE_NODES, "the header's limit is the kernels'");
 // (sequence, KV head), and parts of the batch's keys, whose records need a workspace.  The lengths are the
 // device's: parts are dealt there, all of about one length.
 // Measured at d 128 in bfloat16, 32 query heads on 8 KV heads, us for the parts + for joining them:
-//   * Parts for two workgroups per CU, as many as are resident; for up to 32 rows, whose
+//   * Parts for two workgroups per CU, as many as are resident (at d 256 one is, and one's parts and two's
+//     take the same: 16 trees 109 and 112 in all, 8 wide ones 199 and 197); for up to 32 rows, whose
 //     records are small, six, which end together more evenly.  16 trees of 9 to 32 nodes over 300
 //     to 4096 keys 43 + 9 with two, 49 + 11 with three, 52 + 14 with four, 58 + 7 with one; 8 of
 //     50 to 64 over 2049 to 8192 63 + 10, 76 + 12, 71 + 14, 117 + 7; 32 single tokens over 300 to
-//     4096 74 + 5 with two, 64 + 5 with four, 62 + 5 with six, 63 + 6 with eight.
+//     4096 74 + 5 with two, 64 + 5 with four, 62 + 5 with six, 63 + 6 with eight.  (The same inputs again
+//     and again, which the MALL holds in part: 58, 57 and 60 in all with two, four and six.)
 //   * Parts of 128 keys or more: one tree of 26 nodes behind 974 keys 12.4 + 4.8, 14.3 + 4.6 with
 //     256, 18.8 + 4.6 with 512.  At most 128 a sequence: two of 50001 and 65537 keys (d 64, one
 //     KV head) 17.1 + 6.4, with 256 15.9 + 8.5.
@@ -2120,8 +2122,7 @@ struct TreeShape {
 constexpr long long kTreePlaces = 2, kTreeFewRows = 32, kTreeFewPlaces = 6, kTreeMost = 128, kTreeOneRange = 512;
 constexpr int kTreeMinTiles = 2;
 
-TreeShape tree_shape(const g950_module* m, long long b, long long h, long long hk, long long d, long long seqlen_q,
-                     long long seqlen_k) {
+TreeShape tree_shape(const g950_module* m, long long b, long long h, long long hk, long long seqlen_q, long long seqlen_k) {
   const long long cus = m ? m->cus : 256, rows = seqlen_q * (h / hk);
   TreeShape f{};
   f.rw = rows <= 64 ? 2 : 4;
@@ -2212,7 +2213,7 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
                     aligned16(q.addr()) && a.q_st % 8 == 0 && a.q_sh % 8 == 0 && o.addr() % 8 == 0 && a.o_st % 4 == 0 &&
                     a.o_sh % 4 == 0;
   if (fast && rows) {
-    const TreeShape f = tree_shape(m, a.B, H, HK, D, std::min(SQ, T), SK);
+    const TreeShape f = tree_shape(m, a.B, H, HK, std::min(SQ, T), SK);
     if (ws.shape[0] && !aligned16(ws.addr())) return fail(G950_USAGE, "%s: workspace_ptr must be 16-byte aligned", op);
     // as many parts as the workspace holds records for; one more than the sequences, or none
     a.parts = (int)std::min(f.parts, ws.shape[0] / (f.units * f.rows * (D + 2)));
@@ -2239,14 +2240,16 @@ int op_paged_attention_tree(g950_module* m, const g950_view* views, uint32_t nvi
   return launch(m, "g950_attn_tree_general", (unsigned)rows, 64u, a, stream);
 }
 
-// Workgroups of a sequence: two for every CU, with 2048 columns each at least (16 trees over
-// 128000 tokens: 32.7 us with two, 35.4 with one, 38 with four; one over 32000 tokens: 13.7 with 1024,
-// 2048 or 4096 columns).
+// Workgroups of a sequence: two for every CU, with 2048 columns each at least.  A call, the same inputs again and
+// again: 16 trees over 128000 columns 15.1 us with 32 each (two a CU), 21.8 with 16, 31.5 with 8; one over 32000
+// 11.0 with 15 (2048 columns), 14.7 with 7, 16.3 with 3.  (Four a CU were slower than two when last tried, 38 us
+// where two took 32.7, by a form of the kernel with four barriers a sum.)
 long long verify_parts(const g950_module* m, long long b, long long v) {
   const long long places = 2 * (m ? m->cus : 256);
   return b < 1 ? 1 : std::max(1ll, std::min({places / b, v / 2048, 64ll}));
 }
-// Places for a part's sums: one a node (and never below 32 a sequence).
+// Places for a part's sums: one a node, and 32 a sequence at least, so that workspaces of that length, enough
+// for trees of up to 32 nodes, serve them in full.
 long long verify_places(long long b, long long t) { return std::max(t, 32 * b); }
 size_t verify_bytes(long long b, long long t, long long parts) {
   return parts > 1 ? (size_t)(t * 16 + verify_places(b, t) * parts * 8) : 0;
@@ -2637,7 +2640,7 @@ size_t g950_paged_attention_tree_workspace(g950_module* m, int64_t b, int64_t h,
   if (b <= 0 || hk <= 0 || h < hk || h % hk || seqlen_q <= 0 || seqlen_k <= 0 || b > most || h > 65536 ||
       seqlen_q > kTreeNodes || seqlen_k > most || (d != 64 && d != 128 && d != 256))
     return 0;
-  const TreeShape f = tree_shape(m, b, h, hk, d, seqlen_q, seqlen_k);
+  const TreeShape f = tree_shape(m, b, h, hk, seqlen_q, seqlen_k);
   return (size_t)(f.parts * f.units * f.rows * (d + 2)) * 4;
 }
 

@@ -24,9 +24,11 @@
 // `parts`, one workgroup each, all of which follow the path on their own and tell each other
 // their sums.  Bound by that chain: 2.8 us a refusal, 3.5 where 16 trees share the chip (waves'
 // sums, barriers, a store and a load past the L2); one workgroup takes 11 over 32000 columns in
-// fp32, 42 over 128000.  One tree of 26 nodes over 32000 columns 2.0 + 10.2 us (gather and parts), 16 of
-// 9 to 26 over 128000, siblings distinct, 4.1 + 24.9; 32 chosen ones over 50257 in bfloat16
-// 2.7 + 12.8.  60 refusals of one root in a row 171 us over 32000 columns as over 128000 (one workgroup
+// fp32, 42 over 128000.  One tree of 26 nodes over 32000 columns 1.7 + 9.8 us (gather and parts), 16 of
+// 9 to 26 over 128000, siblings distinct, 4.0 + 24.8; 32 chosen ones over 50257 in bfloat16 2.6 + 12.6, by time stamps in a
+// workgroup, each tree's mean: nodes 0.7, walk 2.6 (the longest path's 5), rows 2.4, sums told and taken 1.6, the
+// token 0.7; the last tree's is there 11 after the first workgroup's start.  Rows of which a wave's share is more
+// than 1024 fp32 columns are read again for every sum: 32 trees over 128000 4.8 + 51, 16 over 151936 4.8 + 33.  60 refusals of one root in a row 171 us over 32000 columns as over 128000 (one workgroup
 // 714 and 2620), 120 of them 335.
 //   * A sum is told in one 64-bit word, by a relaxed atomic, in a place of its own for every
 //     (sequence, round, part); the launch before empties the places (a pattern that no sum
@@ -210,8 +212,8 @@ __device__ __forceinline__ void verify_tree_body(const VerifyArgs& a) {
     from = min(of * len + w * share, end);
     to = min(from + share, end);
   };
-  // A wave's share of up to U vectors of each row stays in registers: the next sum of the
-  // same node and the search for the token need no loads.
+  // A wave's share of up to U vectors a lane of each row stays in registers: the next sum of the
+  // same node and the search for the token need no loads.  (Longer shares are read again.)
   constexpr int U = 4;
   const bool fits = share <= 64 * N * U;
   u32x4 wp[U], wq[U];

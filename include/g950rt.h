@@ -294,7 +294,8 @@ typedef struct g950_scalar {
  *           f32 | bf16 | f16 (draft the same), tokens_ptr[T] i32 | i64 (next the same),
  *           uniform_next_ptr f32[B], uniform_ptr f32[T], workspace_ptr f32 (1-D, 16-byte
  *           aligned, any length: g950_verify_tree_workspace gives the one that serves all; calls
- *           that may overlap need one each).  A sequence without nodes: count 0, path and next -1
+ *           that may overlap need one each).  A sequence without nodes: count 0, path and next -1.
+ *           Of sequences with rows in common (a cu_seqlens_q_ptr that falls) the answers are undefined
  *   scalars distinct
  * G950_OP_PAGED_KEEP_PATH  the path's rows moved to where its tokens belong: cache row base
  *                      + i gets what row base + path[b,i] held, for i < count[b] and i <=
@@ -398,7 +399,8 @@ size_t g950_paged_attention_tree_workspace(g950_module *module, int64_t b, int64
                                            int64_t seqlen_q, int64_t seqlen_k);
 
 /* Bytes of workspace_ptr with which G950_OP_VERIFY_TREE has a sequence's columns
- * added up by as many workgroups as pays: b trees of `tokens` nodes in all, v columns. */
+ * added up by as many workgroups as pays: b trees of `tokens` nodes in all, v columns.
+ * (16 bytes a node, and 8 a node, 32 a tree at least, for each workgroup of a tree.) */
 size_t g950_verify_tree_workspace(g950_module *module, int64_t b, int64_t tokens, int64_t v);
 
 /* Run every contract check and the kernel choice of g950_launch without
